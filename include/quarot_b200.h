@@ -272,6 +272,60 @@ int qr_kv_decode_i4(void* o, const void* q, const void* kv_data, const void* kv_
                     const int32_t* kv_indices, const int32_t* last_page_offset, int batch, int num_layers, int layer,
                     int num_heads, int page_size, int head_dim, int hadamard_q, void* stream);
 
+/* The operators below have no upstream counterpart (upstream refuses sequences with different page counts,
+ * quarot/transformers/kv_cache.py:214-216, attends one new token at a time, :104-112, and has no window); they work on
+ * the layout above.
+ *
+ * qr_kv_page_table: page table and slot map of a step from request lengths, in one launch and without a host read.
+ *   seq_lens [batch]   cached tokens before the step
+ *   new_lens [batch]   tokens that the step adds, or NULL: one each
+ *   block_table [batch, max_blocks]  pages of the sequences in order, or NULL: page j of sequence b is j * batch + b
+ *   free_pages [num_free]  pages handed out, in the order of the sequences, to those that need more; the block table
+ *                      gets them.  num_free < 0: nothing is handed out, the block table holds the pages already.
+ * Writes
+ *   kv_indptr [batch + 1], kv_indices [batch * max_blocks] (entries behind the last page: -1), last_page_offset [batch]:
+ *                      the sequences WITH the new tokens, as the other calls take them
+ *   append_indptr [batch + 1]  prefix sum of new_lens (also the qo_indptr of qr_kv_attend_i4)
+ *   slot_map, positions [new_tokens]  page * page_size + slot and position in its sequence of every new token
+ *   seq_lens_out [batch], status [2] = (free pages taken, sequences refused)
+ * A sequence whose row of the block table, the free list or the new_tokens rows cannot hold its new tokens is refused: it
+ * keeps its old length, takes no page, and its tokens get slot and position -1.  Sequences are served in order; once the
+ * free list has run out every later sequence that needs a page is refused.  new_tokens may exceed the sum of new_lens
+ * (a padded batch): the rows behind get -1.  Negative lengths count as 0.  Outputs must not overlap inputs.
+ * batch <= 8192 and batch * max_blocks < 2^31 (QR_EUNSUPPORTED otherwise). */
+int qr_kv_page_table(const int32_t* seq_lens, const int32_t* new_lens, int batch, int64_t new_tokens, int page_size,
+                     int max_blocks, int32_t* block_table, const int32_t* free_pages, int64_t num_free,
+                     int32_t* kv_indptr, int32_t* kv_indices, int32_t* last_page_offset, int32_t* append_indptr,
+                     int64_t* slot_map, int32_t* positions, int32_t* seq_lens_out, int32_t* status, void* stream);
+
+/* qr_kv_append_slots_i4: qr_kv_append_i4 with the page slots taken from a slot map (qr_kv_page_table): the same bytes in
+ * the same places.  A token whose slot lies outside the pool (-1 among others) is left out.  k and v [tokens, heads,
+ * head_dim] fp16 with strides in elements (multiples of 4; the last axis is contiguous, 8-byte aligned). */
+int qr_kv_append_slots_i4(void* kv_data, void* kv_param, int64_t num_pages, const int64_t* slot_map, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, int64_t tokens, int num_layers, int layer, int num_heads, int page_size,
+                          int head_dim, int hadamard_k, void* stream);
+
+/* qr_kv_attend_i4: attention of the last new tokens of every sequence over the cache, which already holds them:
+ *   o[i, h] = sum_t softmax_t(q[i, h] . K[t, h / g] / sqrt(head_dim)) V[t, h / g],   g = num_q_heads / num_kv_heads,
+ * for the new tokens i of sequence b, rows qo_indptr[b] .. qo_indptr[b + 1] of q and o; token i of n stands at position
+ * P = length - n + i and sees t <= P; with window > 0 only t > P - window and the first sink_tokens tokens.  A row that
+ * sees nothing gives zeros.  qo_indptr NULL: one new token per sequence (total_q == batch, max_q_len == 1).
+ *   q, o [total_q, num_q_heads, head_dim] fp16 with strides in elements (multiples of 4; last axis contiguous, 8-byte
+ *   aligned); total_q rows exist, a sequence whose rows lie beyond them is left out, as are rows that belong to none.
+ *   max_q_len: an upper bound of the new tokens of any sequence (it sets the grid and chooses the kernel; rows of a
+ *   sequence beyond it may be left unwritten).  kv_indices outside 0 .. num_pages - 1 read the last page.
+ *   hadamard_q: the query is Walsh-Hadamard transformed (and rounded to fp16) first.
+ * Scales are positive, as qr_kv_append_i4 writes them; what lies in tokens that a row does not see, infinities and NaN
+ * among it, does not reach it.  The sums are in fp32; the softmax weights, with the value scale in them, are rounded to
+ * fp16 for the tensor cores, the codes are exact.  Same result from call to call. */
+int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, const void* q, int64_t q_token_stride,
+                    int64_t q_head_stride, const void* kv_data, const void* kv_param, int64_t num_pages,
+                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_offset,
+                    const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
+                    int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
+                    int hadamard_q, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

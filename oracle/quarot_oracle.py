@@ -254,3 +254,115 @@ def paged_decode_attention(q, pages, params, layer, kv_indptr, kv_indices, last_
         p = torch.softmax(s, dim=-1)
         outs.append(torch.einsum("ht,thd->hd", p, v))
     return torch.stack(outs, 0)
+
+
+def kv_hadamard_fp16(x):
+    """The rotated query as the kernels hold it: Walsh-Hadamard butterflies over 128 values in fp32 with the strides 1, 2,
+    4 .. 64, times fp32(1 / sqrt(128)), rounded to fp16.  Sums and differences of fp32 numbers, so it is exact to the bit."""
+    y = x.float()
+    n, h = x.shape[-1], 1
+    while h < n:
+        y = y.view(*x.shape[:-1], n // (2 * h), 2, h)
+        y = torch.stack((y[..., 0, :] + y[..., 1, :], y[..., 0, :] - y[..., 1, :]), -2).reshape(x.shape)
+        h *= 2
+    return (y * torch.tensor(0.08838834764831845, dtype=torch.float32)).half()
+
+
+def kv_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, free_pages=None, max_blocks=None):
+    """Page table and slot map of a step, sequence by sequence (lists in, dict of lists out; block_table is updated)."""
+    batch = len(seq_lens)
+    width = len(block_table[0]) if block_table is not None else max_blocks
+    pages = lambda n: -(-n // page_size)  # noqa: E731
+    out = dict(kv_indptr=[0], kv_indices=[], last_page_offset=[], append_indptr=[0], seq_lens=[],
+               slot_map=[-1] * new_tokens, positions=[-1] * new_tokens)
+    wanted = taken = refused = 0
+    for b in range(batch):
+        old, new = min(max(seq_lens[b], 0), width * page_size), max(new_lens[b], 0)
+        row = out["append_indptr"][-1]
+        out["append_indptr"].append(row + new)
+        ok = new == 0 or (pages(old + new) <= width and row + new <= new_tokens)
+        if ok and block_table is not None and free_pages is not None:
+            need = pages(old + new) - pages(old)
+            first = wanted
+            wanted += need
+            if need and wanted > len(free_pages):
+                ok = False
+            else:
+                block_table[b][pages(old):pages(old) + need] = free_pages[first:first + need]
+                taken += need
+        refused += not ok
+        after = old + new if ok else old
+        mine = [block_table[b][j] if block_table is not None else j * batch + b for j in range(pages(after))]
+        out["kv_indices"] += mine
+        out["kv_indptr"].append(len(out["kv_indices"]))
+        out["seq_lens"].append(after)
+        out["last_page_offset"].append(after - max(len(mine) - 1, 0) * page_size)
+        for i in range(new if ok else 0):
+            pos = old + i
+            slot = mine[pos // page_size] * page_size + pos % page_size
+            out["slot_map"][row + i], out["positions"][row + i] = max(slot, -1), pos
+    out["kv_indices"] += [-1] * (batch * width - len(out["kv_indices"]))
+    out["status"] = [taken, refused]
+    return out
+
+
+def paged_attention(q, pages, params, layer, kv_indptr, kv_indices, last_page_offset, qo_indptr, window=0, sinks=0):
+    """Causal attention of the last new tokens of every sequence over the paged cache, in fp64, row by row of the
+    definition; query head h reads KV head h // group, window > 0: only the last `window` tokens and the first `sinks`.
+
+    q [tokens, heads, d] -> (o fp64 [tokens, heads, d], bound fp64): |result - o| <= bound holds for an evaluation that
+      * rounds the result to fp16 (2^-11 |o|, 2^-25 below the normal numbers),
+      * rounds softmax weights times value scale to fp16, relative to the largest of them: 2^-11 for each (2^-25 of the
+        largest where that is more), against values c - 7.5 of the centred codes (at most 7.5 scales from the centre),
+      * has scores that are off by at most e_t = 2^-19 (31 |s_t| sum|q| + |z_t| |sum q|) / sqrt(d): products of a query with
+        codes 16 + c <= 31 summed in fp32 (128 terms and the corrections, each off by 2^-23 of the sum of magnitudes at
+        most), which changes weight t by the factor exp(e_t): sum p_t (exp(e_t) - 1) |v_t - o|, twice for the denominator's
+        own change,
+      * sums and joins everything else in fp32: 2^-18 of the largest magnitude.
+    A row that sees nothing is 0."""
+    d, heads = q.shape[-1], q.shape[1]
+    page_size, kv_heads = pages.shape[4], pages.shape[3]
+    group = heads // kv_heads
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    bound = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(len(last_page_offset)):
+        first, last = int(kv_indptr[b]), int(kv_indptr[b + 1])
+        r0, r1 = int(qo_indptr[b]), int(qo_indptr[b + 1])
+        n = (last - first - 1) * page_size + int(last_page_offset[b]) if last > first else 0
+        if n <= 0 or r1 <= r0:
+            continue
+        mine = kv_indices[first:last].long()
+        pos = torch.arange(n - (r1 - r0), n).view(-1, 1)
+        t = torch.arange(n).view(1, -1)
+        see = t <= pos
+        if window > 0:
+            see &= (t > pos - window) | (t < sinks)
+        for h in range(kv_heads):
+            kv, codes, par = [], [], []
+            for which in (0, 1):
+                data = pages[mine, layer, which, h].reshape(-1, d // 2)[:n]
+                pr = params[mine, layer, which, h].reshape(-1, 2)[:n].double()
+                cc = torch.stack((data & 0x0F, data >> 4), -1).reshape(n, d).double()
+                codes.append(cc)
+                par.append(pr)
+                kv.append(cc * pr[:, :1] - pr[:, 1:])
+            for e in range(h * group, (h + 1) * group):
+                qq = q[r0:r1, e].double()
+                for i in range(r1 - r0):
+                    vis = see[i]
+                    if not bool(vis.any()):
+                        continue
+                    k, v, s = kv[0][vis], kv[1][vis], par[1][vis, :1]
+                    sc = (k @ qq[i]) / math.sqrt(d)
+                    p = torch.exp(sc - sc.max())
+                    p = p / p.sum()
+                    o = p @ v
+                    out[r0 + i, e] = o
+                    kp = par[0][vis]
+                    es = (2.0 ** -19 * (31 * kp[:, 0].abs() * qq[i].abs().sum() + kp[:, 1].abs() * qq[i].sum().abs()) / math.sqrt(d))
+                    w = p[:, None] * s
+                    off = (codes[1][vis] - 7.5).abs()
+                    rounding = torch.maximum(2.0 ** -11 * w, 2.0 ** -25 * w.max())
+                    bound[r0 + i, e] = ((2.0 ** -11 * o.abs()).clamp(min=2.0 ** -25) + (rounding * off).sum(0)
+                                        + 2 * ((p * torch.expm1(es))[:, None] * (v - o).abs()).sum(0) + 2.0 ** -18 * v.abs().max())
+    return out, bound

@@ -1,0 +1,520 @@
+// Attention over the paged 4-bit cache for few query rows per KV head (decode, drafted tokens, short chunks; any number
+// of rows is right, 8 to 32 at a time).  Causal, with an optional sliding window and sink tokens, grouped query heads.
+//
+// Mathematics.  With key codes c, scale s and zero z per (token, head), the score of row r and token t is
+//   s_t <q_r, c_t> - z_t sum(q_r),   and value = s' c' - z'  (s', z' the value parameters).
+// The tensor cores see only small whole numbers: a code is put into the mantissa of 16.0 (fp16 0x4C00 | c << 6 is exactly
+// 16 + c), two logical instructions per pair of codes and no arithmetic, and the 16 is taken out of the sums in fp32.
+// Weights: w_t = exp2(score_t + log2 s'_t - M) with M the running maximum of that exponent, so that the value scale is
+// inside the weight, the largest weight is 1 and rounding w to fp16 (the B operand of the second product) is a relative
+// error of at most 2^-11 / 2 for every token that matters; the sums
+//   l = sum w / s'_t  (the softmax denominator)  and  y = sum w (z'_t / s'_t - 7.5)
+// are of the unrounded w in fp32, and the centre 7.5 of the codes is taken out with the ROUNDED weights (one more MMA
+// row of ones), so that a rounding error of w meets c' - 7.5 and not 16 + c':
+//   o = (sum w~ (16 + c') - 23.5 sum w~ - y) / l.
+//
+// Mapping.  A warp takes blocks of 32 tokens.  Scores: S^T = K Q^T with mma.m16n8k16, 16 tokens as M, 8 rows as N; lane
+// (g, c) = (lane / 4, lane % 4) reads 16 bytes of each of its token rows (32 codes), and since the order of the 128
+// dimensions is free as long as the query follows it, nibbles j and j + 4 of a word are a fragment register as they
+// stand.  Weights: S^T leaves the tensor core as (token, row) pairs and movmatrix turns it into the B operand (tokens as
+// K).  Values: O^T = V^T w, dimensions as M; a fragment register holds two tokens of one dimension, made by one byte
+// permute per four of them.  Which token sits in which fragment row is free too and is chosen so that all reads of the
+// shared-memory ring are free of bank conflicts.  Warps keep their own softmax state and are merged through shared
+// memory; few (tile, head) pairs: a cluster shares the token axis and is merged through distributed shared memory.
+// Every warp has its own ring of cp.async stages, so no barrier runs inside the loop.
+// What bounds it: reading 136 bytes per (token, KV head) once per tile of rows.
+#include "kv_common.cuh"
+
+#include <math.h>
+
+namespace qr {
+
+constexpr int kRwWarps = 8;
+constexpr int kRwStages = 4;
+constexpr int kRwTok = 32;                              // tokens per block
+constexpr int kRwStageBytes = kRwTok * (64 + 64 + 4 + 4);
+constexpr int kRwRing = kRwWarps * kRwStages * kRwStageBytes;
+constexpr int kRwORow = kHeadDim + 4;                   // floats per row of the merge buffers
+
+template <int NT>
+struct RwShared {
+  __half q[8 * NT][kHeadDim];                           // rows in fragment order
+  float qsum[8 * NT];
+  int pos[8 * NT];                                      // position of the row, -1: not a row
+  float m[kRwWarps][8 * NT], l[kRwWarps][8 * NT];
+  float part_m[8 * NT], part_l[8 * NT];
+  float part_o[8 * NT][kHeadDim];
+};
+
+__device__ __forceinline__ void rw_cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void rw_cp4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void rw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void rw_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// nibbles J and J + 4 of a word as the fp16 pair (16 + c_J, 16 + c_{J+4})
+template <int J>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  const uint32_t x = J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6;
+  return (x & 0x03C003C0u) | 0x4C004C00u;
+}
+
+// Row of a block's stage that holds 64 bytes of codes: 16-byte chunk ch of row r lies at chunk ch ^ rw_swz(r).
+__device__ __forceinline__ int rw_swz(int r) { return (r & 2); }
+// Token of a 16-token tile in fragment slot s: the four tokens that a V fragment reads at once, and the two of a K
+// fragment, differ in the bank halves that their rows start in.
+__device__ __forceinline__ int rw_token_even(int c) { return c; }              // slot 2 c
+__device__ __forceinline__ int rw_token_odd(int c) { return 4 + (c ^ 1); }     // slot 2 c + 1
+
+__device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void rw_store_row(const KvAttendParams& p, const KvTile& w, int head_kv, int r, int d4, float4 v, float inv) {
+  const int row = w.row0 + r;
+  const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
+  const __half2 h0 = __floats2half2_rn(v.x * inv, v.y * inv), h1 = __floats2half2_rn(v.z * inv, v.w * inv);
+  uint2 out;
+  out.x = *reinterpret_cast<const uint32_t*>(&h0);
+  out.y = *reinterpret_cast<const uint32_t*>(&h1);
+  *reinterpret_cast<uint2*>(p.o + (w.tok0 + tok) * p.o_ts + (int64_t)(head_kv * p.group + hh) * p.o_hs + d4) = out;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(32 * kRwWarps, 1)
+kv_attend_rows_kernel(const KvAttendParams p) {
+  constexpr int R = 8 * NT;
+  extern __shared__ __align__(128) unsigned char s_dyn[];
+  unsigned char* ring = s_dyn;
+  RwShared<NT>& sh = *reinterpret_cast<RwShared<NT>*>(s_dyn + kRwRing);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int unit = blockIdx.x / p.splits;
+  uint32_t crank = 0;
+  if (p.splits > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  const int head_kv = unit % p.kv_heads;
+  const KvTile w = kv_find_tile(p, unit / p.kv_heads, R, lane);
+  if (w.rows == 0) return;                              // the whole cluster has the same tile
+
+  for (int r = warp; r < R; r += kRwWarps) {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int pos = -1;
+    if (r < w.rows) {
+      const int row = w.row0 + r;
+      const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
+      pos = w.pos0 + tok;
+      load4_f16(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane, x);
+      if (p.hadamard_q) {
+        fwht128_warp(x, lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
+      }
+    }
+    float sum = x[0] + x[1] + x[2] + x[3];
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    // dimension d = 32 cc + 8 wi + e sits in register (2 wi + e % 4 / 2, e % 2), half e / 4, of lane column cc
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const int d = 4 * lane + e4, e = d & 7;
+      sh.q[r][(d >> 5) * 32 + ((d >> 3) & 3) * 8 + (e & 3) * 2 + (e >> 2)] = __float2half_rn(x[e4]);
+    }
+    if (lane == 0) { sh.qsum[r] = sum; sh.pos[r] = pos; }
+  }
+  __syncthreads();
+
+  uint32_t qf[NT][16];
+  float qs[NT][2];
+  int ps[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * i]);
+      qf[n][4 * i] = u.x; qf[n][4 * i + 1] = u.y; qf[n][4 * i + 2] = u.z; qf[n][4 * i + 3] = u.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; ps[n][k] = sh.pos[8 * n + 2 * c + k]; }
+  }
+  const int last_row = w.row0 + w.rows - 1;
+  const int p_min = w.pos0 + fast_div(w.row0, p.group_div), p_max = w.pos0 + fast_div(last_row, p.group_div);
+  const KvBlocks blk = kv_blocks<kRwTok>(p_min, p_max, p.window, p.sinks);
+  // the CTAs of a cluster take contiguous ranges of blocks, the warps of a CTA every eighth one
+  const int per = (blk.count + p.splits - 1) / p.splits;
+  const int begin = (int)crank * per + warp, end = min((int)(crank + 1) * per, blk.count);
+
+  const int first_page = p.indptr[w.b];
+  const int tokens = min(p_max + 1, w.seq_len);         // tokens from here on are not read
+  const size_t page_rows = (size_t)p.layers * 2 * p.kv_heads * p.page_size;
+  const size_t row_k = ((size_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
+  const size_t row_v = row_k + (size_t)p.kv_heads * p.page_size;
+  const uint32_t my_ring = smem_u32(ring) + warp * (kRwStages * kRwStageBytes);
+
+  // lane copies chunk c of the rows g + 8 i of a block
+  auto page_ids = [&](int bi, int (&id)[4]) {
+    const int t0 = kv_block_index(blk, bi) * kRwTok;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + g + 8 * i;
+      id[i] = t < tokens ? __ldg(p.indices + first_page + fast_div(t, p.page_div)) : 0;
+    }
+  };
+  auto issue = [&](int bi, int stage, const int (&id)[4]) {
+    const int t0 = kv_block_index(blk, bi) * kRwTok;
+    const uint32_t st = my_ring + stage * kRwStageBytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = g + 8 * i, t = t0 + r;
+      const bool ok = t < tokens;
+      const int slot = ok ? t - fast_div(t, p.page_div) * p.page_size : 0;
+      const size_t page = min((size_t)(uint32_t)id[i], (size_t)p.num_pages - 1);   // an index outside the pool reads its last page
+      const size_t rk = page * page_rows + row_k + slot, rv = page * page_rows + row_v + slot;
+      const uint32_t at = (uint32_t)(r * 64 + ((c ^ rw_swz(r)) << 4));
+      rw_cp16(st + at, p.data + rk * 64 + 16 * c, ok ? 16 : 0);
+      rw_cp16(st + kRwTok * 64 + at, p.data + rv * 64 + 16 * c, ok ? 16 : 0);
+      if (c < 2) rw_cp4(st + kRwTok * 128 + c * kRwTok * 4 + r * 4, p.param + (c ? rv : rk), ok ? 4 : 0);
+    }
+  };
+
+  float o[NT][8][4], ws[NT][4], l[NT][2], y[NT][2], m[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][t][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ws[n][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { l[n][k] = 0.0f; y[n][k] = 0.0f; m[n][k] = -INFINITY; }
+  }
+
+  int id[4];
+#pragma unroll
+  for (int s = 0; s < kRwStages - 1; ++s) {
+    const int bi = begin + s * kRwWarps;
+    if (bi < end) { page_ids(bi, id); issue(bi, s, id); }
+    rw_commit();
+  }
+  if (begin + (kRwStages - 1) * kRwWarps < end) page_ids(begin + (kRwStages - 1) * kRwWarps, id);
+
+  int stage = 0;
+  const float sm_scale = 0.08838834764831845f * 1.4426950408889634f;   // log2(e) / sqrt(128)
+  for (int bi = begin; bi < end; bi += kRwWarps) {
+    {
+      const int ahead = bi + (kRwStages - 1) * kRwWarps;
+      if (ahead < end) issue(ahead, stage == 0 ? kRwStages - 1 : stage - 1, id);
+      rw_commit();
+      if (ahead + kRwWarps < end) page_ids(ahead + kRwWarps, id);
+    }
+    rw_wait<kRwStages - 1>();
+    __syncwarp();
+    const unsigned char* st = ring + warp * (kRwStages * kRwStageBytes) + stage * kRwStageBytes;
+    const int t0 = kv_block_index(blk, bi) * kRwTok;
+    const bool edge = t0 + kRwTok - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kRwTok - 1 >= p.sinks);
+
+    float s[2][NT][4];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      // fragment rows g and g + 8: tokens 16 a + tau and 16 a + 8 + tau
+      const int tau = (g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1);
+      const int r0 = 16 * a + tau, r1 = r0 + 8;
+      const uint4 x = *reinterpret_cast<const uint4*>(st + r0 * 64 + ((c ^ rw_swz(r0)) << 4));
+      const uint4 z = *reinterpret_cast<const uint4*>(st + r1 * 64 + ((c ^ rw_swz(r1)) << 4));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][n][e] = 0.0f;
+      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, zw[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+      for (int wi = 0; wi < 4; ++wi) {
+        const uint32_t a0 = code_pair<0>(xw[wi]), a1 = code_pair<0>(zw[wi]), a2 = code_pair<1>(xw[wi]), a3 = code_pair<1>(zw[wi]);
+        const uint32_t b0 = code_pair<2>(xw[wi]), b1 = code_pair<2>(zw[wi]), b2 = code_pair<3>(xw[wi]), b3 = code_pair<3>(zw[wi]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_f16(s[a][n], a0, a1, a2, a3, qf[n][4 * wi], qf[n][4 * wi + 1]);
+          mma_f16(s[a][n], b0, b1, b2, b3, qf[n][4 * wi + 2], qf[n][4 * wi + 3]);
+        }
+      }
+    }
+    float rv[2][2], zv[2][2];                           // 1 / s', z' / s' - 7.5 of the lane's four tokens
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 16 * a + 8 * h + ((g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1));
+        const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 128 + r * 4));
+        float2 vp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 132 + r * 4));
+        // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
+        if (vp.x < 9.31322575e-10f) vp.x = 9.31322575e-10f;
+        rv[a][h] = __fdividef(1.0f, vp.x);
+        zv[a][h] = fmaf(vp.y, rv[a][h], -7.5f);
+        // x - x: 0, or NaN where key parameters are not finite (the score of such a token may not end up at -infinity)
+        const float lv = __log2f(vp.x) + ((kp.x - kp.x) + (kp.y - kp.y));
+        const float ks = kp.x * sm_scale, kz = fmaf(16.0f, ks, kp.y * sm_scale);
+        const int t = t0 + r;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float v = fmaf(ks, s[a][n][2 * h + k], fmaf(-kz, qs[n][k], lv));
+            if (edge) {
+              const bool see = t <= ps[n][k] && (p.window <= 0 || t > ps[n][k] - p.window || t < p.sinks);
+              v = see ? v : -INFINITY;
+            }
+            s[a][n][2 * h + k] = v;
+            top[n][k] = fmaxf(top[n][k], v);
+          }
+      }
+    bool grows = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top[n][k] = fmaxf(top[n][k], __shfl_xor_sync(0xffffffffu, top[n][k], x));
+        grows |= top[n][k] > m[n][k];
+      }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float mn = fmaxf(m[n][k], top[n][k]);
+          f[k] = mn == -INFINITY ? 1.0f : exp2f(m[n][k] - mn);
+          m[n][k] = mn;
+          l[n][k] *= f[k];
+          y[n][k] *= f[k];
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][t][e] *= f[e & 1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ws[n][e] *= f[e & 1];
+      }
+    }
+    uint32_t pb[2][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float w0 = exp2f(s[a][n][2 * h] - m0), w1 = exp2f(s[a][n][2 * h + 1] - m1);
+          if (edge) {
+            // a hidden token leaves the sums alone whatever its parameters hold
+            if (w0 != 0.0f) { l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]); }
+            if (w1 != 0.0f) { l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]); }
+          } else {
+            l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]);
+            l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]);
+          }
+          const __half2 wh = __floats2half2_rn(w0, w1);
+          pb[a][n][h] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&wh));
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      // slots 2c, 2c + 1, 2c + 8, 2c + 9: tokens of the tile
+      const int ta = 16 * a + rw_token_even(c), tb = 16 * a + rw_token_odd(c);
+      const unsigned char* sv = st + kRwTok * 64 + (g & 1) * 8;
+      const uint2 va = *reinterpret_cast<const uint2*>(sv + ta * 64 + (((g >> 1) ^ rw_swz(ta)) << 4));
+      const uint2 vb = *reinterpret_cast<const uint2*>(sv + tb * 64 + (((g >> 1) ^ rw_swz(tb)) << 4));
+      const uint2 vc = *reinterpret_cast<const uint2*>(sv + (ta + 8) * 64 + (((g >> 1) ^ rw_swz(ta + 8)) << 4));
+      const uint2 vd = *reinterpret_cast<const uint2*>(sv + (tb + 8) * 64 + (((g >> 1) ^ rw_swz(tb + 8)) << 4));
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {                    // four dimensions of the lane's sixteen
+        const uint32_t sel = (q4 & 1) ? 0x7632u : 0x5410u;
+        const uint32_t ab = __byte_perm(q4 < 2 ? va.x : va.y, q4 < 2 ? vb.x : vb.y, sel);
+        const uint32_t cd = __byte_perm(q4 < 2 ? vc.x : vc.y, q4 < 2 ? vd.x : vd.y, sel);
+        const uint32_t a0 = code_pair<0>(ab), a1 = code_pair<1>(ab), a2 = code_pair<0>(cd), a3 = code_pair<1>(cd);
+        const uint32_t b0 = code_pair<2>(ab), b1 = code_pair<3>(ab), b2 = code_pair<2>(cd), b3 = code_pair<3>(cd);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_f16(o[n][2 * q4], a0, a1, a2, a3, pb[a][n][0], pb[a][n][1]);
+          mma_f16(o[n][2 * q4 + 1], b0, b1, b2, b3, pb[a][n][0], pb[a][n][1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16(ws[n], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[a][n][0], pb[a][n][1]);
+    }
+    __syncwarp();                                       // the stage is filled again in the next round
+    stage = stage + 1 == kRwStages ? 0 : stage + 1;
+  }
+  rw_wait<0>();
+  __syncthreads();                                      // the ring becomes the merge buffer
+
+  float* merge = reinterpret_cast<float*>(ring);        // [warp][row][kRwORow]
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], x);
+        y[n][k] += __shfl_xor_sync(0xffffffffu, y[n][k], x);
+      }
+      const int r = 8 * n + 2 * c + k;
+      const float off = fmaf(23.5f, ws[n][k], y[n][k]);
+      float* dst = merge + ((size_t)warp * R + r) * kRwORow + 16 * g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        *reinterpret_cast<float4*>(dst + 4 * t) = make_float4(o[n][2 * t][k] - off, o[n][2 * t][2 + k] - off,
+                                                              o[n][2 * t + 1][k] - off, o[n][2 * t + 1][2 + k] - off);
+      if (g == 0) { sh.m[warp][r] = m[n][k]; sh.l[warp][r] = l[n][k]; }
+    }
+  __syncthreads();
+  for (int r = warp; r < w.rows; r += kRwWarps) {
+    float mm = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kRwWarps; ++x) mm = fmaxf(mm, sh.m[x][r]);
+    float ll = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int x = 0; x < kRwWarps; ++x) {
+      if (sh.m[x][r] == -INFINITY && sh.l[x][r] == 0.0f) continue;     // a warp that saw no token of the row
+      const float f = exp2f(sh.m[x][r] - mm);
+      const float4 v = *reinterpret_cast<const float4*>(merge + ((size_t)x * R + r) * kRwORow + 4 * lane);
+      ll = fmaf(sh.l[x][r], f, ll);
+      acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    }
+    if (p.splits == 1) {
+      rw_store_row(p, w, head_kv, r, 4 * lane, acc, ll != 0.0f ? 1.0f / ll : 0.0f);     // a row that sees nothing gives zeros
+    } else {
+      *reinterpret_cast<float4*>(&sh.part_o[r][4 * lane]) = acc;
+      if (lane == 0) { sh.part_m[r] = mm; sh.part_l[r] = ll; }
+    }
+  }
+  if (p.splits > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // the CTAs of the cluster deal out the rows
+    for (int r = (int)crank + p.splits * warp; r < w.rows; r += p.splits * kRwWarps) {
+      float mm = -INFINITY;
+      for (int x = 0; x < p.splits; ++x) mm = fmaxf(mm, peer_f32(peer_addr(&sh.part_m[r], x)));
+      float ll = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int x = 0; x < p.splits; ++x) {
+        const float mx = peer_f32(peer_addr(&sh.part_m[r], x)), lx = peer_f32(peer_addr(&sh.part_l[r], x));
+        if (mx == -INFINITY && lx == 0.0f) continue;
+        const float f = exp2f(mx - mm);
+        const float4 v = peer_f32x4(peer_addr(&sh.part_o[r][4 * lane], x));
+        ll = fmaf(lx, f, ll);
+        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+      }
+      rw_store_row(p, w, head_kv, r, 4 * lane, acc, ll != 0.0f ? 1.0f / ll : 0.0f);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+template <int NT>
+static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
+  constexpr int R = 8 * NT;
+  constexpr size_t smem = kRwRing + sizeof(RwShared<NT>);
+  static_assert(kRwWarps * R * kRwORow * sizeof(float) <= kRwRing, "the merge buffer lies in the ring");
+  static_assert(smem <= 227 * 1024, "shared memory");
+  // tiles: at most one ragged tile per sequence beyond the full ones; a grid of equal shares per sequence needs no search
+  const int64_t per_seq = (max_rows + R - 1) / R;
+  const int64_t bound = p.total_q * p.group / R + p.batch;
+  const bool uniform = !p.qo_indptr || p.batch * per_seq <= 2 * bound;
+  p.tiles_per_seq = uniform ? (int)per_seq : 0;
+  p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
+  const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= num_sms()) splits *= 2;
+  p.splits = splits;
+  if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
+  QR_CUDA(cudaFuncSetAttribute(kv_attend_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(units * splits));
+  cfg.blockDim = dim3(32 * kRwWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  QR_CUDA(cudaLaunchKernelEx(&cfg, kv_attend_rows_kernel<NT>, (const KvAttendParams)p));
+  return QR_OK;
+}
+
+int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
+  if (max_rows <= 8) return launch_rows<1>(p, max_rows, st);
+  if (max_rows <= 16) return launch_rows<2>(p, max_rows, st);
+  return launch_rows<4>(p, max_rows, st);
+}
+
+}  // namespace qr
+
+extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, const void* q, int64_t q_token_stride,
+                               int64_t q_head_stride, const void* kv_data, const void* kv_param, int64_t num_pages,
+                               const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_offset,
+                               const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
+                               int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
+                               int hadamard_q, void* stream) {
+  using namespace qr;
+  if (batch < 0 || total_q < 0 || max_q_len < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative size");
+  if (batch == 0 || total_q == 0 || max_q_len == 0) return QR_OK;
+  if (!o || !q || !kv_data || !kv_param || !kv_indptr || !kv_indices || !last_page_offset)
+    return fail(QR_EINVAL, "qr_kv_attend_i4: null pointer");
+  if (head_dim != kHeadDim) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: head_dim = %d (only 128)", head_dim);
+  if (num_layers < 1 || layer < 0 || layer >= num_layers || page_size < 1 || num_pages < 1)
+    return fail(QR_EINVAL, "qr_kv_attend_i4: bad layer / page size / pages");
+  if (num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads)
+    return fail(QR_EINVAL, "qr_kv_attend_i4: %d query heads over %d KV heads (a multiple is needed)", num_q_heads, num_kv_heads);
+  if (window < 0 || sink_tokens < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative window or sink tokens");
+  if (!qo_indptr && (total_q != batch || max_q_len != 1))
+    return fail(QR_EINVAL, "qr_kv_attend_i4: without qo_indptr every sequence has one new token");
+  if (max_q_len > total_q) return fail(QR_EINVAL, "qr_kv_attend_i4: max_q_len exceeds the number of new tokens");
+  const int group = num_q_heads / num_kv_heads;
+  if (total_q * group > 0x3fffffffll || (int64_t)batch * max_q_len * group > 0xffffffffffll)
+    return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many query rows");
+  if (((uintptr_t)q & 7) || ((uintptr_t)o & 7) || ((uintptr_t)kv_data & 15) || ((uintptr_t)kv_param & 3) || (q_token_stride & 3) ||
+      (q_head_stride & 3) || (o_token_stride & 3) || (o_head_stride & 3))
+    return fail(QR_EALIGN, "qr_kv_attend_i4: q and o must be 8-byte aligned with strides that are multiples of 4, the pages 16-byte aligned");
+  KvAttendParams p = {};
+  p.o = reinterpret_cast<__half*>(o); p.q = reinterpret_cast<const __half*>(q);
+  p.data = reinterpret_cast<const uint8_t*>(kv_data); p.param = reinterpret_cast<const __half2*>(kv_param);
+  p.indptr = kv_indptr; p.indices = kv_indices; p.last_page_offset = last_page_offset; p.qo_indptr = qo_indptr;
+  p.q_ts = q_token_stride; p.q_hs = q_head_stride; p.o_ts = o_token_stride; p.o_hs = o_head_stride;
+  p.total_q = total_q; p.batch = batch; p.layers = num_layers; p.layer = layer; p.kv_heads = num_kv_heads; p.group = group;
+  p.page_size = page_size; p.num_pages = num_pages;
+  p.page_div = make_fastdiv((uint32_t)page_size); p.group_div = make_fastdiv((uint32_t)group);
+  p.window = window; p.sinks = window > 0 ? sink_tokens : 0; p.hadamard_q = hadamard_q;
+  p.status = kernel_status_ptr();
+  return launch_kv_attend_rows(p, max_q_len * group, (cudaStream_t)stream);
+}

@@ -5,6 +5,9 @@
 // [num_pages, layers, 2, heads, page_size, 2] fp16 = (scale, zero); value = code * scale - zero.  Sequence b owns the
 // pages kv_indices[kv_indptr[b] .. kv_indptr[b + 1]), the last of which holds last_page_offset[b] tokens.
 //
+// kv_append_kernel takes its page slots from the page table (the position of a token follows from the lengths) or from a
+// slot map with one entry per token, as qr_kv_page_table writes it.
+//
 // kv_append_kernel: one warp per (new token, head).  The lane holds four of the 128 values of the head: optional
 // Walsh-Hadamard transform of the key over the head dimension (two butterfly stages in registers, five warp-shuffle
 // stages, fp32, scale 1/sqrt(128), rounded to fp16), min / max by shuffles, the asymmetric quantiser in the fp16
@@ -19,13 +22,11 @@
 // separately.  The eight partial states are merged
 // through shared memory.  The query's Hadamard transform, which upstream applies with a separate kernel, runs at
 // the start of the same kernel.
-#include "common.cuh"
+#include "kv_common.cuh"
 
 #include <math.h>
 
 namespace qr {
-
-constexpr int kHeadDim = 128;
 
 struct KvAppendParams {
   uint8_t* data;
@@ -38,31 +39,10 @@ struct KvAppendParams {
   const int32_t* append_indptr; // [batch + 1], or null: one token per sequence
   int batch, layers, layer, heads, page_size, tokens;
   int hadamard_k;
+  const int64_t* slots;         // [tokens] page * page_size + slot, outside the pool: the token is left out; or null
+  int64_t num_slots;            // pages of the pool x page_size
+  int64_t k_ts, k_hs, v_ts, v_hs;   // strides of k and v in elements between tokens and between heads
 };
-
-// Walsh-Hadamard transform of 128 values held four per lane (element index = 4 lane + e), unscaled.
-__device__ __forceinline__ void fwht128_warp(float (&x)[4], int lane) {
-  {
-    const float a = x[0] + x[1], b = x[0] - x[1], c = x[2] + x[3], d = x[2] - x[3];
-    x[0] = a + c; x[1] = b + d; x[2] = a - c; x[3] = b - d;
-  }
-#pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const float sg = (lane & s) ? -1.0f : 1.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float o = __shfl_xor_sync(0xffffffffu, x[e], s);
-      x[e] = fmaf(x[e], sg, o);
-    }
-  }
-}
-
-__device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-}
 
 // Asymmetric int4 codes of one (token, head) row, four values per lane, with the fp16 arithmetic of the reference:
 //   scale = fp16(max(fp16(max - min), 1e-5) / 15), zero = -min, code = clamp(rint(fp16(fp16(x + zero) / scale)), 0, 15).
@@ -98,29 +78,37 @@ kv_append_kernel(const KvAppendParams p) {
   const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= (long long)p.tokens * p.heads) return;
   const int tok = (int)(item / p.heads), head = (int)(item % p.heads);
-  int b = tok, j = 0, append_len = 1;
-  if (p.append_indptr) {
-    int lo = 0, hi = p.batch;                // largest b with append_indptr[b] <= tok
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.append_indptr[mid] <= tok) lo = mid; else hi = mid;
+  long long page;
+  int slot;
+  if (p.slots) {
+    const long long s = p.slots[tok];
+    if (s < 0 || s >= p.num_slots) return;
+    page = s / p.page_size;
+    slot = (int)(s - page * p.page_size);
+  } else {
+    int b = tok, j = 0, append_len = 1;
+    if (p.append_indptr) {
+      int lo = 0, hi = p.batch;                // largest b with append_indptr[b] <= tok
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.append_indptr[mid] <= tok) lo = mid; else hi = mid;
+      }
+      b = lo;
+      j = tok - p.append_indptr[b];
+      append_len = p.append_indptr[b + 1] - p.append_indptr[b];
     }
-    b = lo;
-    j = tok - p.append_indptr[b];
-    append_len = p.append_indptr[b + 1] - p.append_indptr[b];
+    // the page table already describes the sequence WITH the appended tokens
+    const int first = p.indptr[b];
+    const long long seq_len = (long long)(p.indptr[b + 1] - first - 1) * p.page_size + p.last_page_offset[b];
+    const long long pos = seq_len - append_len + j;
+    if (pos < 0) return;
+    page = p.indices[first + (int)(pos / p.page_size)];
+    slot = (int)(pos % p.page_size);
   }
-  // the page table already describes the sequence WITH the appended tokens
-  const int first = p.indptr[b];
-  const long long seq_len = (long long)(p.indptr[b + 1] - first - 1) * p.page_size + p.last_page_offset[b];
-  const long long pos = seq_len - append_len + j;
-  if (pos < 0) return;
-  const long long page = p.indices[first + (int)(pos / p.page_size)];
-  const int slot = (int)(pos % p.page_size);
-  const size_t src = ((size_t)tok * p.heads + head) * kHeadDim + 4 * lane;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float x[4];
-    load4_f16((which == 0 ? p.k : p.v) + src, x);
+    load4_f16((which == 0 ? p.k + (tok * p.k_ts + head * p.k_hs) : p.v + (tok * p.v_ts + head * p.v_hs)) + 4 * lane, x);
     __half h[4];
     if (which == 0 && p.hadamard_k) {
       fwht128_warp(x, lane);
@@ -386,8 +374,37 @@ int qr_kv_append_i4(void* kv_data, void* kv_param, const int32_t* kv_indptr, con
   p.k = reinterpret_cast<const __half*>(k); p.v = reinterpret_cast<const __half*>(v); p.append_indptr = append_indptr;
   p.batch = batch; p.layers = num_layers; p.layer = layer; p.heads = num_heads; p.page_size = page_size;
   p.tokens = (int)tokens; p.hadamard_k = hadamard_k;
+  p.slots = nullptr; p.num_slots = 0;
+  p.k_hs = p.v_hs = qr::kHeadDim; p.k_ts = p.v_ts = (int64_t)num_heads * qr::kHeadDim;
   const long long items = tokens * num_heads;
   const unsigned grid = (unsigned)((items + 7) / 8);
+  qr::kv_append_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+  QR_LAUNCH_CHECK("kv_append_kernel");
+  return QR_OK;
+}
+
+int qr_kv_append_slots_i4(void* kv_data, void* kv_param, int64_t num_pages, const int64_t* slot_map, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, int64_t tokens, int num_layers, int layer, int num_heads, int page_size,
+                          int head_dim, int hadamard_k, void* stream) {
+  if (tokens < 0) return qr::fail(QR_EINVAL, "qr_kv_append_slots_i4: negative size");
+  if (tokens == 0) return QR_OK;
+  if (!kv_data || !kv_param || !slot_map || !k || !v) return qr::fail(QR_EINVAL, "qr_kv_append_slots_i4: null pointer");
+  if (head_dim != qr::kHeadDim) return qr::fail(QR_EUNSUPPORTED, "qr_kv_append_slots_i4: head_dim = %d (only 128)", head_dim);
+  if (num_layers < 1 || layer < 0 || layer >= num_layers || num_heads < 1 || page_size < 1 || num_pages < 1)
+    return qr::fail(QR_EINVAL, "qr_kv_append_slots_i4: bad layer / heads / page size / pages");
+  if (tokens > 0x7fffffffll || tokens * num_heads > (1ll << 33)) return qr::fail(QR_EUNSUPPORTED, "qr_kv_append_slots_i4: too many tokens");
+  if (((uintptr_t)k & 7) || ((uintptr_t)v & 7) || ((uintptr_t)kv_data & 1) || ((uintptr_t)kv_param & 3) || ((uintptr_t)slot_map & 7) ||
+      (k_token_stride & 3) || (k_head_stride & 3) || (v_token_stride & 3) || (v_head_stride & 3))
+    return qr::fail(QR_EALIGN, "qr_kv_append_slots_i4: k and v must be 8-byte aligned with strides that are multiples of 4");
+  qr::KvAppendParams p = {};
+  p.data = reinterpret_cast<uint8_t*>(kv_data); p.param = reinterpret_cast<__half2*>(kv_param);
+  p.k = reinterpret_cast<const __half*>(k); p.v = reinterpret_cast<const __half*>(v);
+  p.layers = num_layers; p.layer = layer; p.heads = num_heads; p.page_size = page_size;
+  p.tokens = (int)tokens; p.hadamard_k = hadamard_k;
+  p.slots = slot_map; p.num_slots = num_pages * page_size;
+  p.k_ts = k_token_stride; p.k_hs = k_head_stride; p.v_ts = v_token_stride; p.v_hs = v_head_stride;
+  const unsigned grid = (unsigned)((tokens * num_heads + 7) / 8);
   qr::kv_append_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
   QR_LAUNCH_CHECK("kv_append_kernel");
   return QR_OK;

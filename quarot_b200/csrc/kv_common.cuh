@@ -1,0 +1,161 @@
+// What the kernels of the paged 4-bit KV cache share: the 128-long Walsh-Hadamard transform of a warp, exact division
+// by the page size, the parameters of the chunk / window attention kernels and the walk over the visible tokens.
+#pragma once
+#include "common.cuh"
+
+namespace qr {
+
+constexpr int kHeadDim = 128;
+
+#ifdef __CUDACC__
+// Walsh-Hadamard transform of 128 values held four per lane (element index = 4 lane + e), unscaled.
+__device__ __forceinline__ void fwht128_warp(float (&x)[4], int lane) {
+  {
+    const float a = x[0] + x[1], b = x[0] - x[1], c = x[2] + x[3], d = x[2] - x[3];
+    x[0] = a + c; x[1] = b + d; x[2] = a - c; x[3] = b - d;
+  }
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const float sg = (lane & s) ? -1.0f : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float o = __shfl_xor_sync(0xffffffffu, x[e], s);
+      x[e] = fmaf(x[e], sg, o);
+    }
+  }
+}
+
+__device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+}
+#endif
+
+// Division of 0 <= n < 2^31 by a fixed d >= 1 as one wide multiplication: with s = ceil(log2 d) and
+// m = ceil(2^(31+s) / d) <= 2^32 - 1 (2^31 for d = 1), m d - 2^(31+s) < d <= 2^s, hence floor(n m / 2^(31+s)) = floor(n / d).
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+};
+static inline FastDiv make_fastdiv(uint32_t d) {
+  FastDiv f;
+  f.d = d;
+  f.s = ilog2(d);
+  f.m = (uint32_t)((((uint64_t)1 << (31 + f.s)) + d - 1) / d);
+  return f;
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ int fast_div(int n, const FastDiv& f) {
+  return (int)(((uint64_t)(uint32_t)n * f.m) >> (31 + f.s));
+}
+#endif
+
+// Attention of new tokens over the cache (qr_kv_attend_i4).
+struct KvAttendParams {
+  __half* o;                    // new token x head x 128, strides below
+  const __half* q;
+  const uint8_t* data;
+  const __half2* param;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* last_page_offset;
+  const int32_t* qo_indptr;     // [batch + 1], or null: one new token per sequence
+  int64_t q_ts, q_hs, o_ts, o_hs;   // strides in elements between tokens and between heads
+  int64_t total_q;
+  int batch, layers, layer, kv_heads, group, page_size;
+  int64_t num_pages;
+  FastDiv page_div, group_div;
+  int window, sinks;            // window 0: none
+  int hadamard_q;
+  int splits;                   // CTAs (one cluster) that share the tokens of a tile of rows
+  int tiles_per_seq;            // > 0: tile index = sequence * tiles_per_seq + tile; 0: found by a search in qo_indptr
+  int max_tiles;                // tiles that the grid holds per KV head
+  int* status;
+};
+
+#ifdef __CUDACC__
+// The tile of query rows that a CTA works on.  Row r of a sequence is (new token r / group, head r % group of the KV head).
+struct KvTile {
+  int b, row0, rows;            // sequence, first row, rows (0: nothing to do)
+  int64_t tok0;                 // first new token of the sequence in q and o
+  int seq_len, pos0;            // cached tokens with the new ones; position of new token 0
+};
+
+// Sequence and tile of rows behind tile index `tile`, by all lanes of a warp.
+__device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile, int tile_rows, int lane) {
+  KvTile w;
+  w.rows = 0; w.b = 0; w.row0 = 0; w.tok0 = 0; w.seq_len = 0; w.pos0 = 0;
+  int j = -1, b = 0;
+  if (p.tiles_per_seq > 0) {
+    b = tile / p.tiles_per_seq;
+    j = tile - b * p.tiles_per_seq;
+  } else {
+    int base = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int bb = b0 + lane;
+      int n = 0;
+      if (bb < p.batch) {
+        const long long rows = (long long)(p.qo_indptr[bb + 1] - p.qo_indptr[bb]) * p.group;
+        n = rows > 0 ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
+      }
+      int end = n;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, end, s);
+        if (lane >= s) end += up;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, base + end > tile);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        b = b0 + src;
+        j = tile - base - (__shfl_sync(0xffffffffu, end, src) - __shfl_sync(0xffffffffu, n, src));
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (j < 0) return w;
+  }
+  if (b >= p.batch) return w;
+  long long tok0 = b, len = 1;
+  if (p.qo_indptr) {
+    tok0 = p.qo_indptr[b];
+    len = p.qo_indptr[b + 1] - tok0;
+  }
+  if (tok0 < 0 || tok0 + len > p.total_q) return w;       // rows beyond q are not touched
+  const long long rows = len * p.group, row0 = (long long)j * tile_rows;
+  if (row0 >= rows) return w;
+  const int first = p.indptr[b];
+  const long long seq = (long long)(p.indptr[b + 1] - first - 1) * p.page_size + p.last_page_offset[b];
+  w.b = b;
+  w.row0 = (int)row0;
+  w.rows = (int)(rows - row0 < tile_rows ? rows - row0 : tile_rows);
+  w.tok0 = tok0;
+  w.seq_len = seq > 0 ? (int)seq : 0;
+  w.pos0 = (int)(seq > 0 ? seq - len : -len);
+  return w;
+}
+
+// Blocks of T tokens that the rows at positions p_min .. p_max see: `head` blocks from token 0 on (the sinks), then the
+// blocks first .. end.  Without a window, or where the two ranges meet, head = 0 and first = 0.
+struct KvBlocks {
+  int head, first, count;
+};
+template <int T>
+__device__ __forceinline__ KvBlocks kv_blocks(int p_min, int p_max, int window, int sinks) {
+  KvBlocks k;
+  const int end = p_max >= 0 ? p_max / T + 1 : 0;
+  const int lo = window > 0 ? max(0, p_min - window + 1) : 0;
+  k.first = min(lo / T, end);
+  k.head = (max(min(sinks, p_max + 1), 0) + T - 1) / T;
+  if (window <= 0 || k.head >= k.first) { k.head = 0; k.first = 0; }
+  k.count = k.head + end - k.first;
+  return k;
+}
+__device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) { return i < k.head ? i : k.first + i - k.head; }
+#endif
+
+int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
+
+}  // namespace qr

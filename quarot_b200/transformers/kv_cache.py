@@ -2,10 +2,15 @@
 
 Same constructor, same `update()` contract and the same memory layout as upstream -- pages
 [pages, layers, 2, heads, page_size, head_dim / 2] uint8 with per-(token, head) fp16 (scale, zero) pairs beside them
--- so a model written against `quarot.transformers.MultiLayerPagedKVCache4Bit` runs unchanged.  Underneath, two fused
+-- so a model written against `quarot.transformers.MultiLayerPagedKVCache4Bit` runs unchanged.  Underneath, fused
 CUDA kernels replace upstream's chain: `qr_kv_append_i4` (Hadamard of the keys over the head dimension, asymmetric
 int4 quantisation, packing and the write into the page slot, for prompt and single-token appends alike) and
 `qr_kv_decode_i4` (Hadamard of the query, then single-token attention straight from the packed pages).
+
+Beyond upstream: `build_page_table` (page table and slot map from request lengths, on the GPU), `append_kv_slots_i4` (the
+append that takes that slot map), `chunk_attention_i4` (causal attention of several new tokens per sequence, ragged, with
+grouped query heads), and a sliding window with sink tokens for chunks and single tokens.  The cache class uses them for
+chunks after the prompt, for sequences of different page counts and with `window_size` / `sink_tokens`.
 
 Not built: `disable_quant=True` (the fp16 variant of the cache) raises NotImplementedError.
 """
@@ -67,9 +72,167 @@ def append_kv_i4(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, k, 
             1 if hadamard_k else 0, _stream(dev)), "append_kv_i4")
 
 
-def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, hadamard_q=False):
+def _check_i32(op, dev, **tensors):
+    for name, (t, n) in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise RuntimeError("%s: %s must be a contiguous int32 tensor on %s" % (op, name, dev))
+        if n is not None and t.numel() < n:
+            raise RuntimeError("%s: %s has %d entries, %d are needed" % (op, name, t.numel(), n))
+
+
+def _check_pages(op, kv_data, kv_param, layer_idx):
+    """Checks of the page pool [pages, layers, 2, heads, page_size, 64] and its parameters; (layers, heads, page_size)."""
+    dev = _ops._check_cuda_contig(op, kv_data=kv_data, kv_param=kv_param)
+    if kv_data.dtype != torch.uint8 or kv_param.dtype != torch.float16:
+        raise RuntimeError("%s: the pages are uint8 and their parameters fp16" % op)
+    if kv_data.dim() != 6 or kv_data.shape[2] != 2 or tuple(kv_param.shape) != tuple(kv_data.shape[:5]) + (2,):
+        raise RuntimeError("%s: pages %s and parameters %s do not belong together" % (op, tuple(kv_data.shape), tuple(kv_param.shape)))
+    if kv_data.shape[5] != 64:
+        raise RuntimeError("%s: head_dim must be 128" % op)
+    if not 0 <= int(layer_idx) < kv_data.shape[1]:
+        raise RuntimeError("%s: layer %d of %d" % (op, layer_idx, kv_data.shape[1]))
+    return dev, kv_data.shape[1], kv_data.shape[3], kv_data.shape[4]
+
+
+def _check_rows(op, dev, name, t):
+    """[tokens, heads, 128] fp16 on dev, last axis contiguous; the strides of the other two."""
+    if t.device != dev or t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != 128:
+        raise RuntimeError("%s: %s must be fp16 [tokens, heads, 128] on %s" % (op, name, dev))
+    ts, hs = t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+    if t.numel() and (t.stride(2) != 1 or ts % 4 or hs % 4 or t.data_ptr() % 8):
+        raise RuntimeError("%s: %s needs a contiguous last axis, 8-byte alignment and strides that are multiples of 4" % (op, name))
+    return ts, hs
+
+
+def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, free_pages=None, max_blocks=None):
+    """Page table and slot map of one step from request lengths, in one launch and without reading anything back.
+
+    seq_lens int32 [batch]: cached tokens before the step; new_lens int32 [batch]: tokens the step adds (None: one each);
+    new_tokens: rows of the slot map, at least the sum of new_lens (the batch size is right for None).  block_table int32
+    [batch, max_blocks] holds the pages of the sequences; pages that a sequence needs beyond those it holds are taken from
+    free_pages (int32, in order) and written into it.  Without free_pages the block table already holds them; without
+    block_table page j of sequence b is j * batch + b (the cache below), at most max_blocks per sequence.
+
+    Returns a dict: kv_indptr [batch + 1], kv_indices [batch * max_blocks] (-1 behind the last page), last_page_offset
+    [batch] -- the sequences WITH the new tokens -- append_indptr [batch + 1], slot_map int64 [new_tokens], positions
+    int32 [new_tokens], seq_lens [batch] after the step, status int32 [2] = (free pages taken, sequences refused).  A
+    sequence that does not fit (free list, block table or slot map too short) is refused: it keeps its length and its
+    tokens get slot and position -1, which append_kv_slots_i4 skips.
+    """
+    op = "build_page_table"
+    if seq_lens.dim() != 1 or not seq_lens.is_cuda:
+        raise RuntimeError("%s: seq_lens must be a one-dimensional CUDA tensor" % op)
+    dev, batch, new_tokens, page_size = seq_lens.device, seq_lens.shape[0], int(new_tokens), int(page_size)
+    if block_table is not None:
+        if block_table.dim() != 2 or block_table.shape[0] != batch or (max_blocks not in (None, block_table.shape[1])):
+            raise RuntimeError("%s: block_table must be [batch, max_blocks]" % op)
+        max_blocks = block_table.shape[1]
+    elif free_pages is not None or max_blocks is None:
+        raise RuntimeError("%s: without a block_table there is no free list, and max_blocks is needed" % op)
+    max_blocks = int(max_blocks)
+    _check_i32(op, dev, seq_lens=(seq_lens, batch), new_lens=(new_lens, batch), block_table=(block_table, None),
+               free_pages=(free_pages, None))
+    if new_tokens < 0 or page_size < 1 or max_blocks < 1:
+        raise RuntimeError("%s: bad number of new tokens, page size or blocks per sequence" % op)
+    with torch.cuda.device(dev):
+        # one allocation for the 32-bit outputs, each on a 16-byte boundary
+        sizes = (batch + 1, batch * max_blocks, batch, batch + 1, new_tokens, batch, 2)
+        names = ("kv_indptr", "kv_indices", "last_page_offset", "append_indptr", "positions", "seq_lens", "status")
+        starts = [0]
+        for n in sizes:
+            starts.append(starts[-1] + (n + 3) // 4 * 4)
+        buf = torch.empty(starts[-1], dtype=torch.int32, device=dev)
+        out = {name: buf[a:a + n] for name, a, n in zip(names, starts, sizes)}
+        out["slot_map"] = torch.empty(new_tokens, dtype=torch.int64, device=dev)
+        if batch == 0:
+            buf.zero_()
+            out["positions"].fill_(-1)
+            out["slot_map"].fill_(-1)
+            return out
+        _lib.check(_lib_c.qr_kv_page_table(
+            seq_lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, batch, new_tokens, page_size, max_blocks,
+            block_table.data_ptr() if block_table is not None else None,
+            free_pages.data_ptr() if free_pages is not None and free_pages.numel() else None,
+            free_pages.numel() if free_pages is not None else -1,
+            out["kv_indptr"].data_ptr(), out["kv_indices"].data_ptr(), out["last_page_offset"].data_ptr(),
+            out["append_indptr"].data_ptr(), out["slot_map"].data_ptr(), out["positions"].data_ptr(), out["seq_lens"].data_ptr(),
+            out["status"].data_ptr(), _stream(dev)), op)
+    return out
+
+
+def append_kv_slots_i4(kv_data, kv_param, slot_map, k, v, layer_idx, hadamard_k=True):
+    """append_kv_i4 with the page slots from a slot map (build_page_table): slot_map int64 [tokens], k and v fp16 [tokens,
+    heads, 128] (strided views are fine).  Tokens whose slot lies outside the pool, -1 among others, are left out."""
+    op = "append_kv_slots_i4"
+    dev, layers, heads, page_size = _check_pages(op, kv_data, kv_param, layer_idx)
+    kt, kh = _check_rows(op, dev, "k", k)
+    vt, vh = _check_rows(op, dev, "v", v)
+    if k.shape != v.shape or k.shape[1] != heads:
+        raise RuntimeError("%s: k %s and v %s over %d heads" % (op, tuple(k.shape), tuple(v.shape), heads))
+    if slot_map.dtype != torch.int64 or slot_map.device != dev or not slot_map.is_contiguous() or slot_map.numel() != k.shape[0]:
+        raise RuntimeError("%s: slot_map must be contiguous int64 on %s with one entry per token" % (op, dev))
+    with torch.cuda.device(dev):
+        _lib.check(_lib_c.qr_kv_append_slots_i4(
+            kv_data.data_ptr(), kv_param.data_ptr(), kv_data.shape[0], slot_map.data_ptr(), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+            k.shape[0], layers, int(layer_idx), heads, page_size, 128, 1 if hadamard_k else 0, _stream(dev)), op)
+
+
+def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr, max_q_len, layer_idx, hadamard_q,
+               window, sink_tokens):
+    dev, layers, kv_heads, page_size = _check_pages(op, kv_data, kv_param, layer_idx)
+    qt, qh = _check_rows(op, dev, "q", q)
+    ot, oh = _check_rows(op, dev, "o", o)
+    if o.shape != q.shape:
+        raise RuntimeError("%s: o %s, q %s" % (op, tuple(o.shape), tuple(q.shape)))
+    tokens, heads = q.shape[:2]
+    if not ((heads < 2 or oh >= 128) and (tokens < 2 or ot >= 128) and
+            (heads < 2 or tokens < 2 or ot >= oh * heads or oh >= ot * tokens)):
+        raise RuntimeError("%s: the rows of o overlap" % op)
+    if heads == 0 or heads % kv_heads:
+        raise RuntimeError("%s: %d query heads over %d KV heads" % (op, heads, kv_heads))
+    batch = last_page_offset.shape[0]
+    _check_i32(op, dev, kv_indptr=(kv_indptr, batch + 1), kv_indices=(kv_indices, None), last_page_offset=(last_page_offset, batch),
+               qo_indptr=(qo_indptr, batch + 1))
+    if window is not None and window < 1 or sink_tokens < 0:
+        raise RuntimeError("%s: window must be positive (None: no window), sink_tokens not negative" % op)
+    with torch.cuda.device(dev):
+        _lib.check(_lib_c.qr_kv_attend_i4(
+            o.data_ptr(), ot, oh, q.data_ptr(), qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), kv_data.shape[0], kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), last_page_offset.data_ptr(), qo_indptr.data_ptr() if qo_indptr is not None else None, tokens,
+            max_q_len, batch, layers, int(layer_idx), heads, kv_heads, page_size, 128, min(int(window), 0x7fffffff) if window else 0,
+            min(int(sink_tokens), 0x7fffffff), 1 if hadamard_q else 0, _stream(dev)), op)
+
+
+def chunk_attention_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr, layer_idx, max_q_len=None,
+                       hadamard_q=False, window=None, sink_tokens=0):
+    """Causal attention of several new tokens per sequence over the packed pages, which already hold them.
+
+    q, o fp16 [tokens, heads, 128] (strided views are fine), the new tokens of sequence b in rows qo_indptr[b] ..
+    qo_indptr[b + 1]; they are the last of its cached tokens.  heads may be a multiple of the cache's heads: query head h
+    reads KV head h // (heads // kv_heads).  window: a token sees itself and the window - 1 tokens before it, and the first
+    sink_tokens tokens.  max_q_len: an upper bound of the new tokens of any sequence (default: all of q; a close bound
+    makes a better grid).  Rows that see nothing give zeros; rows of o that belong to no sequence stay as they are."""
+    max_q_len = q.shape[0] if max_q_len is None else int(max_q_len)
+    if qo_indptr is None:
+        raise RuntimeError("chunk_attention_i4: qo_indptr is needed")
+    if max_q_len < 1 and q.shape[0]:
+        raise RuntimeError("chunk_attention_i4: max_q_len must be positive")
+    _attend_i4("chunk_attention_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr,
+               min(max_q_len, q.shape[0]), layer_idx, hadamard_q, window, sink_tokens)
+
+
+def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, hadamard_q=False, window=None,
+                    sink_tokens=0):
     """o[b, h] = softmax(q[b, h] K^T / sqrt(d)) V over the packed pages, one new token per sequence
-    (quarot/transformers/kv_cache.py:64-72); with hadamard_q the query is Hadamard-transformed first."""
+    (quarot/transformers/kv_cache.py:64-72); with hadamard_q the query is Hadamard-transformed first.  With a window only
+    the last `window` tokens and the first sink_tokens are seen; the query may have a multiple of the cache's heads."""
+    if window is not None or q.dim() == 3 and q.shape[1] != kv_data.shape[3]:
+        if q.shape[0] != last_page_offset.shape[0]:
+            raise RuntimeError("batch_decode_i4: %d queries for %d sequences" % (q.shape[0], last_page_offset.shape[0]))
+        return _attend_i4("batch_decode_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, None, 1, layer_idx,
+                          hadamard_q, window, sink_tokens)
     batch, heads, head_dim = q.shape
     assert o.shape == q.shape and q.dtype == o.dtype == torch.float16 and q.is_contiguous() and o.is_contiguous()
     dev = kv_data.device
@@ -80,32 +243,56 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             1 if hadamard_q else 0, _stream(dev)), "batch_decode_i4")
 
 
-class _AttentionStub(object):
-    """What `update()` hands back once the prompt is cached: attention of one new token against the cache."""
+_TABLE_KEYS = ("kv_data", "kv_indptr", "kv_indices", "last_page_offset", "kv_param")
 
-    def __init__(self, cache_page_size, device, n_layers, disable_quant, hadamard_dtype):
+
+class _AttentionStub(object):
+    """What `update()` hands back once the prompt is cached: attention of the new tokens against the cache."""
+
+    def __init__(self, cache_page_size, device, n_layers, disable_quant, hadamard_dtype, window_size=None, sink_tokens=0):
         self.cache_page_size = cache_page_size
         self.n_layers = n_layers
         self.disable_quant = disable_quant
         self.hadamard_dtype = hadamard_dtype
+        self.window_size = window_size
+        self.sink_tokens = sink_tokens
 
-    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx):
+    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, chunk=None):
         batch_size, q_len, num_qo_heads, head_dim = q.shape
-        assert q_len == 1
-        q = q.reshape(batch_size, num_qo_heads, head_dim).contiguous()
-        attn_output = torch.empty_like(q)
-        batch_decode_i4(attn_output, q, **attention_kwargs, layer_idx=layer_idx,
-                        hadamard_q=self.hadamard_dtype is not None)
-        return attn_output.unsqueeze(1)
+        table = {k: attention_kwargs[k] for k in _TABLE_KEYS}
+        if chunk is None:
+            assert q_len == 1
+            q = q.reshape(batch_size, num_qo_heads, head_dim).contiguous()
+            attn_output = torch.empty_like(q)
+            batch_decode_i4(attn_output, q, **table, layer_idx=layer_idx, hadamard_q=self.hadamard_dtype is not None,
+                            window=self.window_size, sink_tokens=self.sink_tokens)
+            return attn_output.unsqueeze(1)
+        added, qo_indptr, keep = chunk
+        assert q_len == added
+        rows = q.reshape(batch_size * q_len, num_qo_heads, head_dim)
+        rows = (rows if keep is None else rows[keep]).contiguous()
+        attn_output = torch.empty_like(rows)
+        chunk_attention_i4(attn_output, rows, **table, qo_indptr=qo_indptr, layer_idx=layer_idx, max_q_len=q_len,
+                           hadamard_q=self.hadamard_dtype is not None, window=self.window_size, sink_tokens=self.sink_tokens)
+        if keep is not None:                    # padded positions of the chunk give zeros
+            full = attn_output.new_zeros((batch_size * q_len, num_qo_heads, head_dim))
+            full[keep] = attn_output
+            attn_output = full
+        return attn_output.view(batch_size, q_len, num_qo_heads, head_dim)
 
 
 class MultiLayerPagedKVCache4Bit:
+    """window_size / sink_tokens: attention of the cached tokens with a sliding window and a few first tokens that stay
+    visible (models trained or run that way); the cache itself keeps every token."""
+
     def __init__(self, batch_size, page_size, max_seq_len, device, n_layers, num_heads, head_dim,
-                 disable_quant=False, hadamard_dtype=torch.float16):
+                 disable_quant=False, hadamard_dtype=torch.float16, window_size=None, sink_tokens=0):
         if disable_quant:
             raise NotImplementedError("MultiLayerPagedKVCache4Bit(disable_quant=True): the fp16 variant of the cache is not built")
         if head_dim != 128:
             raise NotImplementedError("MultiLayerPagedKVCache4Bit: head_dim must be 128 (as in the upstream kernels)")
+        if window_size is not None and window_size < 1 or sink_tokens < 0:
+            raise ValueError("MultiLayerPagedKVCache4Bit: window_size must be positive (None: no window), sink_tokens not negative")
         self.page_size = page_size
         self.batch_size = batch_size
         max_page_cnt = self.page_cnt_from_length(max_seq_len)
@@ -120,7 +307,7 @@ class MultiLayerPagedKVCache4Bit:
         self.device = device
         self.hadamard_dtype = hadamard_dtype
         self._stub = _AttentionStub(self.page_size, device, n_layers, disable_quant=self.disable_quant,
-                                    hadamard_dtype=self.hadamard_dtype)
+                                    hadamard_dtype=self.hadamard_dtype, window_size=window_size, sink_tokens=sink_tokens)
 
     def page_cnt_from_length(self, length):
         return (length + self.page_size - 1) // self.page_size
@@ -136,8 +323,9 @@ class MultiLayerPagedKVCache4Bit:
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
         """First call per layer (the prompt): caches the keys / values and returns them unchanged, for the caller's own
-        prefill attention.  Later calls (one token per sequence): caches the token and returns a callable that maps the
-        query [batch, 1, heads, head_dim] to the attention output against the cache."""
+        prefill attention.  Later calls: cache one token per sequence, or a chunk of them, and return a callable that maps
+        the query [batch, tokens, heads, head_dim] to the attention output against the cache.  cache_kwargs may hold an
+        attention_mask [batch, cached + new tokens]; sequences may then differ in length by more than a page."""
         b_sz, added_length, num_heads, head_dim = key_states.shape
         assert b_sz == self.batch_size
         attention_mask = (cache_kwargs or {}).get("attention_mask")
@@ -149,42 +337,53 @@ class MultiLayerPagedKVCache4Bit:
         had = self.hadamard_dtype is not None
         k = key_states.reshape(b_sz * added_length, num_heads, head_dim)
         v = value_states.reshape(b_sz * added_length, num_heads, head_dim)
+        if not self._needs_init[layer_idx] and added_length == 1:
+            append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
+                         specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx, hadamard_k=had)
+            return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
+        keep = new_lens = None
+        if attention_mask is not None:
+            new_mask = attention_mask[:, -added_length:].bool()
+            keep = new_mask.flatten()
+            new_lens = new_mask.sum(dim=-1, dtype=torch.int32)
+            k, v = k[keep], v[keep]
+        else:
+            new_lens = torch.full((b_sz,), added_length, dtype=torch.int32, device=self.device)
+        total = torch.full_like(new_lens, self.length) if attention_mask is None else attention_mask.sum(dim=-1, dtype=torch.int32)
+        table = build_page_table(total - new_lens, new_lens, k.shape[0], self.page_size,
+                                 max_blocks=self.pages.shape[0] // self.batch_size)
+        append_kv_slots_i4(self.pages, self.scales, table["slot_map"], k, v, layer_idx, hadamard_k=had)
         if self._needs_init[layer_idx]:
             self._needs_init[layer_idx] = False
-            if attention_mask is not None:
-                keep = attention_mask.flatten().bool()
-                k, v = k[keep], v[keep]
-                seqlens = torch.nn.functional.pad(
-                    torch.cumsum(attention_mask.sum(dim=-1, dtype=torch.int32), dim=0, dtype=torch.int32), (1, 0))
-            else:
-                seqlens = torch.arange(self.batch_size + 1, device=self.device, dtype=torch.int) * added_length
-            append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
-                         specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx,
-                         seqlen_indptr=seqlens.to(torch.int32).contiguous(), hadamard_k=had)
             return key_states, value_states
-        assert added_length == 1
-        append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
-                     specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx, hadamard_k=had)
-        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
+        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
+                                 chunk=(added_length, table["append_indptr"], keep))
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         """Page table of the cache as the kernels take it: sequence b owns pages b, b + batch, b + 2 batch, ..."""
         if attention_mask is not None:
             seqlens = attention_mask.sum(dim=-1, dtype=torch.int32)
         else:
-            seqlens = torch.tensor([self.length], dtype=torch.int32, device=self.device).expand(self.batch_size)
-        page_cnt = self.page_cnt_from_length(seqlens)
-        if (page_cnt[0] != page_cnt).any():
-            raise NotImplementedError("Current implementation does not support the case where batches have different number of pages")
-        page_cnt = page_cnt[0]
-        page_ptr = seqlens % self.page_size
-        page_ptr = torch.where((seqlens != 0) & (page_ptr == 0), self.page_size, page_ptr)
-        ar = functools.partial(torch.arange, device=self.device, dtype=torch.int)
+            seqlens = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self.device)
+        if seqlens.is_cuda:
+            most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
+            table = build_page_table(seqlens, torch.zeros_like(seqlens), 0, self.page_size,
+                                     max_blocks=max(self.page_cnt_from_length(most), 1))
+            indptr, indices, last = (table[k] for k in ("kv_indptr", "kv_indices", "last_page_offset"))
+            if attention_mask is not None:
+                indices = indices[:int(indptr[-1])]
+            elif self.length == 0:
+                indices = indices[:0]
+        else:
+            page_cnt = self.page_cnt_from_length(seqlens)
+            indptr = torch.nn.functional.pad(torch.cumsum(page_cnt, 0), (1, 0)).to(torch.int32)
+            indices = torch.cat([torch.arange(n, dtype=torch.int32) * self.batch_size + b for b, n in enumerate(page_cnt.tolist())])
+            last = (seqlens - (page_cnt - 1).clamp(min=0) * self.page_size).to(torch.int32)
         return {
             "kv_data": self.pages,
-            "kv_indptr": (ar(0, self.batch_size + 1) * page_cnt).to(torch.int32).contiguous(),
-            "kv_indices": ((ar(page_cnt) * self.batch_size).unsqueeze(0) + ar(self.batch_size).unsqueeze(1)).view(-1).to(torch.int32).contiguous(),
-            "last_page_offset": page_ptr.to(torch.int32).contiguous(),
+            "kv_indptr": indptr,
+            "kv_indices": indices,
+            "last_page_offset": last,
             "kv_param": self.scales,
         }
 
