@@ -5,9 +5,10 @@
 //   s_t <q_r, c_t> - z_t sum(q_r),   and value = s' c' - z'  (s', z' the value parameters).
 // The tensor cores see only small whole numbers: a code is put into the mantissa of 16.0 (fp16 0x4C00 | c << 6 is exactly
 // 16 + c), two logical instructions per pair of codes and no arithmetic, and the 16 is taken out of the sums in fp32.
-// Weights: w_t = exp2(score_t + log2 s'_t - M) with M the running maximum of that exponent, so that the value scale is
-// inside the weight, the largest weight is 1 and rounding w to fp16 (the B operand of the second product) is a relative
-// error of at most 2^-11 / 2 for every token that matters; the sums
+// Weights: w_t = exp2(score_t + log2 s'_t - M) with M following the running maximum of that exponent in steps of at least
+// 8 (so that sums are rarely multiplied through), times 2^6: the value scale is inside the weight, the largest weight lies
+// between 2^6 and 2^14 and rounding w to fp16 (the B operand of the second product) is a relative error of at most 2^-11
+// down to weights 2^-20 of the largest; the sums
 //   l = sum w / s'_t  (the softmax denominator)  and  y = sum w (z'_t / s'_t - 7.5)
 // are of the unrounded w in fp32, and the centre 7.5 of the codes is taken out with the ROUNDED weights (one more MMA
 // row of ones), so that a rounding error of w meets c' - 7.5 and not 16 + c':
@@ -66,35 +67,12 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-// nibbles J and J + 4 of a word as the fp16 pair (16 + c_J, 16 + c_{J+4})
-template <int J>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  const uint32_t x = J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6;
-  return (x & 0x03C003C0u) | 0x4C004C00u;
-}
-
 // Row of a block's stage that holds 64 bytes of codes: 16-byte chunk ch of row r lies at chunk ch ^ rw_swz(r).
 __device__ __forceinline__ int rw_swz(int r) { return (r & 2); }
 // Token of a 16-token tile in fragment slot s: the four tokens that a V fragment reads at once, and the two of a K
 // fragment, differ in the bank halves that their rows start in.
 __device__ __forceinline__ int rw_token_even(int c) { return c; }              // slot 2 c
 __device__ __forceinline__ int rw_token_odd(int c) { return 4 + (c ^ 1); }     // slot 2 c + 1
-
-__device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float peer_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 peer_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 
 __device__ __forceinline__ void rw_store_row(const KvAttendParams& p, const KvTile& w, int head_kv, int r, int d4, float4 v, float inv) {
   const int row = w.row0 + r;
@@ -116,7 +94,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int unit = blockIdx.x / p.splits;
   uint32_t crank = 0;
-  if (p.splits > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  if (p.splits > 1) crank = kv_cluster_rank();
   const int head_kv = unit % p.kv_heads;
   const KvTile w = kv_find_tile(p, unit / p.kv_heads, R, lane);
   if (w.rows == 0) return;                              // the whole cluster has the same tile
@@ -301,7 +279,8 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top[n][k] = fmaxf(top[n][k], __shfl_xor_sync(0xffffffffu, top[n][k], x));
-        grows |= top[n][k] > m[n][k];
+        top[n][k] = top[n][k] > m[n][k] + 8.0f ? top[n][k] : m[n][k];
+        grows |= top[n][k] != m[n][k];
       }
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -309,8 +288,8 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         float f[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float mn = fmaxf(m[n][k], top[n][k]);
-          f[k] = mn == -INFINITY ? 1.0f : exp2f(m[n][k] - mn);
+          const float mn = top[n][k];
+          f[k] = mn != m[n][k] ? ex2(m[n][k] - mn) : 1.0f;
           m[n][k] = mn;
           l[n][k] *= f[k];
           y[n][k] *= f[k];
@@ -326,12 +305,12 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     uint32_t pb[2][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : 6.0f - m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : 6.0f - m[n][1];
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float w0 = exp2f(s[a][n][2 * h] - m0), w1 = exp2f(s[a][n][2 * h + 1] - m1);
+          const float w0 = ex2(s[a][n][2 * h] + m0), w1 = ex2(s[a][n][2 * h + 1] + m1);
           if (edge) {
             // a hidden token leaves the sums alone whatever its parameters hold
             if (w0 != 0.0f) { l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]); }
@@ -404,7 +383,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
 #pragma unroll
     for (int x = 0; x < kRwWarps; ++x) {
       if (sh.m[x][r] == -INFINITY && sh.l[x][r] == 0.0f) continue;     // a warp that saw no token of the row
-      const float f = exp2f(sh.m[x][r] - mm);
+      const float f = ex2(sh.m[x][r] - mm);
       const float4 v = *reinterpret_cast<const float4*>(merge + ((size_t)x * R + r) * kRwORow + 4 * lane);
       ll = fmaf(sh.l[x][r], f, ll);
       acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
@@ -417,24 +396,24 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     }
   }
   if (p.splits > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    kv_cluster_barrier();
     // the CTAs of the cluster deal out the rows
     for (int r = (int)crank + p.splits * warp; r < w.rows; r += p.splits * kRwWarps) {
       float mm = -INFINITY;
-      for (int x = 0; x < p.splits; ++x) mm = fmaxf(mm, peer_f32(peer_addr(&sh.part_m[r], x)));
+      for (int x = 0; x < p.splits; ++x) mm = fmaxf(mm, kv_peer_f32(kv_peer_addr(&sh.part_m[r], x)));
       float ll = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int x = 0; x < p.splits; ++x) {
-        const float mx = peer_f32(peer_addr(&sh.part_m[r], x)), lx = peer_f32(peer_addr(&sh.part_l[r], x));
+        const float mx = kv_peer_f32(kv_peer_addr(&sh.part_m[r], x)), lx = kv_peer_f32(kv_peer_addr(&sh.part_l[r], x));
         if (mx == -INFINITY && lx == 0.0f) continue;
-        const float f = exp2f(mx - mm);
-        const float4 v = peer_f32x4(peer_addr(&sh.part_o[r][4 * lane], x));
+        const float f = ex2(mx - mm);
+        const float4 v = kv_peer_f32x4(kv_peer_addr(&sh.part_o[r][4 * lane], x));
         ll = fmaf(lx, f, ll);
         acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
       }
       rw_store_row(p, w, head_kv, r, 4 * lane, acc, ll != 0.0f ? 1.0f / ll : 0.0f);
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    kv_cluster_barrier();
   }
 }
 
@@ -516,5 +495,6 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
   p.page_div = make_fastdiv((uint32_t)page_size); p.group_div = make_fastdiv((uint32_t)group);
   p.window = window; p.sinks = window > 0 ? sink_tokens : 0; p.hadamard_q = hadamard_q;
   p.status = kernel_status_ptr();
-  return launch_kv_attend_rows(p, max_q_len * group, (cudaStream_t)stream);
+  const int64_t rows = max_q_len * group;
+  return rows > 64 ? launch_kv_attend_tc(p, rows, (cudaStream_t)stream) : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
 }

@@ -139,11 +139,6 @@ struct KvDecodeParams {
 
 constexpr int kKvDecWarps = 8;
 
-__device__ __forceinline__ uint32_t kv_cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void kv_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

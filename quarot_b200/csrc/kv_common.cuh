@@ -33,6 +33,47 @@ __device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) {
 }
 #endif
 
+#ifdef __CUDACC__
+// Nibbles J and J + 4 of a word (or of two 16-bit halves) as the fp16 pair (16 + c_J, 16 + c_{J+4}): a code in the upper
+// mantissa bits of 16.0.
+template <int J>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  const uint32_t x = J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6;
+  return (x & 0x03C003C0u) | 0x4C004C00u;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Clusters that share a token axis.
+__device__ __forceinline__ uint32_t kv_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void kv_cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the place of `local` in the shared memory of CTA `rank` of the cluster, and loads from there
+__device__ __forceinline__ uint32_t kv_peer_addr(const void* local, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float kv_peer_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 kv_peer_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+#endif
+
 // Division of 0 <= n < 2^31 by a fixed d >= 1 as one wide multiplication: with s = ceil(log2 d) and
 // m = ceil(2^(31+s) / d) <= 2^32 - 1 (2^31 for d = 1), m d - 2^(31+s) < d <= 2^s, hence floor(n m / 2^(31+s)) = floor(n / d).
 struct FastDiv {
@@ -157,5 +198,6 @@ __device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) { return
 #endif
 
 int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
+int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
 
 }  // namespace qr
