@@ -3,19 +3,24 @@
 //
 // One CTA takes up to 256 query rows of one (sequence, KV head) -- row = (new token, query head of the group), so a
 // group shares the tokens it reads -- as two tiles of 128, and walks over the visible tokens in blocks of 128:
-//   S_i = Q_i (16 + Ck)^T          tcgen05.mma 128 x 128 x 128, Q and the key codes in shared memory
+//   S_i = Q_i (16 + Ck)^T          tcgen05.mma 128 x 64 x 128 twice, Q and the key codes in shared memory
 //   P_i = softmax weights          S from tensor memory to registers and back as fp16
-//   O_i += P_i (Cv - 8)            P from tensor memory, the value codes, transposed, in shared memory
+//   O_i += P_i (Cv - 7.5)          P from tensor memory, the value codes, transposed, in shared memory
 // The tensor cores see the codes, which are exact in fp16, never dequantised keys or values: scales and zero points
 // of a token are folded into its column of S and into its weight, as described in kv_attend_rows.cu:
 //   score_t = s_t S_t - (z_t + 16 s_t) sum(q),   w_t = exp2(score_t + log2 s'_t - M),
-//   l = sum w / s',   y = sum w (z' / s' - 8),   o = (O - y) / l,
-// which leaves the fp16 rounding of w as the only one in front of the result's own.  M follows the running maximum in
-// steps: it moves (and O is multiplied through, a rare pass over tensor memory) only where a block's maximum is more than
-// 2^8 above it, weights are scaled by 2^6, so they stay below 2^14 and the normal fp16 range reaches down to 2^-20.
+//   l = sum w / s',   y = sum w (z' / s' - 7.5),   o = (O - y) / l,
+// which leaves the fp16 rounding of w as the only one in front of the result's own (7.5 is the centre of the codes: the
+// rounding meets at most 7.5).  M does not follow the maximum: it is set 6 below the first one, so that the largest weight
+// is about 2^6, and moves only where a weight would pass 2^15 (everything summed up is then multiplied through, by powers
+// of two, which round nothing).  So weights are made in one pass, without looking for a maximum first, and the normal
+// fp16 range reaches down to at least 2^-20 of the largest.
 //
-// Warps: two warpgroups make the softmax of one row tile each, so that one works while the tensor cores are on the other's
-// tile (S_0, O_0, S_1, O_1 in that order); four warps unpack the next block; one thread issues the MMAs.  A token's
+// S is made and used in halves of 64 tokens with a buffer each, the weights lie over the half of S they came from: while
+// the softmax is on one half, the tensor cores make the products of the other and then its next scores.
+//
+// Warps: two warpgroups make the softmax of one row tile each, four warps unpack keys, four unpack values, two issue the
+// MMAs of a row tile each.  A token's
 // five numbers are per COLUMN of S, so a thread that owned a whole row would have to read all of them: S is read
 // with the 16x256b shape instead, which gives a lane two neighbouring columns of eight in four rows, the numbers of
 // a column pair serve four rows, and a row's maximum is two shuffles away.  Unpacking: keys as they stand (two
@@ -23,8 +28,8 @@
 // eight tokens, so that both operands are K-major 128-byte-swizzled tiles written by conflict-free 16-byte stores.
 // Few tiles: a cluster shares the token axis and merges through distributed shared memory.
 //
-// Registers: 512 threads start with 128 each; the softmax warpgroups go up to 192, the unpacking warps down to 88 and the
-// MMA warpgroup to 40 (sum 512 x 128).  All waits are bounded (tc_ptx.cuh).
+// Registers: 20 warps, five per scheduler, start with 96 each; the softmax warps go up to 160, the unpacking warps down to
+// 64 and the MMA warpgroup to 32 (per scheduler 2 x 160 + 2 x 64 + 32 = 5 x 96).  All waits are bounded (tc_ptx.cuh).
 #include "kv_common.cuh"
 #include "tc_ptx.cuh"
 
@@ -32,17 +37,20 @@
 
 namespace qr {
 
-constexpr int kAtThreads = 512;
+constexpr int kAtThreads = 640;
 constexpr int kAtRows = 256;
 constexpr int kAtTok = 128;
 constexpr int kAtTile = 128 * 128 * 2;                    // bytes of one 128 x 128 fp16 operand tile
-constexpr int kAtPairFloats = 12;                         // per column pair: ks ks kz kz | lv lv rv rv | zv zv - -
+constexpr int kAtPairFloats = 12;                         // per column pair: ks ks kz kz | lv lv - - | rv rv zv zv
+constexpr uint32_t kTmem = 0;                             // the CTA owns all 512 columns of tensor memory, from 0 on
 constexpr int kAtParStages = 3;
-constexpr uint32_t kAtIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // fp16 x fp16 -> fp32, K-major, 128 x 128
+constexpr float kAtTop = 15.0f;                           // weights are at most 2^15
+constexpr uint32_t kAtIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);    // fp16 x fp16 -> fp32, K-major, 128 x 64
+constexpr uint32_t kAtIdescO = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // 128 x 128
 
 struct AtShared {
   float par[kAtParStages][kAtTok / 2][kAtPairFloats];
-  long long row[2][kAtTok];                               // rows of the key block of the tokens, -1: not read
+  long long row[2][2][kAtTok];                            // [keys / values][block & 1] rows of the tokens, -1: not read
   float qsum[kAtRows];
   int pos[kAtRows];
   float m[kAtRows], l[kAtRows];
@@ -53,22 +61,52 @@ struct AtShared {
 constexpr size_t kAtSmem = 1024 + 6 * kAtTile + sizeof(AtShared);
 static_assert(kAtSmem <= 227 * 1024, "shared memory");
 
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t acc) {
+// One look at a barrier (a try_wait may sleep for some thousand cycles).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 da, {%1, %3};\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(kDescHiKmajorSw128), "r"(kAtIdesc), "r"(acc) : "memory");
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok;
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t acc) {
+// The MMAs and commits are written for a warp whose lanes all run the issuing loop: addresses and descriptors then stay in
+// uniform registers, and only the instruction itself is predicated on the elected lane.
+__device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(kDescHiKmajorSw128), "r"(kAtIdesc), "r"(acc) : "memory");
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%2, %4};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %5, p;\n\t}"
+      ::"r"(lead), "r"(d), "r"(a_lo), "r"(b_lo), "n"(kDescHiKmajorSw128), "n"(kAtIdescS), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], db, %5, p;\n\t}"
+      ::"r"(lead), "r"(d), "r"(a_tmem), "r"(b_lo), "n"(kDescHiKmajorSw128), "n"(kAtIdescO), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(uint32_t lead, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}"
+      ::"r"(lead), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r));
+  return r;
 }
 // 16 lanes x 64 columns of tensor memory: lane (g, c) gets columns 8 k + 2 c, + 1 of row g in r[4 k], r[4 k + 1] and of row
 // g + 8 in r[4 k + 2], r[4 k + 3].  No wait: tmem_ld_done() below.
@@ -83,25 +121,29 @@ __device__ __forceinline__ void tmem_ld_16x256_x8(uint32_t taddr, uint32_t* r) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st_16x256_x8(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st_16x256_x4(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-        "r"(taddr) : "memory");
-}
-// 16 lanes x 32 columns of fp16 pairs (64 matrix columns): r[2 k] is row g, r[2 k + 1] row g + 8, column pair 4 k + c.
-__device__ __forceinline__ void tmem_st_16x128_x8(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], "
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
       ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(taddr) : "memory");
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+// 16 lanes x 16 columns of fp16 pairs (32 matrix columns): r[2 k] is row g, r[2 k + 1] row g + 8, column pair 4 k + c.
+__device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x128_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
 }
 // Waits for the loads of this thread; the registers pass through, so that no use of them moves above the wait.
 template <int N>
@@ -133,9 +175,9 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   return r;
 }
 template <int J>
-__device__ __forceinline__ uint32_t at_centred_pair(uint32_t w) {     // 16 + c - 24, exact
+__device__ __forceinline__ uint32_t at_centred_pair(uint32_t w) {     // 16 + c - 23.5, exact
   const uint32_t x = code_pair<J>(w);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(24.0f));
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(23.5f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -150,17 +192,178 @@ __device__ __forceinline__ __half* at_out_row(const KvAttendParams& p, const KvT
   return p.o + (w.tok0 + tok) * p.o_ts + (int64_t)(head_kv * p.group + hh) * p.o_hs;
 }
 
+// What a lane of a softmax warp keeps of its four rows (g + 8 x of the warp's 32).
+struct AtRows {
+  float m[4], qs[4];
+  uint64_t l2[4], y2[4];
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// -infinity for the columns of a pair that a row at position pos does not see; t: token of the first
+__device__ __forceinline__ void at_hide(float& v0, float& v1, int t, int pos, int window, int sinks) {
+  const int lo = window > 0 ? pos - window : -1;
+  if (t > pos || (t <= lo && t >= sinks)) v0 = -INFINITY;
+  if (t + 1 > pos || (t + 1 <= lo && t + 1 >= sinks)) v1 = -INFINITY;
+}
+
+// The exponents of 32 columns, relative to M, in place of S; the lane's largest is returned.
+__device__ __forceinline__ float at_scores(uint32_t (&s)[2][16], const float* par, const AtRows& w) {
+  uint64_t off[4], qq[4];
+  float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    off[x] = f2_pack(-w.m[x], -w.m[x]);                   // +infinity before the row has seen a token: M has to be set
+    qq[x] = f2_pack(w.qs[x], w.qs[x]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
+    const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
+    const uint64_t ks = f2_pack(a.x, a.y), kz = f2_pack(a.z, a.w), lv = f2_pack(b.x, b.y);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
+      uint64_t v = f2_fma(kz, qq[x], lv);
+      v = f2_fma(ks, f2_pack(__uint_as_float(r[0]), __uint_as_float(r[1])), v);
+      float v0, v1;
+      f2_unpack(f2_add(v, off[x]), v0, v1);
+      if (x & 1) top1 = max3(top1, v0, v1); else top0 = max3(top0, v0, v1);
+      r[0] = __float_as_uint(v0);
+      r[1] = __float_as_uint(v1);
+    }
+  }
+  return fmaxf(top0, top1);
+}
+
+// Hides what the rows do not see (pos: positions of the warp's rows, t: token of the lane's first column); the largest of
+// what is left.
+__device__ __forceinline__ float at_mask(uint32_t (&s)[2][16], const int* pos, int t, int window, int sinks) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int ps = pos[8 * x];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
+      float v0 = __uint_as_float(r[0]), v1 = __uint_as_float(r[1]);
+      at_hide(v0, v1, t + 8 * k, ps, window, sinks);
+      top = max3(top, v0, v1);
+      r[0] = __float_as_uint(v0);
+      r[1] = __float_as_uint(v1);
+    }
+  }
+  return top;
+}
+
+// The weights of 32 columns: into the sums, and as fp16 to tensor memory.
+__device__ __forceinline__ void at_weights(const uint32_t (&s)[2][16], const float* par, AtRows& w, uint32_t t_p) {
+  uint32_t pk[2][8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float4 b = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats + 8);
+    const uint64_t rv = f2_pack(b.x, b.y), zv = f2_pack(b.z, b.w);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
+      const float w0 = ex2(__uint_as_float(r[0])), w1 = ex2(__uint_as_float(r[1]));
+      const uint64_t ww = f2_pack(w0, w1);
+      w.l2[x] = f2_fma(ww, rv, w.l2[x]);
+      w.y2[x] = f2_fma(ww, zv, w.y2[x]);
+      const __half2 wh = __floats2half2_rn(w0, w1);
+      pk[x >> 1][2 * k + (x & 1)] = *reinterpret_cast<const uint32_t*>(&wh);
+    }
+  }
+  tmem_st_16x128_x4(t_p, pk[0]);
+  tmem_st_16x128_x4(t_p + (16u << 16), pk[1]);
+}
+
+// The largest exponents of the four rows over 32 columns, relative to nothing.
+__device__ __forceinline__ void at_tops(uint32_t (&s)[2][16], const float* par, const AtRows& w, float (&top)[4], bool edge, const int* pos, int t,
+                                        int window, int sinks) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) top[x] = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
+    const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
+      float v0 = fmaf(a.x, __uint_as_float(r[0]), fmaf(a.z, w.qs[x], b.x)), v1 = fmaf(a.y, __uint_as_float(r[1]), fmaf(a.w, w.qs[x], b.y));
+      if (edge) at_hide(v0, v1, t + 8 * k, pos[8 * x], window, sinks);
+      top[x] = max3(top[x], v0, v1);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+  }
+}
+
+// Multiplies columns of O (fp32) by the factors of the four rows.
+__device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
+#pragma unroll 1
+  for (int q = 0; q < 8; ++q) {
+    uint32_t o[16];
+    const uint32_t at = t_o + (q >> 1) * 32 + ((uint32_t)(q & 1) << 20);
+    tmem_ld_16x256_x4(at, o);
+    tmem_ld_done<16>(o);
+    const float fa = q & 1 ? f[2] : f[0], fb = q & 1 ? f[3] : f[1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? fb : fa));
+    tmem_st_16x256_x4(at, o);
+  }
+  tmem_st_done();
+}
+
+// M has become mn: l, y and the weights of the first `pieces` x 32 columns, which are in tensor memory, follow.  The
+// factors are powers of two (M moves in whole steps) or 0.
+__device__ __forceinline__ void at_follow(AtRows& w, const float (&mn)[4], float (&f)[4], int pieces, uint32_t t_p) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    f[x] = mn[x] == w.m[x] ? 1.0f : w.m[x] == -INFINITY ? 0.0f : ex2(w.m[x] - mn[x]);
+    w.m[x] = mn[x];
+    const uint64_t ff = f2_pack(f[x], f[x]);
+    w.l2[x] = f2_fma(w.l2[x], ff, 0);
+    w.y2[x] = f2_fma(w.y2[x], ff, 0);
+  }
+  tmem_st_done();
+#pragma unroll 1
+  for (int q = 0; q < 2 * pieces; ++q) {
+    uint32_t h[8];
+    const uint32_t at = t_p + (q >> 1) * 16 + ((uint32_t)(q & 1) << 20);
+    tmem_ld_16x128_x4(at, h);
+    tmem_ld_done<8>(h);
+    const float fa = q & 1 ? f[2] : f[0], fb = q & 1 ? f[3] : f[1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+      const float ff = e & 1 ? fb : fa;
+      const __half2 r = __floats2half2_rn(v.x * ff, v.y * ff);
+      h[e] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    tmem_st_16x128_x4(at, h);
+  }
+  tmem_st_done();
+}
+
 __global__ void __launch_bounds__(kAtThreads, 1)
 kv_attend_tc_kernel(const KvAttendParams p) {
   extern __shared__ unsigned char s_raw[];
   const uint32_t base = (smem_u32(s_raw) + 1023u) & ~1023u;
   unsigned char* smem = s_raw + (base - smem_u32(s_raw));
-  // [Q tile 0, Q tile 1][K 2 stages][V 2 stages][AtShared]; the merge area is Q and K, the fp16 result goes through Q
+  // [Q tile 0, Q tile 1][K 2 stages][V 2 stages][AtShared]; the merge area is Q and K, the fp16 result of a row tile goes
+  // through its Q tile
   const uint32_t s_q = base, s_k = base + 2 * kAtTile, s_v = base + 4 * kAtTile;
   AtShared& sh = *reinterpret_cast<AtShared*>(smem + 6 * kAtTile);
   const uint32_t bars = smem_u32(sh.bars);
   const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, par_full = bars + 64, s_full = bars + 88,
-                 p_full = bars + 104, o_full = bars + 120;                          // 2, 2, 2, 2, 3, 2, 2, 2
+                 p_full = bars + 120, pv_done = bars + 152, o_full = bars + 168;   // 2 2 2 2 3 [2][2] [2][2] 2 2
   volatile int* abort_flag = &sh.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t crank = 0;
@@ -179,195 +382,165 @@ kv_attend_tc_kernel(const KvAttendParams p) {
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(k_full + 8 * s, 4); mbar_init(k_empty + 8 * s, 1);
-      mbar_init(v_full + 8 * s, 4); mbar_init(v_empty + 8 * s, 1);
-      mbar_init(s_full + 8 * s, 1); mbar_init(p_full + 8 * s, 4); mbar_init(o_full + 8 * s, 1);
+      mbar_init(k_full + 8 * s, 4); mbar_init(k_empty + 8 * s, tiles);
+      mbar_init(v_full + 8 * s, 4); mbar_init(v_empty + 8 * s, tiles);
+      mbar_init(s_full + 16 * s, 1); mbar_init(s_full + 16 * s + 8, 1);
+      mbar_init(p_full + 16 * s, 4); mbar_init(p_full + 16 * s + 8, 4);
+      mbar_init(pv_done + 8 * s, 1); mbar_init(o_full + 8 * s, 1);
     }
     for (int s = 0; s < kAtParStages; ++s) mbar_init(par_full + 8 * s, 4);
     sh.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
   }
   // query rows: 8 dimensions 8 i .. 8 i + 7 lie as 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart
-  for (int r = warp; r < 128 * tiles; r += kAtThreads / 32) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int pos = -1;
-    if (r < w.rows) {
-      const int row = w.row0 + r;
-      const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
-      pos = w.pos0 + tok;
-      load4_f16(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane, x);
+  constexpr int kWarps = kAtThreads / 32, kTogether = 7;  // loads in flight per warp: two rounds for 256 rows
+  for (int r0 = warp; r0 < 128 * tiles; r0 += kTogether * kWarps) {
+    uint2 raw[kTogether];
+    int pos[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int r = r0 + u * kWarps;
+      raw[u] = make_uint2(0, 0);
+      pos[u] = -1;
+      if (r < w.rows) {
+        const int row = w.row0 + r;
+        const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
+        pos[u] = w.pos0 + tok;
+        raw[u] = *reinterpret_cast<const uint2*>(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int r = r0 + u * kWarps;
+      if (r >= 128 * tiles) break;
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw[u].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw[u].y));
+      float x[4] = {lo.x, lo.y, hi.x, hi.y};
       if (p.hadamard_q) {
         fwht128_warp(x, lane);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
       }
-    }
-    float sum = x[0] + x[1] + x[2] + x[3];
+      float sum = x[0] + x[1] + x[2] + x[3];
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    const bool odd = lane & 1;
-    const float give0 = odd ? x[0] : x[2], give1 = odd ? x[1] : x[3];
-    const float got0 = __shfl_xor_sync(0xffffffffu, give0, 1), got1 = __shfl_xor_sync(0xffffffffu, give1, 1);
-    const __half2 h0 = odd ? __floats2half2_rn(got0, x[2]) : __floats2half2_rn(x[0], got0);
-    const __half2 h1 = odd ? __floats2half2_rn(got1, x[3]) : __floats2half2_rn(x[1], got1);
-    const int rr = r & 127, ch = (lane >> 1) & 7;
-    unsigned char* dst = smem + (r >> 7) * kAtTile + (lane >> 4) * (kAtTile / 2) + rr * 128 + ((ch ^ (rr & 7)) << 4) + (odd ? 8 : 0);
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&h0);
-    u.y = *reinterpret_cast<const uint32_t*>(&h1);
-    *reinterpret_cast<uint2*>(dst) = u;
-    if (lane == 0) { sh.qsum[r] = sum; sh.pos[r] = pos; }
+      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      const bool odd = lane & 1;
+      const float give0 = odd ? x[0] : x[2], give1 = odd ? x[1] : x[3];
+      const float got0 = __shfl_xor_sync(0xffffffffu, give0, 1), got1 = __shfl_xor_sync(0xffffffffu, give1, 1);
+      const __half2 h0 = odd ? __floats2half2_rn(got0, x[2]) : __floats2half2_rn(x[0], got0);
+      const __half2 h1 = odd ? __floats2half2_rn(got1, x[3]) : __floats2half2_rn(x[1], got1);
+      const int rr = r & 127, ch = (lane >> 1) & 7;
+      unsigned char* dst = smem + (r >> 7) * kAtTile + (lane >> 4) * (kAtTile / 2) + rr * 128 + ((ch ^ (rr & 7)) << 4) + (odd ? 8 : 0);
+      uint2 q;
+      q.x = *reinterpret_cast<const uint32_t*>(&h0);
+      q.y = *reinterpret_cast<const uint32_t*>(&h1);
+      *reinterpret_cast<uint2*>(dst) = q;
+      if (lane == 0) { sh.qsum[r] = sum; sh.pos[r] = pos[u]; }
+    }
   }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
 
   if (warp < 8) {
-    // ---------------------------------------------------------------- softmax of one row tile
-    regs_inc<192>();
+    // ---------------------------------------------------------------- softmax: 32 rows of a row tile
+    regs_inc<160>();
     const int i = warp >> 2, g = lane >> 2, c = lane & 3;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;                    // first tensor-memory lane of the warp, << 16
-    const uint32_t t_s = tmem + i * 128 + lanes, t_o = tmem + 256 + i * 128 + lanes;
+    const uint32_t t_s = kTmem + i * 128 + lanes, t_o = kTmem + 256 + i * 128 + lanes;
     const int row0 = i * 128 + (warp & 3) * 32;                           // the lane's rows: row0 + g + 8 x, x = 0 .. 3
-    float m[4], qs[4];
-    uint64_t l2[4], y2[4];
-    int ps[4];
+    const int* pos = &sh.pos[row0 + g];
+    AtRows rw;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      m[x] = -INFINITY;
-      l2[x] = 0; y2[x] = 0;
-      qs[x] = i < tiles ? sh.qsum[row0 + g + 8 * x] : 0.0f;
-      ps[x] = i < tiles ? sh.pos[row0 + g + 8 * x] : -1;
+      rw.m[x] = -INFINITY;
+      rw.l2[x] = 0; rw.y2[x] = 0;
+      rw.qs[x] = i < tiles ? sh.qsum[row0 + g + 8 * x] : 0.0f;
     }
     bool ok = i < tiles;
-    for (int j = 0; ok && j < n; ++j) {
-      const int t0 = kv_block_index(blk, begin + j) * kAtTok;
-      const bool edge = t0 + kAtTok - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kAtTok - 1 >= p.sinks);
-      const int ring = j % kAtParStages;
-      ok = mbar_wait(par_full + 8 * ring, (j / kAtParStages) & 1, abort_flag, p.status, 71) &&
-           mbar_wait(s_full + 8 * i, j & 1, abort_flag, p.status, 72);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t s[2][64];                                  // [rows 0 - 15 / 16 - 31 of the warp][4 k + ..]
-      tmem_ld_16x256_x8(t_s, s[0]);
-      tmem_ld_16x256_x8(t_s + (16u << 16), s[1]);
-      tmem_ld_16x256_x8(t_s + 64, s[0] + 32);
-      tmem_ld_16x256_x8(t_s + 64 + (16u << 16), s[1] + 32);
-      tmem_ld_done<64>(s[0]);
-      tmem_ld_done<64>(s[1]);
-      const float* par = &sh.par[ring][c][0];
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    // 32 columns of half h: exponents, M where it has to move, weights
+    auto piece = [&](uint32_t (&s)[2][16], int h, int part, const float* par, bool edge, int t) {
+      const uint32_t t_sb = t_s + 64 * (h & 1);
+      float top = at_scores(s, par, rw);
+      if (edge) top = at_mask(s, pos, t, p.window, p.sinks);
+      if (__any_sync(0xffffffffu, top > kAtTop)) {
+        // a weight would pass 2^15, or a row sees its first token
+        tmem_ld_16x256_x4(t_sb + 32 * part, s[0]);
+        tmem_ld_16x256_x4(t_sb + 32 * part + (16u << 16), s[1]);
+        tmem_ld_done<16>(s[0]);
+        tmem_ld_done<16>(s[1]);
+        float mn[4], f[4];
+        at_tops(s, par, rw, mn, edge, pos, t, p.window, p.sinks);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
-        const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
-        const uint64_t ks = f2_pack(a.x, a.y), kz = f2_pack(a.z, a.w), lv = f2_pack(b.x, b.y);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
-          uint64_t v = f2_fma(kz, f2_pack(qs[x], qs[x]), lv);
-          v = f2_fma(ks, f2_pack(__uint_as_float(r[0]), __uint_as_float(r[1])), v);
-          float v0, v1;
-          f2_unpack(v, v0, v1);
-          if (edge) {
-            const int t = t0 + 8 * k + 2 * c;
-            const int lo = p.window > 0 ? ps[x] - p.window : -1;
-            if (t > ps[x] || (t <= lo && t >= p.sinks)) v0 = -INFINITY;
-            if (t + 1 > ps[x] || (t + 1 <= lo && t + 1 >= p.sinks)) v1 = -INFINITY;
-          }
-          top[x] = fmaxf(top[x], fmaxf(v0, v1));
-          r[0] = __float_as_uint(v0);
-          r[1] = __float_as_uint(v1);
+        for (int x = 0; x < 4; ++x) mn[x] = mn[x] - rw.m[x] > kAtTop ? ceilf(mn[x]) - 1.0f : rw.m[x];
+        at_follow(rw, mn, f, part, t_sb);
+        if (h > 0) {                                      // the products of half h - 1 may still be on their way
+          ok = mbar_wait(pv_done + 8 * i, (h - 1) & 1, abort_flag, p.status, 73) && ok;
+          tc_fence_after();
+          at_scale_o(t_o, f);
         }
+        at_scores(s, par, rw);
+        if (edge) at_mask(s, pos, t, p.window, p.sinks);
       }
-      bool grows = false;
-      float mn[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        mn[x] = top[x] > m[x] + 8.0f ? top[x] : m[x];
-        grows |= mn[x] != m[x];
-      }
-      if (__any_sync(0xffffffffu, grows)) {
-        float f[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          f[x] = mn[x] != m[x] ? ex2(m[x] - mn[x]) : 1.0f;
-          m[x] = mn[x];
-          const uint64_t ff = f2_pack(f[x], f[x]);
-          l2[x] = f2_fma(l2[x], ff, 0);
-          y2[x] = f2_fma(y2[x], ff, 0);
-        }
-        if (j > 0) {                                      // the products of the blocks before are complete: S follows them
+      // the weights take the place of columns of S that are in registers
+      at_weights(s, par, rw, t_sb + 16 * part);
+    };
+    // two pieces of 32 columns per half block; the next piece is on its way while one is worked on
+    uint32_t sa[2][16], sb[2][16];                        // [rows 0 - 15 / 16 - 31 of the warp][..]
+    int ring = 0, ring_phase = 0;
+    bool fetched = false;
 #pragma unroll 1
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t o[32];
-            const uint32_t at = t_o + (q4 >> 1) * 64 + ((uint32_t)(q4 & 1) << 20);
-            tmem_ld_16x256_x8(at, o);
-            tmem_ld_done<32>(o);
-            const float fa = q4 & 1 ? f[2] : f[0], fb = q4 & 1 ? f[3] : f[1];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? fb : fa));
-            tmem_st_16x256_x8(at, o);
-          }
-          tmem_st_done();
-        }
+    for (int h = 0; ok && h < 2 * n; ++h) {               // half blocks of 64 tokens
+      const int buf = h & 1;
+      const uint32_t t_sb = t_s + 64 * buf;
+      if (!buf) {
+        if (h && ++ring == kAtParStages) { ring = 0; ring_phase ^= 1; }
+        ok = mbar_wait(par_full + 8 * ring, ring_phase, abort_flag, p.status, 71);
       }
-#pragma unroll
-      for (int hcol = 0; hcol < 2; ++hcol) {              // 64 columns at a time
-        uint32_t pk[2][16];
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const int k = 8 * hcol + kk;
-          const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 6);
-          const float2 d = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 8);
-          const uint64_t rv = f2_pack(b.x, b.y), zv = f2_pack(d.x, d.y);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
-            const float off = m[x] == -INFINITY ? 0.0f : 6.0f - m[x];
-            float v0, v1;
-            f2_unpack(f2_add(f2_pack(__uint_as_float(r[0]), __uint_as_float(r[1])), f2_pack(off, off)), v0, v1);
-            const float w0 = ex2(v0), w1 = ex2(v1);
-            const uint64_t ww = f2_pack(w0, w1);
-            if (edge) {
-              // a hidden token leaves the sums alone whatever its parameters hold
-              const uint64_t rr = f2_pack(w0 != 0.0f ? b.x : 0.0f, w1 != 0.0f ? b.y : 0.0f);
-              const uint64_t zz = f2_pack(w0 != 0.0f ? d.x : 0.0f, w1 != 0.0f ? d.y : 0.0f);
-              l2[x] = f2_fma(ww, rr, l2[x]);
-              y2[x] = f2_fma(ww, zz, y2[x]);
-            } else {
-              l2[x] = f2_fma(ww, rv, l2[x]);
-              y2[x] = f2_fma(ww, zv, y2[x]);
-            }
-            const __half2 wh = __floats2half2_rn(w0, w1);
-            pk[x >> 1][2 * kk + (x & 1)] = *reinterpret_cast<const uint32_t*>(&wh);
-          }
-        }
-        tmem_st_16x128_x8(t_s + 32 * hcol, pk[0]);        // over S, which is in registers
-        tmem_st_16x128_x8(t_s + 32 * hcol + (16u << 16), pk[1]);
+      if (!fetched) {
+        ok = mbar_wait(s_full + 16 * i + 8 * buf, (h >> 1) & 1, abort_flag, p.status, 72) && ok;
+        tc_fence_after();
+        tmem_ld_16x256_x4(t_sb, sa[0]);
+        tmem_ld_16x256_x4(t_sb + (16u << 16), sa[1]);
       }
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      const int t0 = kv_block_index(blk, begin + (h >> 1)) * kAtTok + 64 * buf;
+      const bool edge = t0 + 63 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + 63 >= p.sinks);
+      const float* par = &sh.par[ring][c + 32 * buf][0];
+      tmem_ld_done<16>(sa[0]);
+      tmem_ld_done<16>(sa[1]);
+      tmem_ld_16x256_x4(t_sb + 32, sb[0]);
+      tmem_ld_16x256_x4(t_sb + 32 + (16u << 16), sb[1]);
+      piece(sa, h, 0, par, edge, t0 + 2 * c);
+      tmem_ld_done<16>(sb[0]);
+      tmem_ld_done<16>(sb[1]);
+      // the scores of the next half do not depend on these weights: where they are there already, they are fetched ahead
+      fetched = h + 1 < 2 * n && __all_sync(0xffffffffu, mbar_test(s_full + 16 * i + 8 * (buf ^ 1), ((h + 1) >> 1) & 1));
+      if (fetched) {
+        tc_fence_after();
+        tmem_ld_16x256_x4(t_s + 64 * (buf ^ 1), sa[0]);
+        tmem_ld_16x256_x4(t_s + 64 * (buf ^ 1) + (16u << 16), sa[1]);
+      }
+      piece(sb, h, 1, par + 16 * kAtPairFloats, edge, t0 + 32 + 2 * c);
       tmem_st_done();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * i);
+      if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * buf);
     }
+    ok = __all_sync(0xffffffffu, ok);
     // sums over the four lanes of a row
     float l[4], y[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      float a, b;
-      f2_unpack(l2[x], a, b);
-      l[x] = a + b;
-      f2_unpack(y2[x], a, b);
-      y[x] = a + b;
+      float e, f;
+      f2_unpack(rw.l2[x], e, f);
+      l[x] = e + f;
+      f2_unpack(rw.y2[x], e, f);
+      y[x] = e + f;
 #pragma unroll
       for (int d = 1; d < 4; d <<= 1) {
         l[x] += __shfl_xor_sync(0xffffffffu, l[x], d);
@@ -375,9 +548,11 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       }
     }
     if (ok && n > 0) {
-      ok = mbar_wait(o_full + 8 * i, 0, abort_flag, p.status, 73);
+      ok = mbar_wait(o_full + 8 * i, 0, abort_flag, p.status, 80);
       ok = __all_sync(0xffffffffu, ok);
     }
+    // the merge area of one row tile lies over operands of the other, whose MMAs may still be running
+    if (p.splits > 1) asm volatile("bar.sync 3, 256;" ::: "memory");
     if (ok) {
       tc_fence_after();
 #pragma unroll 1
@@ -391,18 +566,18 @@ kv_attend_tc_kernel(const KvAttendParams p) {
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float ll = q4 & 1 ? l[2 + h] : l[h], yy = q4 & 1 ? y[2 + h] : y[h];
-          const int r = row0 + 16 * (q4 & 1) + 8 * h + g;
+        for (int hh = 0; hh < 2; ++hh) {
+          const float ll = q4 & 1 ? l[2 + hh] : l[hh], yy = q4 & 1 ? y[2 + hh] : y[hh];
+          const int r = row0 + 16 * (q4 & 1) + 8 * hh + g;
           const float inv = p.splits > 1 ? 1.0f : (ll != 0.0f ? 1.0f / ll : 0.0f);      // a row that sees nothing gives zeros
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float a = (__uint_as_float(o[4 * k + 2 * h]) - yy) * inv, b = (__uint_as_float(o[4 * k + 2 * h + 1]) - yy) * inv;
+            const float e0 = (__uint_as_float(o[4 * k + 2 * hh]) - yy) * inv, e1 = (__uint_as_float(o[4 * k + 2 * hh + 1]) - yy) * inv;
             const int col = 64 * (q4 >> 1) + 8 * k + 2 * c;
             if (p.splits > 1) {
-              *reinterpret_cast<float2*>(smem + at_part_off(r, col >> 2) + (col & 2) * 4) = make_float2(a, b);
+              *reinterpret_cast<float2*>(smem + at_part_off(r, col >> 2) + (col & 2) * 4) = make_float2(e0, e1);
             } else {
-              const __half2 hv = __floats2half2_rn(a, b);
+              const __half2 hv = __floats2half2_rn(e0, e1);
               *reinterpret_cast<__half2*>(smem + r * 256 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2) = hv;
             }
           }
@@ -411,7 +586,7 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       if (p.splits > 1) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (c == 0) { sh.m[row0 + g + 8 * x] = m[x]; sh.l[row0 + g + 8 * x] = l[x]; }
+          if (c == 0) { sh.m[row0 + g + 8 * x] = rw.m[x]; sh.l[row0 + g + 8 * x] = l[x]; }
       } else {
         __syncwarp();
         for (int rr = 0; rr < 32; ++rr) {                 // a row is 256 contiguous bytes
@@ -431,7 +606,8 @@ kv_attend_tc_kernel(const KvAttendParams p) {
         float ll = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int x = 0; x < p.splits; ++x) {
-          const float mx = kv_peer_f32(kv_peer_addr(&sh.m[r], x)), lx = kv_peer_f32(kv_peer_addr(&sh.l[r], x));
+          const float mx = kv_peer_f32(kv_peer_addr(&sh.m[r], x));
+          const float lx = kv_peer_f32(kv_peer_addr(&sh.l[r], x));
           if (mx == -INFINITY && lx == 0.0f) continue;
           const float f = ex2(mx - mm);
           const float4 v = kv_peer_f32x4(kv_peer_addr(smem + at_part_off(r, lane), x));
@@ -447,21 +623,17 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       }
       kv_cluster_barrier();                                  // nobody leaves while its shared memory may still be read
     }
-  } else if (warp < 12) {
-    // ---------------------------------------------------------------- unpacking of keys, values and parameters
-    regs_dec<88>();
-    const int tid = threadIdx.x - 256, pw = warp - 8;
+  } else if (warp < 16) {
+    // ---------------------------------------------------------------- unpacking: warps 8 - 11 keys and parameters, 12 - 15 values
+    regs_dec<64>();
+    const int tid = threadIdx.x & 127, pw = warp & 3;
+    const int what = warp >= 12;
     const int first_page = p.indptr[w.b];
     const int tokens = min(p_max + 1, w.seq_len);
     const size_t page_rows = (size_t)p.layers * 2 * p.kv_heads * p.page_size;
     const size_t row_k = ((size_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
     const size_t v_rows = (size_t)p.kv_heads * p.page_size;               // from a key row to the value row of its token
-    const float sm_scale = 0.08838834764831845f * 1.4426950408889634f;    // log2(e) / sqrt(128)
-    // keys: row (lane & 7) + 8 (warp + 4 it), 16-byte chunk lane / 8; values: tokens 64 (warp & 1) + 8 (lane & 7) + 0 .. 7,
-    // 8 bytes (16 dimensions) at 32 (warp / 2) + 8 (lane / 8)
-    const int kr = (lane & 7) + 8 * pw, kc = lane >> 3;
-    const int vt = 64 * (pw & 1) + 8 * (lane & 7), vb = 32 * (pw >> 1) + 8 * (lane >> 3);
-
+    const size_t row_0 = row_k + (what ? v_rows : 0);
     auto page_id = [&](int j) -> int {
       const int t = kv_block_index(blk, begin + j) * kAtTok + tid;
       return t < tokens ? __ldg(p.indices + first_page + fast_div(t, p.page_div)) : 0;
@@ -472,163 +644,188 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       if (t < tokens) {
         const int slot = t - fast_div(t, p.page_div) * p.page_size;
         const size_t page = min((size_t)(uint32_t)id, (size_t)p.num_pages - 1);        // an index outside the pool reads its last page
-        row = (long long)(page * page_rows + row_k + slot);
+        row = (long long)(page * page_rows + row_0 + slot);
       }
-      sh.row[j & 1][tid] = row;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      sh.row[what][j & 1][tid] = row;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + what) : "memory");
       return row;
     };
-    uint4 kw[4];
-    uint2 vw[8];
-    uint32_t kp = 0, vp = 0;
-    auto load_k = [&](int j) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const long long row = sh.row[j & 1][kr + 32 * it];
-        kw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.data + row * 64 + 16 * kc)) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    auto load_v = [&](int j) {
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const long long row = sh.row[j & 1][vt + it];
-        vw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint2*>(p.data + (row + (long long)v_rows) * 64 + vb)) : make_uint2(0, 0);
-      }
-    };
-    auto load_par = [&](long long row) {
-      kp = 0; vp = 0;
-      if (row >= 0) {
-        kp = __ldg(reinterpret_cast<const uint32_t*>(p.param + row));
-        vp = __ldg(reinterpret_cast<const uint32_t*>(p.param + row + v_rows));
-      }
-    };
-    bool ok = true;
+    // a wait that ran out of time sets the abort flag: the others end at once, and what is written then is read by nobody
     int id = 0;
-    if (n > 0) {
-      const long long row = put_rows(0, page_id(0));
-      load_par(row);
-      load_k(0);
-      load_v(0);
-      if (n > 1) id = page_id(1);
-    }
-    for (int j = 0; j < n; ++j) {
-      const int stage = j & 1, ring = j % kAtParStages;
-      {
-        // parameters of token tid; its slot of the ring is free: block j - 3 is through (v_empty of block j - 1 was awaited)
-        const float2 k2 = __half22float2(*reinterpret_cast<const __half2*>(&kp));
-        float2 v2 = __half22float2(*reinterpret_cast<const __half2*>(&vp));
-        // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
-        if (v2.x < 9.31322575e-10f) v2.x = 9.31322575e-10f;
-        const float rv = __fdividef(1.0f, v2.x), ks = k2.x * sm_scale;
-        float* q = &sh.par[ring][tid >> 1][tid & 1];
-        q[0] = ks;
-        q[2] = -fmaf(16.0f, ks, k2.y * sm_scale);
-        // x - x: 0, or NaN where key parameters are not finite (the score of such a token may not end up at -infinity)
-        q[4] = __log2f(v2.x) + ((k2.x - k2.x) + (k2.y - k2.y));
-        q[6] = rv;
-        q[8] = fmaf(v2.y, rv, -8.0f);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(par_full + 8 * ring);
-      }
-      if (j + 1 < n) {
-        const long long row = put_rows(j + 1, id);        // everybody has read the rows of block j - 1
-        load_par(row);
-        if (j + 2 < n) id = page_id(j + 2);
-      }
-      if (j >= 2) {
-        ok = mbar_wait(k_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 74);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; }
-      }
-      {
-        const uint32_t dst = s_k + stage * kAtTile + (kc >> 1) * (kAtTile / 2);
+    if (!what) {
+      // row (lane & 7) + 8 (warp + 4 it), 16-byte chunk lane / 8
+      const float sm_scale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
+      const int kr = (lane & 7) + 8 * pw, kc = lane >> 3;
+      uint4 kw[4];
+      uint32_t kp = 0, vp = 0;
+      auto load = [&](int j, long long mine) {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          const int r = kr + 32 * it;
-          const uint32_t ww[4] = {kw[it].x, kw[it].y, kw[it].z, kw[it].w};
+          const long long row = sh.row[0][j & 1][kr + 32 * it];
+          kw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.data + row * 64 + 16 * kc)) : make_uint4(0, 0, 0, 0);
+        }
+        kp = 0; vp = 0;
+        if (mine >= 0) {
+          kp = __ldg(reinterpret_cast<const uint32_t*>(p.param + mine));
+          vp = __ldg(reinterpret_cast<const uint32_t*>(p.param + mine + v_rows));
+        }
+      };
+      if (n > 0) {
+        load(0, put_rows(0, page_id(0)));
+        if (n > 1) id = page_id(1);
+      }
+      for (int j = 0; j < n; ++j) {
+        const int stage = j & 1, ring = j % kAtParStages;
+        long long mine = -1;
+        if (j + 1 < n) {
+          mine = put_rows(j + 1, id);                     // everybody has read the rows of block j - 1
+          if (j + 2 < n) id = page_id(j + 2);
+        }
+        if (j >= 2) {
+          mbar_wait(k_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 74);
+          __syncwarp();
+        }
+        {
+          // parameters of token tid; the slot of the ring is free: the scores of block j - 2 were issued after the weights of
+          // block j - 3 had been made
+          const float2 k2 = __half22float2(*reinterpret_cast<const __half2*>(&kp));
+          float2 v2 = __half22float2(*reinterpret_cast<const __half2*>(&vp));
+          // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
+          if (v2.x < 9.31322575e-10f) v2.x = 9.31322575e-10f;
+          const float rv = __fdividef(1.0f, v2.x), ks = k2.x * sm_scale;
+          // x - x: 0, or NaN where it is not finite.  Then the weight of the token is NaN in the rows that see it, and its
+          // other numbers are 0, so that a weight 0 leaves the sums of the rows that do not see it alone.
+          const float bad = ((k2.x - k2.x) + (k2.y - k2.y)) + ((v2.x - v2.x) + (v2.y - v2.y));
+          const bool fine = bad == 0.0f;
+          float* q = &sh.par[ring][tid >> 1][tid & 1];
+          q[0] = ks;
+          q[2] = -fmaf(16.0f, ks, k2.y * sm_scale);
+          q[4] = __log2f(v2.x) + bad;
+          q[8] = fine ? rv : 0.0f;
+          q[10] = fine ? fmaf(v2.y, rv, -7.5f) : 0.0f;
+        }
+        const uint32_t dst = s_k + stage * kAtTile + (kc >> 1) * (kAtTile / 2);
+#pragma unroll 1
+        for (int r = kr; r < kAtTok; r += 32) {           // the words of the next round move up: see the note on code size
+          const uint32_t ww[4] = {kw[0].x, kw[0].y, kw[0].z, kw[0].w};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int ch = 4 * (kc & 1) + x;
             st_shared16(dst + r * 128 + ((ch ^ (r & 7)) << 4), code_pair<0>(ww[x]), code_pair<1>(ww[x]), code_pair<2>(ww[x]),
                         code_pair<3>(ww[x]));
           }
+          kw[0] = kw[1]; kw[1] = kw[2]; kw[2] = kw[3];
+        }
+        if (j + 1 < n) load(j + 1, mine);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(par_full + 8 * ring);
+          mbar_arrive(k_full + 8 * stage);
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_full + 8 * stage);
-      if (j + 1 < n) load_k(j + 1);
-      if (j >= 2) {
-        ok = mbar_wait(v_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 75);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; }
+    } else {
+      // tokens 64 (warp & 1) + 8 (lane & 7) + 0 .. 7, 8 bytes (16 dimensions) at 32 (warp / 2) + 8 (lane / 8)
+      const int vt = 64 * (pw & 1) + 8 * (lane & 7), vb = 32 * (pw >> 1) + 8 * (lane >> 3);
+      uint2 vw[8];
+      auto load = [&](int j) {
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const long long row = sh.row[1][j & 1][vt + it];
+          vw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint2*>(p.data + row * 64 + vb)) : make_uint2(0, 0);
+        }
+      };
+      if (n > 0) {
+        put_rows(0, page_id(0));
+        load(0);
+        if (n > 1) id = page_id(1);
       }
-      {
+      for (int j = 0; j < n; ++j) {
+        const int stage = j & 1;
+        if (j + 1 < n) {
+          put_rows(j + 1, id);
+          if (j + 2 < n) id = page_id(j + 2);
+        }
+        if (j >= 2) {
+          mbar_wait(v_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 75);
+          __syncwarp();
+        }
         const uint32_t dst = s_v + stage * kAtTile + (pw & 1) * (kAtTile / 2);
+        const int tg = lane & 7;
+#pragma unroll 1
+        for (int d0 = 2 * vb; d0 < 2 * vb + 16; d0 += 8) {  // eight dimensions: one word of each token
 #pragma unroll
-        for (int half = 0; half < 4; ++half) {            // four dimensions of the lane's sixteen
-          const uint32_t sel = (half & 1) ? 0x7632u : 0x5410u;
-          uint32_t x[4];
+          for (int half = 0; half < 2; ++half) {
+            uint32_t x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[i] = __byte_perm(half < 2 ? vw[2 * i].x : vw[2 * i].y, half < 2 ? vw[2 * i + 1].x : vw[2 * i + 1].y, sel);
-          const int d0 = 2 * vb + 4 * half;
-          const int tg = lane & 7;
-          st_shared16(dst + d0 * 128 + ((tg ^ (d0 & 7)) << 4), at_centred_pair<0>(x[0]), at_centred_pair<0>(x[1]),
-                      at_centred_pair<0>(x[2]), at_centred_pair<0>(x[3]));
-          st_shared16(dst + (d0 + 1) * 128 + ((tg ^ ((d0 + 1) & 7)) << 4), at_centred_pair<1>(x[0]), at_centred_pair<1>(x[1]),
-                      at_centred_pair<1>(x[2]), at_centred_pair<1>(x[3]));
-          st_shared16(dst + (d0 + 2) * 128 + ((tg ^ ((d0 + 2) & 7)) << 4), at_centred_pair<2>(x[0]), at_centred_pair<2>(x[1]),
-                      at_centred_pair<2>(x[2]), at_centred_pair<2>(x[3]));
-          st_shared16(dst + (d0 + 3) * 128 + ((tg ^ ((d0 + 3) & 7)) << 4), at_centred_pair<3>(x[0]), at_centred_pair<3>(x[1]),
-                      at_centred_pair<3>(x[2]), at_centred_pair<3>(x[3]));
+            for (int i = 0; i < 4; ++i) x[i] = __byte_perm(vw[2 * i].x, vw[2 * i + 1].x, half ? 0x7632u : 0x5410u);
+            const uint32_t at = dst + (d0 + 4 * half) * 128;                // d0 is a multiple of 8
+            st_shared16(at + ((tg ^ (4 * half)) << 4), at_centred_pair<0>(x[0]), at_centred_pair<0>(x[1]), at_centred_pair<0>(x[2]),
+                        at_centred_pair<0>(x[3]));
+            st_shared16(at + 128 + ((tg ^ (4 * half + 1)) << 4), at_centred_pair<1>(x[0]), at_centred_pair<1>(x[1]),
+                        at_centred_pair<1>(x[2]), at_centred_pair<1>(x[3]));
+            st_shared16(at + 256 + ((tg ^ (4 * half + 2)) << 4), at_centred_pair<2>(x[0]), at_centred_pair<2>(x[1]),
+                        at_centred_pair<2>(x[2]), at_centred_pair<2>(x[3]));
+            st_shared16(at + 384 + ((tg ^ (4 * half + 3)) << 4), at_centred_pair<3>(x[0]), at_centred_pair<3>(x[1]),
+                        at_centred_pair<3>(x[2]), at_centred_pair<3>(x[3]));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) vw[i].x = vw[i].y;
         }
+        if (j + 1 < n) load(j + 1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full + 8 * stage);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_full + 8 * stage);
-      if (j + 1 < n) load_v(j + 1);
     }
     if (p.splits > 1) { kv_cluster_barrier(); kv_cluster_barrier(); }
   } else {
     // ---------------------------------------------------------------- MMA issue
-    regs_dec<40>();
-    if (warp == 12) {
-      if (lane == 0 && n > 0) {
-        bool ok = mbar_wait(k_full, 0, abort_flag, p.status, 76);
-        auto scores = [&](int i, int stage) {
-          const uint32_t a = desc_lo(s_q + i * kAtTile), b = desc_lo(s_k + stage * kAtTile);
+    regs_dec<32>();
+    const int i = warp - 16;                              // a warp per row tile: they do not wait for each other
+    if (i < tiles && n > 0) {
+      const uint32_t lead = elect_lane();
+      const uint32_t t_s = kTmem + i * 128, t_o = kTmem + 256 + i * 128;
+      const uint32_t q = desc_lo(s_q) + i * (kAtTile >> 4);
+      bool ok = mbar_wait(k_full, 0, abort_flag, p.status, 76);
+      // scores of a half of the block in K stage `stage`
+      auto scores = [&](int buf, int stage) {
+        const uint32_t b = desc_lo(s_k) + stage * (kAtTile >> 4) + buf * (64 * 128 >> 4), d = t_s + buf * 64;
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint32_t off = ((ks >> 2) * (kAtTile / 2) + (ks & 3) * 32) >> 4;
-            umma_f16_ss(tmem + i * 128, a + off, b + off, ks > 0);
-          }
-          umma_commit(s_full + 8 * i);
-        };
-        if (ok) {
-          tc_fence_after();
-          for (int i = 0; i < tiles; ++i) scores(i, 0);
-          umma_commit(k_empty);
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint32_t off = ((ks >> 2) * (kAtTile / 2) + (ks & 3) * 32) >> 4;
+          umma_f16_ss(lead, d, q + off, b + off, ks > 0);
         }
-        for (int j = 0; ok && j < n; ++j) {
-          const int stage = j & 1;
-          ok = mbar_wait(v_full + 8 * stage, (j >> 1) & 1, abort_flag, p.status, 77);
-          if (ok && j + 1 < n) ok = mbar_wait(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, abort_flag, p.status, 78);
-          for (int i = 0; ok && i < tiles; ++i) {
-            ok = mbar_wait(p_full + 8 * i, j & 1, abort_flag, p.status, 79);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t b = desc_lo(s_v + stage * kAtTile);
+        umma_commit_lead(lead, s_full + 16 * i + 8 * buf);
+      };
+      if (ok) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int buf = 0; buf < 2; ++buf) scores(buf, 0);
+        umma_commit_lead(lead, k_empty);
+      }
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j) {
+        const int stage = j & 1;
+        const bool more = j + 1 < n;
+        ok = mbar_wait(v_full + 8 * stage, (j >> 1) & 1, abort_flag, p.status, 77);
+        if (ok && more) ok = mbar_wait(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, abort_flag, p.status, 78);
+#pragma unroll 1
+        for (int buf = 0; ok && buf < 2; ++buf) {
+          ok = mbar_wait(p_full + 16 * i + 8 * buf, j & 1, abort_flag, p.status, 79);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = desc_lo(s_v) + stage * (kAtTile >> 4) + buf * (kAtTile / 2 >> 4);
+          const uint32_t first = buf | j;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-              const uint32_t off = ((ks >> 2) * (kAtTile / 2) + (ks & 3) * 32) >> 4;
-              umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + ks * 8, b + off, j > 0 || ks > 0);
-            }
-            if (j + 1 < n) scores(i, stage ^ 1);
-            else umma_commit(o_full + 8 * i);
-          }
-          if (ok) {
-            if (j + 1 < n) umma_commit(k_empty + 8 * (stage ^ 1));
-            umma_commit(v_empty + 8 * stage);
-          }
+          for (int ks = 0; ks < 4; ++ks) umma_f16_ts(lead, t_o, t_s + buf * 64 + ks * 8, b + ks * 2, ks > 0 ? 1u : first);
+          // scores of half h imply the products of half h - 2: the softmax is at most one phase of pv_done behind
+          umma_commit_lead(lead, (more || !buf ? pv_done : o_full) + 8 * i);
+          if (more) scores(buf, stage ^ 1);                 // over the weights, which the products before it have read
+        }
+        if (ok) {
+          if (more) umma_commit_lead(lead, k_empty + 8 * (stage ^ 1));
+          umma_commit_lead(lead, v_empty + 8 * stage);
         }
       }
       __syncwarp();
@@ -638,9 +835,9 @@ kv_attend_tc_kernel(const KvAttendParams p) {
   drain_after_abort(abort_flag);
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(kTmem, 512);
   }
 }
 
