@@ -10,7 +10,7 @@
 // The call writes a few megabytes at most, so it is one launch without a second pass: every CTA makes the three prefix
 // sums of the whole batch itself (512 threads x 4 sequences per round, the sums of up to 8192 sequences in shared
 // memory) and then takes its share of the flat list of outputs; an entry finds its sequence by a binary search in
-// shared memory, four entries of kv_indices per search.  A new page is read from the free list by everyone, never from
+// shared memory, 128 to 512 entries of kv_indices per search.  A new page is read from the free list by everyone, never from
 // the block table, whose new entries are written in the same launch: no CTA waits for another.
 #include "kv_common.cuh"
 
@@ -71,6 +71,8 @@ __device__ __forceinline__ int pt_find(const int* s, int n, int i) {
   return lo;
 }
 
+// R: rounds of 128 entries of kv_indices that a warp takes at a time (4 where there is enough for every warp, 1 otherwise)
+template <int R>
 __global__ void __launch_bounds__(kPtThreads)
 kv_page_table_kernel(const PageTableParams p) {
   extern __shared__ int s_pt[];
@@ -178,30 +180,52 @@ kv_page_table_kernel(const PageTableParams p) {
     *fresh = true;
     return p.free_pages[(size_t)s_free[b] + (j - s_held[b])];
   };
+  // kv_indices: a warp takes 128 R entries, looks their first sequence up once and walks on from there
   const int stride = gridDim.x * kPtThreads, at = blockIdx.x * kPtThreads + tid;
+  const int lane = tid & 31;
   const long long cap = (long long)p.batch * W;
   const int pages = (int)base_pages;
   const bool vec = (reinterpret_cast<uintptr_t>(p.kv_indices) & 15) == 0;
-  for (long long i0 = 4ll * at; i0 < cap; i0 += 4ll * stride) {
-    int v[4] = {-1, -1, -1, -1};
-    if (i0 < pages) {
-      int b = pt_find(s_pages, p.batch, (int)i0);
+  for (long long seg = at >> 5; seg * (128 * R) < cap; seg += stride >> 5) {
+    const long long i_seg = seg * (128 * R);
+    const int b_seg = i_seg < pages ? pt_find(s_pages, p.batch, (int)i_seg) : 0;
+    int v[R][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = (int)i0 + k;
-        if (i < pages) {
-          while (s_pages[b + 1] <= i) ++b;
-          bool fresh;
-          const int j = i - s_pages[b];
-          v[k] = page_of(b, j, &fresh);
-          if (fresh) p.block_table[(size_t)b * W + j] = v[k];
+    for (int r = 0; r < R; ++r) {
+      const long long i0 = i_seg + 128 * r + 4 * lane;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[r][k] = -1;
+      if (i0 < pages) {
+        int b = b_seg;
+        while (s_pages[b + 1] <= (int)i0) ++b;
+        int j = (int)i0 - s_pages[b];
+        if (!p.block_table || j + 4 > s_held[b] || i0 + 4 > pages) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int i = (int)i0 + k;
+            if (i < pages) {
+              while (s_pages[b + 1] <= i) ++b;
+              bool fresh;
+              j = i - s_pages[b];
+              v[r][k] = page_of(b, j, &fresh);
+              if (fresh) p.block_table[(size_t)b * W + j] = v[r][k];
+            }
+          }
+        } else {
+          const int32_t* src = p.block_table + (size_t)b * W + j;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[r][k] = src[k];
         }
       }
     }
-    if (vec && i0 + 4 <= cap) {
-      *reinterpret_cast<int4*>(p.kv_indices + i0) = make_int4(v[0], v[1], v[2], v[3]);
-    } else {
-      for (int k = 0; k < 4 && i0 + k < cap; ++k) p.kv_indices[i0 + k] = v[k];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long i0 = i_seg + 128 * r + 4 * lane;
+      if (vec && i0 + 4 <= cap) {
+        *reinterpret_cast<int4*>(p.kv_indices + i0) = make_int4(v[r][0], v[r][1], v[r][2], v[r][3]);
+      } else {
+        for (int k = 0; k < 4 && i0 + k < cap; ++k) p.kv_indices[i0 + k] = v[r][k];
+      }
     }
   }
   const int rows = s_rows[p.batch];
@@ -248,10 +272,12 @@ extern "C" int qr_kv_page_table(const int32_t* seq_lens, const int32_t* new_lens
   p.slot_map = slot_map; p.positions = positions; p.seq_lens_out = seq_lens_out; p.status = status;
   const size_t smem = (size_t)(4 * batch + 2) * sizeof(int);
   // one CTA per 2048 page entries or 512 tokens, at most one per SM: each of them makes the prefix sums for itself
-  const int64_t want = ((int64_t)batch * max_blocks + 4 * kPtThreads - 1) / (4 * kPtThreads) + (new_tokens + kPtThreads - 1) / kPtThreads;
+  const int64_t cap = (int64_t)batch * max_blocks;
+  const int64_t want = (cap + 4 * kPtThreads - 1) / (4 * kPtThreads) + (new_tokens + kPtThreads - 1) / kPtThreads;
   const int grid = (int)(want < num_sms() ? (want > 0 ? want : 1) : num_sms());
-  if (smem > 48 * 1024) QR_CUDA(cudaFuncSetAttribute(kv_page_table_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kv_page_table_kernel<<<grid, kPtThreads, smem, (cudaStream_t)stream>>>(p);
+  auto kern = cap > 512ll * (kPtThreads / 32) * num_sms() ? kv_page_table_kernel<4> : kv_page_table_kernel<1>;
+  if (smem > 48 * 1024) QR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kern<<<grid, kPtThreads, smem, (cudaStream_t)stream>>>(p);
   QR_LAUNCH_CHECK("kv_page_table_kernel");
   return QR_OK;
 }

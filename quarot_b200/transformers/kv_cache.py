@@ -72,38 +72,56 @@ def append_kv_i4(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, k, 
             1 if hadamard_k else 0, _stream(dev)), "append_kv_i4")
 
 
-def _check_i32(op, dev, **tensors):
-    for name, (t, n) in tensors.items():
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-            raise RuntimeError("%s: %s must be a contiguous int32 tensor on %s" % (op, name, dev))
-        if n is not None and t.numel() < n:
-            raise RuntimeError("%s: %s has %d entries, %d are needed" % (op, name, t.numel(), n))
+def _launch(op, dev, fn, *args):
+    """fn(*args, stream) on the current stream of dev.  The calls below are short next to what a device context and a
+    stream object cost to make, so the context is entered only where dev is not the current device."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, op)
+
+
+def _check_i32(op, dev, name, t, n):
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
+        raise RuntimeError("%s: %s must be a contiguous int32 tensor on %s" % (op, name, dev))
+    if t.numel() < n:
+        raise RuntimeError("%s: %s has %d entries, %d are needed" % (op, name, t.numel(), n))
+    return t.data_ptr()
 
 
 def _check_pages(op, kv_data, kv_param, layer_idx):
-    """Checks of the page pool [pages, layers, 2, heads, page_size, 64] and its parameters; (layers, heads, page_size)."""
-    dev = _ops._check_cuda_contig(op, kv_data=kv_data, kv_param=kv_param)
-    if kv_data.dtype != torch.uint8 or kv_param.dtype != torch.float16:
+    """Checks of the page pool [pages, layers, 2, heads, page_size, 64] and its parameters; its device and sizes."""
+    dev = kv_data.device
+    if dev.type != "cuda" or kv_param.device != dev or not kv_data.is_contiguous() or not kv_param.is_contiguous():
+        raise RuntimeError("%s: the pages and their parameters must be contiguous tensors on one CUDA device" % op)
+    if kv_data.dtype is not torch.uint8 or kv_param.dtype is not torch.float16:
         raise RuntimeError("%s: the pages are uint8 and their parameters fp16" % op)
-    if kv_data.dim() != 6 or kv_data.shape[2] != 2 or tuple(kv_param.shape) != tuple(kv_data.shape[:5]) + (2,):
-        raise RuntimeError("%s: pages %s and parameters %s do not belong together" % (op, tuple(kv_data.shape), tuple(kv_param.shape)))
-    if kv_data.shape[5] != 64:
+    shape = tuple(kv_data.shape)
+    if len(shape) != 6 or shape[2] != 2 or tuple(kv_param.shape) != shape[:5] + (2,):
+        raise RuntimeError("%s: pages %s and parameters %s do not belong together" % (op, shape, tuple(kv_param.shape)))
+    if shape[5] != 64:
         raise RuntimeError("%s: head_dim must be 128" % op)
-    if not 0 <= int(layer_idx) < kv_data.shape[1]:
-        raise RuntimeError("%s: layer %d of %d" % (op, layer_idx, kv_data.shape[1]))
-    return dev, kv_data.shape[1], kv_data.shape[3], kv_data.shape[4]
+    if not 0 <= layer_idx < shape[1]:
+        raise RuntimeError("%s: layer %d of %d" % (op, layer_idx, shape[1]))
+    return dev, shape
 
 
 def _check_rows(op, dev, name, t):
-    """[tokens, heads, 128] fp16 on dev, last axis contiguous; the strides of the other two."""
-    if t.device != dev or t.dtype != torch.float16 or t.dim() != 3 or t.shape[2] != 128:
+    """[tokens, heads, 128] fp16 on dev, last axis contiguous; address, strides of the other two."""
+    shape = t.shape
+    if t.dtype is not torch.float16 or t.device != dev or len(shape) != 3 or shape[2] != 128:
         raise RuntimeError("%s: %s must be fp16 [tokens, heads, 128] on %s" % (op, name, dev))
-    ts, hs = t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
-    if t.numel() and (t.stride(2) != 1 or ts % 4 or hs % 4 or t.data_ptr() % 8):
+    ts, hs, ds = t.stride()
+    ts, hs = ts if shape[0] > 1 else 0, hs if shape[1] > 1 else 0
+    at = t.data_ptr()
+    if (ds != 1 or ts % 4 or hs % 4 or at % 8) and t.numel():
         raise RuntimeError("%s: %s needs a contiguous last axis, 8-byte alignment and strides that are multiples of 4" % (op, name))
-    return ts, hs
+    return at, ts, hs
 
 
 def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, free_pages=None, max_blocks=None):
@@ -132,77 +150,76 @@ def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None
     elif free_pages is not None or max_blocks is None:
         raise RuntimeError("%s: without a block_table there is no free list, and max_blocks is needed" % op)
     max_blocks = int(max_blocks)
-    _check_i32(op, dev, seq_lens=(seq_lens, batch), new_lens=(new_lens, batch), block_table=(block_table, None),
-               free_pages=(free_pages, None))
     if new_tokens < 0 or page_size < 1 or max_blocks < 1:
         raise RuntimeError("%s: bad number of new tokens, page size or blocks per sequence" % op)
-    with torch.cuda.device(dev):
-        # one allocation for the 32-bit outputs, each on a 16-byte boundary
-        sizes = (batch + 1, batch * max_blocks, batch, batch + 1, new_tokens, batch, 2)
-        names = ("kv_indptr", "kv_indices", "last_page_offset", "append_indptr", "positions", "seq_lens", "status")
-        starts = [0]
-        for n in sizes:
-            starts.append(starts[-1] + (n + 3) // 4 * 4)
-        buf = torch.empty(starts[-1], dtype=torch.int32, device=dev)
-        out = {name: buf[a:a + n] for name, a, n in zip(names, starts, sizes)}
-        out["slot_map"] = torch.empty(new_tokens, dtype=torch.int64, device=dev)
-        if batch == 0:
-            buf.zero_()
-            out["positions"].fill_(-1)
-            out["slot_map"].fill_(-1)
-            return out
-        _lib.check(_lib_c.qr_kv_page_table(
-            seq_lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, batch, new_tokens, page_size, max_blocks,
-            block_table.data_ptr() if block_table is not None else None,
-            free_pages.data_ptr() if free_pages is not None and free_pages.numel() else None,
-            free_pages.numel() if free_pages is not None else -1,
-            out["kv_indptr"].data_ptr(), out["kv_indices"].data_ptr(), out["last_page_offset"].data_ptr(),
-            out["append_indptr"].data_ptr(), out["slot_map"].data_ptr(), out["positions"].data_ptr(), out["seq_lens"].data_ptr(),
-            out["status"].data_ptr(), _stream(dev)), op)
-    return out
+    seq_p, new_p = _check_i32(op, dev, "seq_lens", seq_lens, batch), _check_i32(op, dev, "new_lens", new_lens, batch)
+    table_p, free_p = _check_i32(op, dev, "block_table", block_table, 0), _check_i32(op, dev, "free_pages", free_pages, 0)
+    # one allocation for all outputs; the slot map (64-bit) and kv_indices come first, on 16-byte boundaries
+    cap, gap = batch * max_blocks, 2 if new_tokens & 1 else 0
+    sizes = [2 * new_tokens, cap, batch + 1, batch, batch + 1, new_tokens, batch, 2]
+    if gap:
+        sizes.insert(1, gap)
+    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+    if batch:
+        at = buf.data_ptr()
+        indices = at + 8 * new_tokens + 4 * gap
+        indptr = indices + 4 * cap
+        last = indptr + 4 * (batch + 1)
+        append = last + 4 * batch
+        positions = append + 4 * (batch + 1)
+        after = positions + 4 * new_tokens
+        _launch(op, dev, _lib_c.qr_kv_page_table, seq_p, new_p, batch, new_tokens, page_size, max_blocks, table_p, free_p or None,
+                -1 if free_pages is None else free_pages.numel(), indptr, indices, last, append, at, positions, after,
+                after + 4 * batch)
+    else:
+        buf.zero_()[:2 * new_tokens].fill_(-1)
+    parts = buf.split_with_sizes(sizes)
+    slots, (indices, indptr, last, append, positions, after, status) = parts[0], parts[-7:]
+    if not batch:
+        positions.fill_(-1)
+    return {"kv_indptr": indptr, "kv_indices": indices, "last_page_offset": last, "append_indptr": append,
+            "slot_map": slots.view(torch.int64), "positions": positions, "seq_lens": after, "status": status}
 
 
 def append_kv_slots_i4(kv_data, kv_param, slot_map, k, v, layer_idx, hadamard_k=True):
     """append_kv_i4 with the page slots from a slot map (build_page_table): slot_map int64 [tokens], k and v fp16 [tokens,
     heads, 128] (strided views are fine).  Tokens whose slot lies outside the pool, -1 among others, are left out."""
     op = "append_kv_slots_i4"
-    dev, layers, heads, page_size = _check_pages(op, kv_data, kv_param, layer_idx)
-    kt, kh = _check_rows(op, dev, "k", k)
-    vt, vh = _check_rows(op, dev, "v", v)
+    layer_idx = int(layer_idx)
+    dev, (pages, layers, _, heads, page_size, _) = _check_pages(op, kv_data, kv_param, layer_idx)
+    k_p, kt, kh = _check_rows(op, dev, "k", k)
+    v_p, vt, vh = _check_rows(op, dev, "v", v)
+    tokens = k.shape[0]
     if k.shape != v.shape or k.shape[1] != heads:
         raise RuntimeError("%s: k %s and v %s over %d heads" % (op, tuple(k.shape), tuple(v.shape), heads))
-    if slot_map.dtype != torch.int64 or slot_map.device != dev or not slot_map.is_contiguous() or slot_map.numel() != k.shape[0]:
+    if slot_map.dtype is not torch.int64 or slot_map.device != dev or not slot_map.is_contiguous() or slot_map.numel() != tokens:
         raise RuntimeError("%s: slot_map must be contiguous int64 on %s with one entry per token" % (op, dev))
-    with torch.cuda.device(dev):
-        _lib.check(_lib_c.qr_kv_append_slots_i4(
-            kv_data.data_ptr(), kv_param.data_ptr(), kv_data.shape[0], slot_map.data_ptr(), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-            k.shape[0], layers, int(layer_idx), heads, page_size, 128, 1 if hadamard_k else 0, _stream(dev)), op)
+    _launch(op, dev, _lib_c.qr_kv_append_slots_i4, kv_data.data_ptr(), kv_param.data_ptr(), pages, slot_map.data_ptr(), k_p, kt, kh,
+            v_p, vt, vh, tokens, layers, layer_idx, heads, page_size, 128, 1 if hadamard_k else 0)
 
 
 def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr, max_q_len, layer_idx, hadamard_q,
                window, sink_tokens):
-    dev, layers, kv_heads, page_size = _check_pages(op, kv_data, kv_param, layer_idx)
-    qt, qh = _check_rows(op, dev, "q", q)
-    ot, oh = _check_rows(op, dev, "o", o)
+    layer_idx = int(layer_idx)
+    dev, (pages, layers, _, kv_heads, page_size, _) = _check_pages(op, kv_data, kv_param, layer_idx)
+    q_p, qt, qh = _check_rows(op, dev, "q", q)
+    o_p, ot, oh = _check_rows(op, dev, "o", o)
     if o.shape != q.shape:
         raise RuntimeError("%s: o %s, q %s" % (op, tuple(o.shape), tuple(q.shape)))
-    tokens, heads = q.shape[:2]
+    tokens, heads, _ = q.shape
     if not ((heads < 2 or oh >= 128) and (tokens < 2 or ot >= 128) and
             (heads < 2 or tokens < 2 or ot >= oh * heads or oh >= ot * tokens)):
         raise RuntimeError("%s: the rows of o overlap" % op)
     if heads == 0 or heads % kv_heads:
         raise RuntimeError("%s: %d query heads over %d KV heads" % (op, heads, kv_heads))
-    batch = last_page_offset.shape[0]
-    _check_i32(op, dev, kv_indptr=(kv_indptr, batch + 1), kv_indices=(kv_indices, None), last_page_offset=(last_page_offset, batch),
-               qo_indptr=(qo_indptr, batch + 1))
     if window is not None and window < 1 or sink_tokens < 0:
         raise RuntimeError("%s: window must be positive (None: no window), sink_tokens not negative" % op)
-    with torch.cuda.device(dev):
-        _lib.check(_lib_c.qr_kv_attend_i4(
-            o.data_ptr(), ot, oh, q.data_ptr(), qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), kv_data.shape[0], kv_indptr.data_ptr(),
-            kv_indices.data_ptr(), last_page_offset.data_ptr(), qo_indptr.data_ptr() if qo_indptr is not None else None, tokens,
-            max_q_len, batch, layers, int(layer_idx), heads, kv_heads, page_size, 128, min(int(window), 0x7fffffff) if window else 0,
-            min(int(sink_tokens), 0x7fffffff), 1 if hadamard_q else 0, _stream(dev)), op)
+    batch = last_page_offset.shape[0]
+    _launch(op, dev, _lib_c.qr_kv_attend_i4, o_p, ot, oh, q_p, qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), pages,
+            _check_i32(op, dev, "kv_indptr", kv_indptr, batch + 1), _check_i32(op, dev, "kv_indices", kv_indices, 0),
+            _check_i32(op, dev, "last_page_offset", last_page_offset, batch), _check_i32(op, dev, "qo_indptr", qo_indptr, batch + 1),
+            tokens, max_q_len, batch, layers, layer_idx, heads, kv_heads, page_size, 128,
+            min(int(window), 0x7fffffff) if window else 0, min(int(sink_tokens), 0x7fffffff), 1 if hadamard_q else 0)
 
 
 def chunk_attention_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr, layer_idx, max_q_len=None,
