@@ -5,10 +5,10 @@
 //   s_t <q_r, c_t> - z_t sum(q_r),   and value = s' c' - z'  (s', z' the value parameters).
 // The tensor cores see only small whole numbers: a code is put into the mantissa of 16.0 (fp16 0x4C00 | c << 6 is exactly
 // 16 + c), two logical instructions per pair of codes and no arithmetic, and the 16 is taken out of the sums in fp32.
-// Weights: w_t = exp2(score_t + log2 s'_t - M) with M following the running maximum of that exponent in steps of at least
-// 8 (so that sums are rarely multiplied through), times 2^6: the value scale is inside the weight, the largest weight lies
-// between 2^6 and 2^14 and rounding w to fp16 (the B operand of the second product) is a relative error of at most 2^-11
-// down to weights 2^-20 of the largest; the sums
+// Weights: w_t = exp2(score_t + log2 s'_t - M) so that the value scale is inside the weight.  M does not follow the
+// maximum: it is set 1 below the first one and moves, in whole steps, only where a weight would pass 2^15, so that sums
+// are rarely multiplied through and no maximum is looked for across lanes.  Rounding w to fp16 (the B operand of the second
+// product) is a relative error of at most 2^-11 down to 2^-14 of the largest; the sums
 //   l = sum w / s'_t  (the softmax denominator)  and  y = sum w (z'_t / s'_t - 7.5)
 // are of the unrounded w in fp32, and the centre 7.5 of the codes is taken out with the ROUNDED weights (one more MMA
 // row of ones), so that a rounding error of w meets c' - 7.5 and not 16 + c':
@@ -31,11 +31,18 @@
 namespace qr {
 
 constexpr int kRwWarps = 8;
-constexpr int kRwStages = 4;
 constexpr int kRwTok = 32;                              // tokens per block
 constexpr int kRwStageBytes = kRwTok * (64 + 64 + 4 + 4);
-constexpr int kRwRing = kRwWarps * kRwStages * kRwStageBytes;
 constexpr int kRwORow = kHeadDim + 4;                   // floats per row of the merge buffers
+constexpr float kRwTop = 15.0f;                         // weights are at most 2^15
+
+// Eight rows: two CTAs per SM with three stages per warp; more rows: one CTA (registers) with four.
+template <int NT>
+struct RwConfig {
+  static constexpr int kStages = NT == 1 ? 3 : 4;
+  static constexpr int kCtas = NT == 1 ? 2 : 1;
+  static constexpr int kRing = kRwWarps * kStages * kRwStageBytes;
+};
 
 template <int NT>
 struct RwShared {
@@ -85,12 +92,14 @@ __device__ __forceinline__ void rw_store_row(const KvAttendParams& p, const KvTi
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * kRwWarps, 1)
+__global__ void __launch_bounds__(32 * kRwWarps, RwConfig<NT>::kCtas)
 kv_attend_rows_kernel(const KvAttendParams p) {
   constexpr int R = 8 * NT;
+  constexpr int kStages = RwConfig<NT>::kStages;
+  constexpr int TA = NT == 1 ? 2 : 1;                   // 16-token tiles worked on together: two hide the MMA chains of one row group
   extern __shared__ __align__(128) unsigned char s_dyn[];
   unsigned char* ring = s_dyn;
-  RwShared<NT>& sh = *reinterpret_cast<RwShared<NT>*>(s_dyn + kRwRing);
+  RwShared<NT>& sh = *reinterpret_cast<RwShared<NT>*>(s_dyn + RwConfig<NT>::kRing);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int unit = blockIdx.x / p.splits;
   uint32_t crank = 0;
@@ -98,6 +107,54 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   const int head_kv = unit % p.kv_heads;
   const KvTile w = kv_find_tile(p, unit / p.kv_heads, R, lane);
   if (w.rows == 0) return;                              // the whole cluster has the same tile
+
+  const int last_row = w.row0 + w.rows - 1;
+  const int p_min = w.pos0 + fast_div(w.row0, p.group_div), p_max = w.pos0 + fast_div(last_row, p.group_div);
+  const KvBlocks blk = kv_blocks<kRwTok>(p_min, p_max, p.window, p.sinks);
+  // the CTAs of a cluster take contiguous ranges of blocks, the warps of a CTA every eighth one
+  const int per = (blk.count + p.splits - 1) / p.splits;
+  const int begin = (int)crank * per + warp, end = min((int)(crank + 1) * per, blk.count);
+
+  const int32_t* pages = p.indices + p.indptr[w.b];
+  const int tokens = min(p_max + 1, w.seq_len);         // tokens from here on are not read
+  // a pool has fewer than 2^32 rows of 64 bytes
+  const uint32_t page_rows = (uint32_t)p.layers * 2 * p.kv_heads * p.page_size;
+  const uint32_t row_k = ((uint32_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
+  const uint32_t v_rows = (uint32_t)p.kv_heads * p.page_size;
+  const uint32_t last_page = (uint32_t)(p.num_pages - 1);
+  const uint32_t my_ring = smem_u32(ring) + warp * (kStages * kRwStageBytes);
+
+  // lane copies chunk c of the rows g + 8 i of a block
+  auto page_ids = [&](int bi, int (&id)[4]) {
+    const int t0 = kv_block_index(blk, bi) * kRwTok + g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = t0 + 8 * i < tokens ? __ldg(pages + fast_div(t0 + 8 * i, p.page_div)) : 0;
+  };
+  auto issue = [&](int bi, int stage, const int (&id)[4]) {
+    const int t0 = kv_block_index(blk, bi) * kRwTok + g;
+    const uint32_t st = my_ring + stage * kRwStageBytes + g * 64 + ((c ^ rw_swz(g)) << 4);
+    const uint32_t sp = my_ring + stage * kRwStageBytes + kRwTok * 128 + (c & 1) * (kRwTok * 4) + g * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + 8 * i;
+      const bool ok = t < tokens;
+      const int slot = t - fast_div(t, p.page_div) * p.page_size;
+      // an index outside the pool reads its last page
+      const uint32_t row = min((uint32_t)id[i], last_page) * page_rows + row_k + (ok ? slot : 0);
+      const uint8_t* src = p.data + (uint64_t)row * 64 + 16 * c;
+      rw_cp16(st + 512 * i, src, ok ? 16 : 0);
+      rw_cp16(st + 512 * i + kRwTok * 64, src + (uint64_t)v_rows * 64, ok ? 16 : 0);
+      if (c < 2) rw_cp4(sp + 32 * i, p.param + (row + (c ? v_rows : 0u)), ok ? 4 : 0);
+    }
+  };
+  int id[4];
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    const int bi = begin + s * kRwWarps;
+    if (bi < end) { page_ids(bi, id); issue(bi, s, id); }
+    rw_commit();
+  }
+  if (begin + (kStages - 1) * kRwWarps < end) page_ids(begin + (kStages - 1) * kRwWarps, id);
 
   for (int r = warp; r < R; r += kRwWarps) {
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -126,58 +183,23 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   }
   __syncthreads();
 
-  uint32_t qf[NT][16];
+  // query fragments: in registers for eight or sixteen rows, from shared memory where they are used for more
+  uint32_t qf[NT <= 2 ? NT : 1][16];
   float qs[NT][2];
   int ps[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    if (NT <= 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * i]);
-      qf[n][4 * i] = u.x; qf[n][4 * i + 1] = u.y; qf[n][4 * i + 2] = u.z; qf[n][4 * i + 3] = u.w;
+      for (int i = 0; i < 4; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * i]);
+        qf[NT <= 2 ? n : 0][4 * i] = u.x; qf[NT <= 2 ? n : 0][4 * i + 1] = u.y;
+        qf[NT <= 2 ? n : 0][4 * i + 2] = u.z; qf[NT <= 2 ? n : 0][4 * i + 3] = u.w;
+      }
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; ps[n][k] = sh.pos[8 * n + 2 * c + k]; }
   }
-  const int last_row = w.row0 + w.rows - 1;
-  const int p_min = w.pos0 + fast_div(w.row0, p.group_div), p_max = w.pos0 + fast_div(last_row, p.group_div);
-  const KvBlocks blk = kv_blocks<kRwTok>(p_min, p_max, p.window, p.sinks);
-  // the CTAs of a cluster take contiguous ranges of blocks, the warps of a CTA every eighth one
-  const int per = (blk.count + p.splits - 1) / p.splits;
-  const int begin = (int)crank * per + warp, end = min((int)(crank + 1) * per, blk.count);
-
-  const int first_page = p.indptr[w.b];
-  const int tokens = min(p_max + 1, w.seq_len);         // tokens from here on are not read
-  const size_t page_rows = (size_t)p.layers * 2 * p.kv_heads * p.page_size;
-  const size_t row_k = ((size_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
-  const size_t row_v = row_k + (size_t)p.kv_heads * p.page_size;
-  const uint32_t my_ring = smem_u32(ring) + warp * (kRwStages * kRwStageBytes);
-
-  // lane copies chunk c of the rows g + 8 i of a block
-  auto page_ids = [&](int bi, int (&id)[4]) {
-    const int t0 = kv_block_index(blk, bi) * kRwTok;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = t0 + g + 8 * i;
-      id[i] = t < tokens ? __ldg(p.indices + first_page + fast_div(t, p.page_div)) : 0;
-    }
-  };
-  auto issue = [&](int bi, int stage, const int (&id)[4]) {
-    const int t0 = kv_block_index(blk, bi) * kRwTok;
-    const uint32_t st = my_ring + stage * kRwStageBytes;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = g + 8 * i, t = t0 + r;
-      const bool ok = t < tokens;
-      const int slot = ok ? t - fast_div(t, p.page_div) * p.page_size : 0;
-      const size_t page = min((size_t)(uint32_t)id[i], (size_t)p.num_pages - 1);   // an index outside the pool reads its last page
-      const size_t rk = page * page_rows + row_k + slot, rv = page * page_rows + row_v + slot;
-      const uint32_t at = (uint32_t)(r * 64 + ((c ^ rw_swz(r)) << 4));
-      rw_cp16(st + at, p.data + rk * 64 + 16 * c, ok ? 16 : 0);
-      rw_cp16(st + kRwTok * 64 + at, p.data + rv * 64 + 16 * c, ok ? 16 : 0);
-      if (c < 2) rw_cp4(st + kRwTok * 128 + c * kRwTok * 4 + r * 4, p.param + (c ? rv : rk), ok ? 4 : 0);
-    }
-  };
 
   float o[NT][8][4], ws[NT][4], l[NT][2], y[NT][2], m[NT][2];
 #pragma unroll
@@ -192,38 +214,32 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     for (int k = 0; k < 2; ++k) { l[n][k] = 0.0f; y[n][k] = 0.0f; m[n][k] = -INFINITY; }
   }
 
-  int id[4];
-#pragma unroll
-  for (int s = 0; s < kRwStages - 1; ++s) {
-    const int bi = begin + s * kRwWarps;
-    if (bi < end) { page_ids(bi, id); issue(bi, s, id); }
-    rw_commit();
-  }
-  if (begin + (kRwStages - 1) * kRwWarps < end) page_ids(begin + (kRwStages - 1) * kRwWarps, id);
-
   int stage = 0;
   const float sm_scale = 0.08838834764831845f * 1.4426950408889634f;   // log2(e) / sqrt(128)
+  // slots of a 16-token tile -> tokens, see rw_token_even: rows g, g + 8 of a K fragment; 2 c, 2 c + 1 (+ 8) of a V fragment
+  const int tau = (g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1), ta = rw_token_even(c), tb = rw_token_odd(c);
+#pragma unroll 1
   for (int bi = begin; bi < end; bi += kRwWarps) {
     {
-      const int ahead = bi + (kRwStages - 1) * kRwWarps;
-      if (ahead < end) issue(ahead, stage == 0 ? kRwStages - 1 : stage - 1, id);
+      const int ahead = bi + (kStages - 1) * kRwWarps;
+      if (ahead < end) issue(ahead, stage == 0 ? kStages - 1 : stage - 1, id);
       rw_commit();
       if (ahead + kRwWarps < end) page_ids(ahead + kRwWarps, id);
     }
-    rw_wait<kRwStages - 1>();
+    rw_wait<kStages - 1>();
     __syncwarp();
-    const unsigned char* st = ring + warp * (kRwStages * kRwStageBytes) + stage * kRwStageBytes;
+    const unsigned char* st = ring + warp * (kStages * kRwStageBytes) + stage * kRwStageBytes;
     const int t0 = kv_block_index(blk, bi) * kRwTok;
     const bool edge = t0 + kRwTok - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kRwTok - 1 >= p.sinks);
-
-    float s[2][NT][4];
+#pragma unroll 1
+    for (int a0 = 0; a0 < 2; a0 += TA) {
+    float s[TA][NT][4];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      // fragment rows g and g + 8: tokens 16 a + tau and 16 a + 8 + tau
-      const int tau = (g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1);
-      const int r0 = 16 * a + tau, r1 = r0 + 8;
-      const uint4 x = *reinterpret_cast<const uint4*>(st + r0 * 64 + ((c ^ rw_swz(r0)) << 4));
-      const uint4 z = *reinterpret_cast<const uint4*>(st + r1 * 64 + ((c ^ rw_swz(r1)) << 4));
+    for (int a = 0; a < TA; ++a) {
+      // fragment rows g and g + 8: tokens tau and 8 + tau of the tile
+      const unsigned char* sk = st + (16 * (a0 + a) + tau) * 64 + ((c ^ rw_swz(tau)) << 4);
+      const uint4 x = *reinterpret_cast<const uint4*>(sk);
+      const uint4 z = *reinterpret_cast<const uint4*>(sk + 8 * 64);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -231,24 +247,25 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
       for (int wi = 0; wi < 4; ++wi) {
-        const uint32_t a0 = code_pair<0>(xw[wi]), a1 = code_pair<0>(zw[wi]), a2 = code_pair<1>(xw[wi]), a3 = code_pair<1>(zw[wi]);
-        const uint32_t b0 = code_pair<2>(xw[wi]), b1 = code_pair<2>(zw[wi]), b2 = code_pair<3>(xw[wi]), b3 = code_pair<3>(zw[wi]);
+        const uint32_t f0 = code_pair<0>(xw[wi]), f1 = code_pair<0>(zw[wi]), f2 = code_pair<1>(xw[wi]), f3 = code_pair<1>(zw[wi]);
+        const uint32_t h0 = code_pair<2>(xw[wi]), h1 = code_pair<2>(zw[wi]), h2 = code_pair<3>(xw[wi]), h3 = code_pair<3>(zw[wi]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16(s[a][n], a0, a1, a2, a3, qf[n][4 * wi], qf[n][4 * wi + 1]);
-          mma_f16(s[a][n], b0, b1, b2, b3, qf[n][4 * wi + 2], qf[n][4 * wi + 3]);
+          uint4 q4;
+          if (NT <= 2) q4 = make_uint4(qf[NT <= 2 ? n : 0][4 * wi], qf[NT <= 2 ? n : 0][4 * wi + 1], qf[NT <= 2 ? n : 0][4 * wi + 2], qf[NT <= 2 ? n : 0][4 * wi + 3]);
+          else q4 = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * wi]);
+          mma_f16(s[a][n], f0, f1, f2, f3, q4.x, q4.y);
+          mma_f16(s[a][n], h0, h1, h2, h3, q4.z, q4.w);
         }
       }
     }
-    float rv[2][2], zv[2][2];                           // 1 / s', z' / s' - 7.5 of the lane's four tokens
-    float top[NT][2];
+    float rv[TA][2], zv[TA][2];                         // 1 / s', z' / s' - 7.5 of the lane's tokens
+    float top = -INFINITY;                              // largest exponent relative to M
 #pragma unroll
-    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < TA; ++a)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = 16 * a + 8 * h + ((g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1));
+        const int r = 16 * (a0 + a) + 8 * h + tau;
         const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 128 + r * 4));
         float2 vp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 132 + r * 4));
         // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
@@ -269,28 +286,24 @@ kv_attend_rows_kernel(const KvAttendParams p) {
               v = see ? v : -INFINITY;
             }
             s[a][n][2 * h + k] = v;
-            top[n][k] = fmaxf(top[n][k], v);
+            top = fmaxf(top, v - m[n][k]);
           }
       }
-    bool grows = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) top[n][k] = fmaxf(top[n][k], __shfl_xor_sync(0xffffffffu, top[n][k], x));
-        top[n][k] = top[n][k] > m[n][k] + 8.0f ? top[n][k] : m[n][k];
-        grows |= top[n][k] != m[n][k];
-      }
-    if (__any_sync(0xffffffffu, grows)) {
+    if (__any_sync(0xffffffffu, top > kRwTop)) {
+      // a weight would pass 2^15, or a row sees its first token: M moves, and what has been summed up is multiplied through
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float f[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float mn = top[n][k];
-          f[k] = mn != m[n][k] ? ex2(m[n][k] - mn) : 1.0f;
-          m[n][k] = mn;
+          float up = fmaxf(s[0][n][k], s[0][n][2 + k]);
+          if (TA == 2) up = fmaxf(up, fmaxf(s[TA - 1][n][k], s[TA - 1][n][2 + k]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, x));
+          const bool move = up - m[n][k] > kRwTop;
+          const float to = ceilf(up) - 1.0f;
+          f[k] = !move ? 1.0f : m[n][k] == -INFINITY ? 0.0f : ex2(m[n][k] - to);
+          m[n][k] = move ? to : m[n][k];
           l[n][k] *= f[k];
           y[n][k] *= f[k];
         }
@@ -302,15 +315,15 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         for (int e = 0; e < 4; ++e) ws[n][e] *= f[e & 1];
       }
     }
-    uint32_t pb[2][NT][2];
+    uint32_t pb[TA][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.0f : 6.0f - m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : 6.0f - m[n][1];
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < TA; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float w0 = ex2(s[a][n][2 * h] + m0), w1 = ex2(s[a][n][2 * h + 1] + m1);
+          const float w0 = ex2(s[a][n][2 * h] - m0), w1 = ex2(s[a][n][2 * h + 1] - m1);
           if (edge) {
             // a hidden token leaves the sums alone whatever its parameters hold
             if (w0 != 0.0f) { l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]); }
@@ -324,32 +337,32 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         }
     }
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < TA; ++a) {
       // slots 2c, 2c + 1, 2c + 8, 2c + 9: tokens of the tile
-      const int ta = 16 * a + rw_token_even(c), tb = 16 * a + rw_token_odd(c);
-      const unsigned char* sv = st + kRwTok * 64 + (g & 1) * 8;
-      const uint2 va = *reinterpret_cast<const uint2*>(sv + ta * 64 + (((g >> 1) ^ rw_swz(ta)) << 4));
-      const uint2 vb = *reinterpret_cast<const uint2*>(sv + tb * 64 + (((g >> 1) ^ rw_swz(tb)) << 4));
-      const uint2 vc = *reinterpret_cast<const uint2*>(sv + (ta + 8) * 64 + (((g >> 1) ^ rw_swz(ta + 8)) << 4));
-      const uint2 vd = *reinterpret_cast<const uint2*>(sv + (tb + 8) * 64 + (((g >> 1) ^ rw_swz(tb + 8)) << 4));
+      const unsigned char* sv = st + kRwTok * 64 + (16 * (a0 + a)) * 64 + (g & 1) * 8;
+      const unsigned char* sa = sv + ta * 64 + (((g >> 1) ^ rw_swz(ta)) << 4);
+      const unsigned char* sb = sv + tb * 64 + (((g >> 1) ^ rw_swz(tb)) << 4);
+      const uint2 va = *reinterpret_cast<const uint2*>(sa), vb = *reinterpret_cast<const uint2*>(sb);
+      const uint2 vc = *reinterpret_cast<const uint2*>(sa + 8 * 64), vd = *reinterpret_cast<const uint2*>(sb + 8 * 64);
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {                    // four dimensions of the lane's sixteen
         const uint32_t sel = (q4 & 1) ? 0x7632u : 0x5410u;
         const uint32_t ab = __byte_perm(q4 < 2 ? va.x : va.y, q4 < 2 ? vb.x : vb.y, sel);
         const uint32_t cd = __byte_perm(q4 < 2 ? vc.x : vc.y, q4 < 2 ? vd.x : vd.y, sel);
-        const uint32_t a0 = code_pair<0>(ab), a1 = code_pair<1>(ab), a2 = code_pair<0>(cd), a3 = code_pair<1>(cd);
-        const uint32_t b0 = code_pair<2>(ab), b1 = code_pair<3>(ab), b2 = code_pair<2>(cd), b3 = code_pair<3>(cd);
+        const uint32_t f0 = code_pair<0>(ab), f1 = code_pair<1>(ab), f2 = code_pair<0>(cd), f3 = code_pair<1>(cd);
+        const uint32_t h0 = code_pair<2>(ab), h1 = code_pair<3>(ab), h2 = code_pair<2>(cd), h3 = code_pair<3>(cd);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16(o[n][2 * q4], a0, a1, a2, a3, pb[a][n][0], pb[a][n][1]);
-          mma_f16(o[n][2 * q4 + 1], b0, b1, b2, b3, pb[a][n][0], pb[a][n][1]);
+          mma_f16(o[n][2 * q4], f0, f1, f2, f3, pb[a][n][0], pb[a][n][1]);
+          mma_f16(o[n][2 * q4 + 1], h0, h1, h2, h3, pb[a][n][0], pb[a][n][1]);
         }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16(ws[n], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[a][n][0], pb[a][n][1]);
     }
+    }
     __syncwarp();                                       // the stage is filled again in the next round
-    stage = stage + 1 == kRwStages ? 0 : stage + 1;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   rw_wait<0>();
   __syncthreads();                                      // the ring becomes the merge buffer
@@ -420,9 +433,9 @@ kv_attend_rows_kernel(const KvAttendParams p) {
 template <int NT>
 static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   constexpr int R = 8 * NT;
-  constexpr size_t smem = kRwRing + sizeof(RwShared<NT>);
-  static_assert(kRwWarps * R * kRwORow * sizeof(float) <= kRwRing, "the merge buffer lies in the ring");
-  static_assert(smem <= 227 * 1024, "shared memory");
+  constexpr size_t smem = RwConfig<NT>::kRing + sizeof(RwShared<NT>);
+  static_assert(kRwWarps * R * kRwORow * sizeof(float) <= RwConfig<NT>::kRing, "the merge buffer lies in the ring");
+  static_assert(RwConfig<NT>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory");
   // tiles: at most one ragged tile per sequence beyond the full ones; a grid of equal shares per sequence needs no search
   const int64_t per_seq = (max_rows + R - 1) / R;
   const int64_t bound = p.total_q * p.group / R + p.batch;
@@ -431,7 +444,7 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= num_sms()) splits *= 2;
+  while (splits < 8 && units * splits * 2 <= RwConfig<NT>::kCtas * num_sms()) splits *= 2;
   p.splits = splits;
   if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   QR_CUDA(cudaFuncSetAttribute(kv_attend_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -475,6 +488,8 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
     return fail(QR_EINVAL, "qr_kv_attend_i4: bad layer / page size / pages");
   if (num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads)
     return fail(QR_EINVAL, "qr_kv_attend_i4: %d query heads over %d KV heads (a multiple is needed)", num_q_heads, num_kv_heads);
+  if (num_pages > 0xffffffffll / (2ll * num_layers * num_kv_heads) / page_size)
+    return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: a pool of 2^32 or more (page, layer, key / value, head, slot) rows");
   if (window < 0 || sink_tokens < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative window or sink tokens");
   if (!qo_indptr && (total_q != batch || max_q_len != 1))
     return fail(QR_EINVAL, "qr_kv_attend_i4: without qo_indptr every sequence has one new token");

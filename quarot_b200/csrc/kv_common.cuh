@@ -39,7 +39,10 @@ __device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) {
 template <int J>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   const uint32_t x = J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6;
-  return (x & 0x03C003C0u) | 0x4C004C00u;
+  uint32_t r;
+  // (x & mask) | bias as one instruction; with both constants as immediates it would be two
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(0x03C003C0u), "r"(0x4C004C00u));
+  return r;
 }
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -75,7 +78,8 @@ __device__ __forceinline__ float4 kv_peer_f32x4(uint32_t addr) {
 #endif
 
 // Division of 0 <= n < 2^31 by a fixed d >= 1 as one wide multiplication: with s = ceil(log2 d) and
-// m = ceil(2^(31+s) / d) <= 2^32 - 1 (2^31 for d = 1), m d - 2^(31+s) < d <= 2^s, hence floor(n m / 2^(31+s)) = floor(n / d).
+// m = ceil(2^(31+s) / d) <= 2^32 - 1 (2^31 for d = 1), m d - 2^(31+s) < d <= 2^s, hence floor(n m / 2^(31+s)) = floor(n / d),
+// the upper half of 2 n times m shifted by s.
 struct FastDiv {
   uint32_t d, m;
   int s;
@@ -89,7 +93,7 @@ static inline FastDiv make_fastdiv(uint32_t d) {
 }
 #ifdef __CUDACC__
 __device__ __forceinline__ int fast_div(int n, const FastDiv& f) {
-  return (int)(((uint64_t)(uint32_t)n * f.m) >> (31 + f.s));
+  return (int)(__umulhi((uint32_t)n << 1, f.m) >> f.s);
 }
 #endif
 
