@@ -27,6 +27,9 @@
 #include "kv_common.cuh"
 
 #include <math.h>
+#include <map>
+#include <mutex>
+#include <utility>
 
 namespace qr {
 
@@ -411,23 +414,57 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   if (p.splits > 1) {
     kv_cluster_barrier();
     // the CTAs of the cluster deal out the rows
-    for (int r = (int)crank + p.splits * warp; r < w.rows; r += p.splits * kRwWarps) {
-      float mm = -INFINITY;
-      for (int x = 0; x < p.splits; ++x) mm = fmaxf(mm, kv_peer_f32(kv_peer_addr(&sh.part_m[r], x)));
-      float ll = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int x = 0; x < p.splits; ++x) {
-        const float mx = kv_peer_f32(kv_peer_addr(&sh.part_m[r], x)), lx = kv_peer_f32(kv_peer_addr(&sh.part_l[r], x));
-        if (mx == -INFINITY && lx == 0.0f) continue;
-        const float f = ex2(mx - mm);
-        const float4 v = kv_peer_f32x4(kv_peer_addr(&sh.part_o[r][4 * lane], x));
-        ll = fmaf(lx, f, ll);
-        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-      }
-      rw_store_row(p, w, head_kv, r, 4 * lane, acc, ll != 0.0f ? 1.0f / ll : 0.0f);
-    }
+    kv_merge_rows<1>(p.splits, (int)crank + p.splits * warp, p.splits * kRwWarps, w.rows, lane, sh.part_m, sh.part_l,
+                     [&](int r) { return &sh.part_o[r][4 * lane]; },
+                     [&](int r, float4 v, float inv) { rw_store_row(p, w, head_kv, r, 4 * lane, v, inv); });
     kv_cluster_barrier();
   }
+}
+
+int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, int64_t most, int* splits) {
+  constexpr int kMost = 16;
+  struct Known { int fit[kMost + 1]; };
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, Known> cache;
+  int dev = 0;
+  QR_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = cache.find({kernel, dev});
+  if (it == cache.end()) {
+    Known k = {};
+    QR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    int per_sm = 0;
+    QR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    k.fit[1] = per_sm * num_sms();
+    for (int s = 2; s <= kMost; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)s;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3((unsigned)s);
+      cfg.blockDim = dim3((unsigned)threads);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+      k.fit[s] = n;
+    }
+    it = cache.emplace(std::make_pair(kernel, dev), k).first;
+  }
+  // cost in parts of one unit's work: a round costs 1/16 of a unit beside its share of the work, twice that where shares
+  // have to be joined, so that a split has to pay
+  double best = 0.0;
+  *splits = 1;
+  for (int s = 1; s <= kMost && s <= most; ++s) {
+    const int fit = it->second.fit[s];
+    if (fit < 1) continue;
+    const double cost = (double)((units + fit - 1) / fit) * (1.0 / s + (s > 1 ? 2.0 : 1.0) / 16);
+    if (s == 1 || cost < best * 0.98) { best = cost; *splits = s; }
+  }
+  return QR_OK;
 }
 
 template <int NT>
@@ -443,11 +480,11 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
+  QR_CUDA(cudaFuncSetAttribute(kv_attend_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= RwConfig<NT>::kCtas * num_sms()) splits *= 2;
+  if (const int rc = kv_pick_splits((const void*)kv_attend_rows_kernel<NT>, 32 * kRwWarps, smem, units, (visible_blocks(p, max_rows, kRwTok) + kRwWarps - 1) / kRwWarps, &splits)) return rc;
   p.splits = splits;
   if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
-  QR_CUDA(cudaFuncSetAttribute(kv_attend_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

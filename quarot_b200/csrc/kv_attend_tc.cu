@@ -39,18 +39,24 @@ namespace qr {
 
 constexpr int kAtThreads = 640;
 constexpr int kAtRows = 256;
-constexpr int kAtTok = 128;
-constexpr int kAtTile = 128 * 128 * 2;                    // bytes of one 128 x 128 fp16 operand tile
-constexpr int kAtPairFloats = 12;                         // per column pair: ks ks kz kz | lv lv - - | rv rv zv zv
+constexpr int kAtTok = 96, kAtHalf = 48;                  // tokens of a block; columns of a score buffer
+constexpr int kAtQTile = 128 * 128 * 2;                   // bytes: 128 rows, two atoms of 64 dimensions
+constexpr int kAtKTile = kAtTok * 128 * 2;                // 96 tokens, two atoms of 64 dimensions
+constexpr int kAtVRows = 144;                             // 128 dimensions, 4 rows for the sums, filled up to a multiple of 16
+constexpr int kAtVAtom = kAtVRows * 128;                  // 64 tokens (of the second atom 32 are used)
+constexpr int kAtVTile = 2 * kAtVAtom;
+constexpr int kAtPairFloats = 8;                          // per column pair: ks ks kz kz | lv lv - -
 constexpr uint32_t kTmem = 0;                             // the CTA owns all 512 columns of tensor memory, from 0 on
+constexpr uint32_t kTmemO = kTmem, kTmemS = kTmem + 2 * kAtVRows;     // O_0 O_1 (144 columns each), then S of (tile, half)
 constexpr int kAtParStages = 3;
 constexpr float kAtTop = 15.0f;                           // weights are at most 2^15
-constexpr uint32_t kAtIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);    // fp16 x fp16 -> fp32, K-major, 128 x 64
-constexpr uint32_t kAtIdescO = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // 128 x 128
+constexpr uint32_t kAtIdescS = (1u << 4) | ((48u >> 3) << 17) | ((128u >> 4) << 24);    // fp16 x fp16 -> fp32, K-major, 128 x 48
+constexpr uint32_t kAtIdescO = (1u << 4) | ((144u >> 3) << 17) | ((128u >> 4) << 24);   // 128 x 144
 
 struct AtShared {
   float par[kAtParStages][kAtTok / 2][kAtPairFloats];
   long long row[2][2][kAtTok];                            // [keys / values][block & 1] rows of the tokens, -1: not read
+  __half vscale[2][kAtTok];                               // [block & 1] 2^-k of the tokens' value codes
   float qsum[kAtRows];
   int pos[kAtRows];
   float m[kAtRows], l[kAtRows];
@@ -58,19 +64,9 @@ struct AtShared {
   uint32_t tmem;
   int abort;
 };
-constexpr size_t kAtSmem = 1024 + 6 * kAtTile + sizeof(AtShared);
+constexpr size_t kAtSmem = 1024 + 2 * kAtQTile + 2 * kAtKTile + 2 * kAtVTile + sizeof(AtShared);
 static_assert(kAtSmem <= 227 * 1024, "shared memory");
 
-// One look at a barrier (a try_wait may sleep for some thousand cycles).
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok;
-}
 // The MMAs and commits are written for a warp whose lanes all run the issuing loop: addresses and descriptors then stay in
 // uniform registers, and only the instruction itself is predicated on the elected lane.
 __device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t acc) {
@@ -121,13 +117,6 @@ __device__ __forceinline__ void tmem_ld_16x256_x8(uint32_t taddr, uint32_t* r) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st_16x256_x4(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
-}
 __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
@@ -136,14 +125,21 @@ __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t* r) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x256_x2(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x128_x2(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr) : "memory");
+}
 // 16 lanes x 16 columns of fp16 pairs (32 matrix columns): r[2 k] is row g, r[2 k + 1] row g + 8, column pair 4 k + c.
 __device__ __forceinline__ void tmem_st_16x128_x4(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
                ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_16x128_x4(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
 }
 // Waits for the loads of this thread; the registers pass through, so that no use of them moves above the wait.
 template <int N>
@@ -175,10 +171,31 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   return r;
 }
 template <int J>
-__device__ __forceinline__ uint32_t at_centred_pair(uint32_t w) {     // 16 + c - 23.5, exact
+__device__ __forceinline__ uint32_t at_centred_pair(uint32_t w, __half2 scale, __half2 bias) {     // (c - 7.5) 2^-k, exact
   const uint32_t x = code_pair<J>(w);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(23.5f));
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), scale, bias);
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Value parameters of a token.  The weight of a token carries sigma = s' 2^k, its codes 2^-k, with the smallest k >= 0 for
+// which 2^10 / sigma and z' / sigma lie in the range of fp16 (k = 0 unless a row is all but constant or tiny; k <= 23, so
+// that (c - 7.5) 2^-k is exact).
+struct AtValue {
+  float sigma, down, z, bad;                              // sigma, 2^-k, z' / sigma - 7.5 2^-k, 0 or NaN
+};
+__device__ __forceinline__ AtValue at_value(uint32_t raw) {
+  float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+  AtValue r;
+  r.bad = (v.x - v.x) + (v.y - v.y);
+  // scales of a cache are positive; below 2^-22 the codes of a token cannot move an fp16 result by more than 2^-18
+  if (!(v.x >= 2.384185791015625e-07f)) v.x = 2.384185791015625e-07f;
+  if (r.bad != 0.0f) v = make_float2(1.0f, 0.0f);
+  const float need = __fdividef(fmaxf(0.03125f, fabsf(v.y) * 6.103515625e-05f), v.x);
+  int k = ((__float_as_int(need) + 0x7fffff) >> 23) - 127;
+  k = min(max(k, 0), 23);
+  r.down = __int_as_float((127 - k) << 23);
+  r.sigma = v.x * __int_as_float((127 + k) << 23);
+  r.z = fmaf(-7.5f, r.down, __fdividef(v.y, r.sigma));
+  return r;
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -195,7 +212,6 @@ __device__ __forceinline__ __half* at_out_row(const KvAttendParams& p, const KvT
 // What a lane of a softmax warp keeps of its four rows (g + 8 x of the warp's 32).
 struct AtRows {
   float m[4], qs[4];
-  uint64_t l2[4], y2[4];
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -210,8 +226,16 @@ __device__ __forceinline__ void at_hide(float& v0, float& v1, int t, int pos, in
   if (t + 1 > pos || (t + 1 <= lo && t + 1 >= sinks)) v1 = -INFINITY;
 }
 
-// The exponents of 32 columns, relative to M, in place of S; the lane's largest is returned.
-__device__ __forceinline__ float at_scores(uint32_t (&s)[2][16], const float* par, const AtRows& w) {
+// 48 columns of S of the warp's 32 rows: s[0] rows 0 - 15, s[1] rows 16 - 31, pairs 4 k + 2 (row / 8 & 1) of column group k.
+__device__ __forceinline__ void at_fetch(uint32_t (&s)[2][24], uint32_t t_s) {
+  tmem_ld_16x256_x4(t_s, s[0]);
+  tmem_ld_16x256_x4(t_s + (16u << 16), s[1]);
+  tmem_ld_16x256_x2(t_s + 32, s[0] + 16);
+  tmem_ld_16x256_x2(t_s + 32 + (16u << 16), s[1] + 16);
+}
+
+// The exponents of 48 columns, relative to M, in place of S; the lane's largest is returned.
+__device__ __forceinline__ float at_scores(uint32_t (&s)[2][24], const float* par, const AtRows& w) {
   uint64_t off[4], qq[4];
   float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
@@ -220,7 +244,7 @@ __device__ __forceinline__ float at_scores(uint32_t (&s)[2][16], const float* pa
     qq[x] = f2_pack(w.qs[x], w.qs[x]);
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 6; ++k) {
     const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
     const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
     const uint64_t ks = f2_pack(a.x, a.y), kz = f2_pack(a.z, a.w), lv = f2_pack(b.x, b.y);
@@ -241,13 +265,13 @@ __device__ __forceinline__ float at_scores(uint32_t (&s)[2][16], const float* pa
 
 // Hides what the rows do not see (pos: positions of the warp's rows, t: token of the lane's first column); the largest of
 // what is left.
-__device__ __forceinline__ float at_mask(uint32_t (&s)[2][16], const int* pos, int t, int window, int sinks) {
+__device__ __forceinline__ float at_mask(uint32_t (&s)[2][24], const int* pos, int t, int window, int sinks) {
   float top = -INFINITY;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int ps = pos[8 * x];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 6; ++k) {
       uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
       float v0 = __uint_as_float(r[0]), v1 = __uint_as_float(r[1]);
       at_hide(v0, v1, t + 8 * k, ps, window, sinks);
@@ -259,35 +283,28 @@ __device__ __forceinline__ float at_mask(uint32_t (&s)[2][16], const int* pos, i
   return top;
 }
 
-// The weights of 32 columns: into the sums, and as fp16 to tensor memory.
-__device__ __forceinline__ void at_weights(const uint32_t (&s)[2][16], const float* par, AtRows& w, uint32_t t_p) {
-  uint32_t pk[2][8];
+// The weights of 48 columns, as fp16 to tensor memory.
+__device__ __forceinline__ void at_weights(const uint32_t (&s)[2][24], uint32_t t_p) {
+  uint32_t pk[2][12];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float4 b = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats + 8);
-    const uint64_t rv = f2_pack(b.x, b.y), zv = f2_pack(b.z, b.w);
+  for (int x = 0; x < 2; ++x) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
-      const float w0 = ex2(__uint_as_float(r[0])), w1 = ex2(__uint_as_float(r[1]));
-      const uint64_t ww = f2_pack(w0, w1);
-      w.l2[x] = f2_fma(ww, rv, w.l2[x]);
-      w.y2[x] = f2_fma(ww, zv, w.y2[x]);
-      const __half2 wh = __floats2half2_rn(w0, w1);
-      pk[x >> 1][2 * k + (x & 1)] = *reinterpret_cast<const uint32_t*>(&wh);
+    for (int e = 0; e < 12; ++e) {
+      const __half2 wh = __floats2half2_rn(ex2(__uint_as_float(s[x][2 * e])), ex2(__uint_as_float(s[x][2 * e + 1])));
+      pk[x][e] = *reinterpret_cast<const uint32_t*>(&wh);
     }
+    tmem_st_16x128_x4(t_p + ((uint32_t)x << 20), pk[x]);
+    tmem_st_16x128_x2(t_p + 16 + ((uint32_t)x << 20), pk[x] + 8);
   }
-  tmem_st_16x128_x4(t_p, pk[0]);
-  tmem_st_16x128_x4(t_p + (16u << 16), pk[1]);
 }
 
-// The largest exponents of the four rows over 32 columns, relative to nothing.
-__device__ __forceinline__ void at_tops(uint32_t (&s)[2][16], const float* par, const AtRows& w, float (&top)[4], bool edge, const int* pos, int t,
+// The largest exponents of the four rows over 48 columns, relative to nothing.
+__device__ __forceinline__ void at_tops(uint32_t (&s)[2][24], const float* par, const AtRows& w, float (&top)[4], bool edge, const int* pos, int t,
                                         int window, int sinks) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) top[x] = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 6; ++k) {
     const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
     const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
 #pragma unroll
@@ -305,65 +322,109 @@ __device__ __forceinline__ void at_tops(uint32_t (&s)[2][16], const float* par, 
   }
 }
 
-// Multiplies columns of O (fp32) by the factors of the four rows.
+// Multiplies O, the columns of the sums included, by the factors of the four rows.
 __device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
 #pragma unroll 1
-  for (int q = 0; q < 8; ++q) {
-    uint32_t o[16];
-    const uint32_t at = t_o + (q >> 1) * 32 + ((uint32_t)(q & 1) << 20);
-    tmem_ld_16x256_x4(at, o);
-    tmem_ld_done<16>(o);
+  for (int q = 0; q < 2 * kAtVRows / 16; ++q) {
+    uint32_t o[8];
+    const uint32_t at = t_o + (q >> 1) * 16 + ((uint32_t)(q & 1) << 20);
+    tmem_ld_16x256_x2(at, o);
+    tmem_ld_done<8>(o);
     const float fa = q & 1 ? f[2] : f[0], fb = q & 1 ? f[3] : f[1];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? fb : fa));
-    tmem_st_16x256_x4(at, o);
+    for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? fb : fa));
+    tmem_st_16x256_x2(at, o);
   }
   tmem_st_done();
 }
 
-// M has become mn: l, y and the weights of the first `pieces` x 32 columns, which are in tensor memory, follow.  The
-// factors are powers of two (M moves in whole steps) or 0.
-__device__ __forceinline__ void at_follow(AtRows& w, const float (&mn)[4], float (&f)[4], int pieces, uint32_t t_p) {
+// The 32 query rows of a softmax warp: into the Q tile, their sums and positions.  Four rows at a time, eight lanes to a row
+// and sixteen dimensions to a lane, so that the rotation needs three exchanges between lanes instead of five.  8 dimensions
+// 8 i .. 8 i + 7 lie as 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart.
+// (A call: inlined, its registers cost the loop of the softmax 5 %.)
+__device__ __noinline__ void at_load_rows(const KvAttendParams& p, int w_row0, int w_rows, int w_pos0, int64_t w_tok0, int head_kv, int row0,
+                                          int lane, unsigned char* tile, float* s_sum, int* s_pos) {
+  const int sub = lane >> 3, l8 = lane & 7;
+  uint2 raw[4], ahead[4];
+  int pos = -1, pos_ahead = -1;
+  auto fetch = [&](int r) {
+    pos_ahead = -1;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    f[x] = mn[x] == w.m[x] ? 1.0f : w.m[x] == -INFINITY ? 0.0f : ex2(w.m[x] - mn[x]);
-    w.m[x] = mn[x];
-    const uint64_t ff = f2_pack(f[x], f[x]);
-    w.l2[x] = f2_fma(w.l2[x], ff, 0);
-    w.y2[x] = f2_fma(w.y2[x], ff, 0);
-  }
-  tmem_st_done();
-#pragma unroll 1
-  for (int q = 0; q < 2 * pieces; ++q) {
-    uint32_t h[8];
-    const uint32_t at = t_p + (q >> 1) * 16 + ((uint32_t)(q & 1) << 20);
-    tmem_ld_16x128_x4(at, h);
-    tmem_ld_done<8>(h);
-    const float fa = q & 1 ? f[2] : f[0], fb = q & 1 ? f[3] : f[1];
+    for (int e = 0; e < 4; ++e) ahead[e] = make_uint2(0, 0);
+    if (r < w_rows) {
+      const int row = w_row0 + r;
+      const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
+      pos_ahead = w_pos0 + tok;
+      const uint2* src = reinterpret_cast<const uint2*>(p.q + (w_tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs) + 4 * l8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-      const float ff = e & 1 ? fb : fa;
-      const __half2 r = __floats2half2_rn(v.x * ff, v.y * ff);
-      h[e] = *reinterpret_cast<const uint32_t*>(&r);
+      for (int e = 0; e < 4; ++e) ahead[e] = src[e];
     }
-    tmem_st_16x128_x4(at, h);
+  };
+  fetch(row0 + sub);
+#pragma unroll 1
+  for (int r = row0 + sub; r < row0 + 32; r += 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw[e] = ahead[e];
+    pos = pos_ahead;
+    if (r + 4 < row0 + 32) fetch(r + 4);
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].y));
+      x[4 * e] = lo.x; x[4 * e + 1] = lo.y; x[4 * e + 2] = hi.x; x[4 * e + 3] = hi.y;
+    }
+    if (p.hadamard_q) {
+#pragma unroll
+      for (int h = 1; h < 16; h <<= 1)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((e & h) == 0) {
+            const float a = x[e], b = x[e + h];
+            x[e] = a + b;
+            x[e + h] = a - b;
+          }
+#pragma unroll 1
+      for (int s = 1; s < 8; s <<= 1) {
+        const float sg = (lane & s) ? -1.0f : 1.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], sg, __shfl_xor_sync(0xffffffffu, x[e], s));
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum += x[e];
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const int rr = r & 127;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      uint32_t h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __half2 hv = __floats2half2_rn(x[8 * v + e], x[8 * v + e + 4]);
+        h[e] = *reinterpret_cast<const uint32_t*>(&hv);
+      }
+      const int ch = 2 * l8 + v;
+      *reinterpret_cast<uint4*>(tile + (ch >> 3) * (kAtQTile / 2) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    if (l8 == 0) { s_sum[r] = sum; s_pos[r] = pos; }
   }
-  tmem_st_done();
 }
 
 __global__ void __launch_bounds__(kAtThreads, 1)
-kv_attend_tc_kernel(const KvAttendParams p) {
+kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   extern __shared__ unsigned char s_raw[];
   const uint32_t base = (smem_u32(s_raw) + 1023u) & ~1023u;
   unsigned char* smem = s_raw + (base - smem_u32(s_raw));
-  // [Q tile 0, Q tile 1][K 2 stages][V 2 stages][AtShared]; the merge area is Q and K, the fp16 result of a row tile goes
-  // through its Q tile
-  const uint32_t s_q = base, s_k = base + 2 * kAtTile, s_v = base + 4 * kAtTile;
-  AtShared& sh = *reinterpret_cast<AtShared*>(smem + 6 * kAtTile);
+  // [Q tile 0, Q tile 1][K 2 stages][V 2 stages][AtShared]; the merge area is Q, K and a part of V, the fp16 result of a row
+  // tile goes through its Q tile
+  const uint32_t s_q = base, s_k = base + 2 * kAtQTile, s_v = s_k + 2 * kAtKTile;
+  AtShared& sh = *reinterpret_cast<AtShared*>(smem + 2 * kAtQTile + 2 * kAtKTile + 2 * kAtVTile);
   const uint32_t bars = smem_u32(sh.bars);
   const uint32_t k_full = bars, k_empty = bars + 16, v_full = bars + 32, v_empty = bars + 48, par_full = bars + 64, s_full = bars + 88,
-                 p_full = bars + 120, pv_done = bars + 152, o_full = bars + 168;   // 2 2 2 2 3 [2][2] [2][2] 2 2
+                 p_full = bars + 120, pv_done = bars + 152, o_full = bars + 168, q_full = bars + 184;   // 2 2 2 2 3 [2][2] [2][2] 2 2 2
   volatile int* abort_flag = &sh.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t crank = 0;
@@ -386,7 +447,7 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       mbar_init(v_full + 8 * s, 4); mbar_init(v_empty + 8 * s, tiles);
       mbar_init(s_full + 16 * s, 1); mbar_init(s_full + 16 * s + 8, 1);
       mbar_init(p_full + 16 * s, 4); mbar_init(p_full + 16 * s + 8, 4);
-      mbar_init(pv_done + 8 * s, 1); mbar_init(o_full + 8 * s, 1);
+      mbar_init(pv_done + 8 * s, 1); mbar_init(o_full + 8 * s, 1); mbar_init(q_full + 8 * s, 4);
     }
     for (int s = 0; s < kAtParStages; ++s) mbar_init(par_full + 8 * s, 4);
     sh.abort = 0;
@@ -396,52 +457,6 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
   }
-  // query rows: 8 dimensions 8 i .. 8 i + 7 lie as 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart
-  constexpr int kWarps = kAtThreads / 32, kTogether = 7;  // loads in flight per warp: two rounds for 256 rows
-  for (int r0 = warp; r0 < 128 * tiles; r0 += kTogether * kWarps) {
-    uint2 raw[kTogether];
-    int pos[kTogether];
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) {
-      const int r = r0 + u * kWarps;
-      raw[u] = make_uint2(0, 0);
-      pos[u] = -1;
-      if (r < w.rows) {
-        const int row = w.row0 + r;
-        const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
-        pos[u] = w.pos0 + tok;
-        raw[u] = *reinterpret_cast<const uint2*>(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) {
-      const int r = r0 + u * kWarps;
-      if (r >= 128 * tiles) break;
-      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw[u].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw[u].y));
-      float x[4] = {lo.x, lo.y, hi.x, hi.y};
-      if (p.hadamard_q) {
-        fwht128_warp(x, lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
-      }
-      float sum = x[0] + x[1] + x[2] + x[3];
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      const bool odd = lane & 1;
-      const float give0 = odd ? x[0] : x[2], give1 = odd ? x[1] : x[3];
-      const float got0 = __shfl_xor_sync(0xffffffffu, give0, 1), got1 = __shfl_xor_sync(0xffffffffu, give1, 1);
-      const __half2 h0 = odd ? __floats2half2_rn(got0, x[2]) : __floats2half2_rn(x[0], got0);
-      const __half2 h1 = odd ? __floats2half2_rn(got1, x[3]) : __floats2half2_rn(x[1], got1);
-      const int rr = r & 127, ch = (lane >> 1) & 7;
-      unsigned char* dst = smem + (r >> 7) * kAtTile + (lane >> 4) * (kAtTile / 2) + rr * 128 + ((ch ^ (rr & 7)) << 4) + (odd ? 8 : 0);
-      uint2 q;
-      q.x = *reinterpret_cast<const uint32_t*>(&h0);
-      q.y = *reinterpret_cast<const uint32_t*>(&h1);
-      *reinterpret_cast<uint2*>(dst) = q;
-      if (lane == 0) { sh.qsum[r] = sum; sh.pos[r] = pos[u]; }
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -451,102 +466,85 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     regs_inc<160>();
     const int i = warp >> 2, g = lane >> 2, c = lane & 3;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;                    // first tensor-memory lane of the warp, << 16
-    const uint32_t t_s = kTmem + i * 128 + lanes, t_o = kTmem + 256 + i * 128 + lanes;
+    const uint32_t t_s = kTmemS + i * (2 * kAtHalf) + lanes, t_o = kTmemO + i * kAtVRows + lanes;
     const int row0 = i * 128 + (warp & 3) * 32;                           // the lane's rows: row0 + g + 8 x, x = 0 .. 3
     const int* pos = &sh.pos[row0 + g];
+    if (i < tiles) {
+      at_load_rows(p, w.row0, w.rows, w.pos0, w.tok0, head_kv, row0, lane, smem + i * kAtQTile, sh.qsum, sh.pos);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + 8 * i);
+    }
     AtRows rw;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       rw.m[x] = -INFINITY;
-      rw.l2[x] = 0; rw.y2[x] = 0;
       rw.qs[x] = i < tiles ? sh.qsum[row0 + g + 8 * x] : 0.0f;
     }
     bool ok = i < tiles;
-    // 32 columns of half h: exponents, M where it has to move, weights
-    auto piece = [&](uint32_t (&s)[2][16], int h, int part, const float* par, bool edge, int t) {
-      const uint32_t t_sb = t_s + 64 * (h & 1);
+    // One copy of the code for all half blocks, the rare branches out of its way: with the loop unrolled, the warps of a
+    // scheduler spent a third of their time on instruction fetches.  The next scores are asked for as soon as the
+    // registers of these are free.
+    uint32_t s[2][24];
+    int ring = 0, ring_phase = 0;
+    const float* par = &sh.par[0][c][0];
+    if (ok && n > 0) {
+      ok = mbar_wait(par_full, 0, abort_flag, p.status, 71) && mbar_wait(s_full + 16 * i, 0, abort_flag, p.status, 72);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      at_fetch(s, t_s);
+    }
+    int t0 = kv_block_index(blk, begin) * kAtTok;         // first token of the half block
+#pragma unroll 1
+    for (int h = 0; ok && h < 2 * n; ++h) {
+      const bool edge = t0 + kAtHalf - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kAtHalf - 1 >= p.sinks);
+      const uint32_t t_sb = t_s + (h & 1) * kAtHalf;
+      tmem_ld_done<24>(s[0]);
+      tmem_ld_done<24>(s[1]);
       float top = at_scores(s, par, rw);
-      if (edge) top = at_mask(s, pos, t, p.window, p.sinks);
-      if (__any_sync(0xffffffffu, top > kAtTop)) {
-        // a weight would pass 2^15, or a row sees its first token
-        tmem_ld_16x256_x4(t_sb + 32 * part, s[0]);
-        tmem_ld_16x256_x4(t_sb + 32 * part + (16u << 16), s[1]);
-        tmem_ld_done<16>(s[0]);
-        tmem_ld_done<16>(s[1]);
+      if (__builtin_expect(edge, 0)) top = at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
+      if (__builtin_expect(__any_sync(0xffffffffu, top > kAtTop), 0)) {
+        // a weight would pass 2^15, or a row sees its first token: M moves, O follows by powers of two (or 0)
+        at_fetch(s, t_sb);
+        tmem_ld_done<24>(s[0]);
+        tmem_ld_done<24>(s[1]);
         float mn[4], f[4];
-        at_tops(s, par, rw, mn, edge, pos, t, p.window, p.sinks);
+        at_tops(s, par, rw, mn, edge, pos, t0 + 2 * c, p.window, p.sinks);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mn[x] = mn[x] - rw.m[x] > kAtTop ? ceilf(mn[x]) - 1.0f : rw.m[x];
-        at_follow(rw, mn, f, part, t_sb);
+        for (int x = 0; x < 4; ++x) {
+          const bool move = mn[x] - rw.m[x] > kAtTop;
+          const float to = ceilf(mn[x]) - 1.0f;
+          f[x] = !move ? 1.0f : rw.m[x] == -INFINITY ? 0.0f : ex2(rw.m[x] - to);
+          rw.m[x] = move ? to : rw.m[x];
+        }
         if (h > 0) {                                      // the products of half h - 1 may still be on their way
           ok = mbar_wait(pv_done + 8 * i, (h - 1) & 1, abort_flag, p.status, 73) && ok;
           tc_fence_after();
           at_scale_o(t_o, f);
         }
         at_scores(s, par, rw);
-        if (edge) at_mask(s, pos, t, p.window, p.sinks);
+        if (edge) at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
       }
-      // the weights take the place of columns of S that are in registers
-      at_weights(s, par, rw, t_sb + 16 * part);
-    };
-    // two pieces of 32 columns per half block; the next piece is on its way while one is worked on
-    uint32_t sa[2][16], sb[2][16];                        // [rows 0 - 15 / 16 - 31 of the warp][..]
-    int ring = 0, ring_phase = 0;
-    bool fetched = false;
-#pragma unroll 1
-    for (int h = 0; ok && h < 2 * n; ++h) {               // half blocks of 64 tokens
-      const int buf = h & 1;
-      const uint32_t t_sb = t_s + 64 * buf;
-      if (!buf) {
-        if (h && ++ring == kAtParStages) { ring = 0; ring_phase ^= 1; }
-        ok = mbar_wait(par_full + 8 * ring, ring_phase, abort_flag, p.status, 71);
-      }
-      if (!fetched) {
-        ok = mbar_wait(s_full + 16 * i + 8 * buf, (h >> 1) & 1, abort_flag, p.status, 72) && ok;
-        tc_fence_after();
-        tmem_ld_16x256_x4(t_sb, sa[0]);
-        tmem_ld_16x256_x4(t_sb + (16u << 16), sa[1]);
-      }
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      const int t0 = kv_block_index(blk, begin + (h >> 1)) * kAtTok + 64 * buf;
-      const bool edge = t0 + 63 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + 63 >= p.sinks);
-      const float* par = &sh.par[ring][c + 32 * buf][0];
-      tmem_ld_done<16>(sa[0]);
-      tmem_ld_done<16>(sa[1]);
-      tmem_ld_16x256_x4(t_sb + 32, sb[0]);
-      tmem_ld_16x256_x4(t_sb + 32 + (16u << 16), sb[1]);
-      piece(sa, h, 0, par, edge, t0 + 2 * c);
-      tmem_ld_done<16>(sb[0]);
-      tmem_ld_done<16>(sb[1]);
-      // the scores of the next half do not depend on these weights: where they are there already, they are fetched ahead
-      fetched = h + 1 < 2 * n && __all_sync(0xffffffffu, mbar_test(s_full + 16 * i + 8 * (buf ^ 1), ((h + 1) >> 1) & 1));
-      if (fetched) {
-        tc_fence_after();
-        tmem_ld_16x256_x4(t_s + 64 * (buf ^ 1), sa[0]);
-        tmem_ld_16x256_x4(t_s + 64 * (buf ^ 1) + (16u << 16), sa[1]);
-      }
-      piece(sb, h, 1, par + 16 * kAtPairFloats, edge, t0 + 32 + 2 * c);
+      at_weights(s, t_sb);                                // in place of S, which is in registers
       tmem_st_done();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * buf);
+      if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * (h & 1));
+      if (h + 1 == 2 * n) break;
+      t0 += kAtHalf;
+      par += kAtHalf / 2 * kAtPairFloats;
+      if (h & 1) {                                        // the block is done
+        if (++ring == kAtParStages) { ring = 0; ring_phase ^= 1; }
+        par = &sh.par[ring][c][0];
+        t0 = kv_block_index(blk, begin + ((h + 1) >> 1)) * kAtTok;
+        ok = mbar_wait(par_full + 8 * ring, ring_phase, abort_flag, p.status, 71) && ok;
+      }
+      ok = mbar_wait(s_full + 16 * i + 8 * ((h + 1) & 1), ((h + 1) >> 1) & 1, abort_flag, p.status, 72) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      at_fetch(s, t_s + ((h + 1) & 1) * kAtHalf);
     }
     ok = __all_sync(0xffffffffu, ok);
-    // sums over the four lanes of a row
-    float l[4], y[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      float e, f;
-      f2_unpack(rw.l2[x], e, f);
-      l[x] = e + f;
-      f2_unpack(rw.y2[x], e, f);
-      y[x] = e + f;
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        l[x] += __shfl_xor_sync(0xffffffffu, l[x], d);
-        y[x] += __shfl_xor_sync(0xffffffffu, y[x], d);
-      }
-    }
     if (ok && n > 0) {
       ok = mbar_wait(o_full + 8 * i, 0, abort_flag, p.status, 80);
       ok = __all_sync(0xffffffffu, ok);
@@ -555,6 +553,25 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     if (p.splits > 1) asm volatile("bar.sync 3, 256;" ::: "memory");
     if (ok) {
       tc_fence_after();
+      // the sums: columns 128, 129 (2^10 w / sigma, in two parts) in lane c = 0, 130, 131 (w (z' / sigma - ..)) in lane c = 1
+      float l[4], y[4];
+#pragma unroll
+      for (int q2 = 0; q2 < 2; ++q2) {
+        uint32_t o[8];
+        if (n > 0) {
+          tmem_ld_16x256_x2(t_o + 128 + ((uint32_t)q2 << 20), o);
+          tmem_ld_done<8>(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = 0;
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const float sum = __uint_as_float(o[2 * hh]) + __uint_as_float(o[2 * hh + 1]);
+          l[2 * q2 + hh] = __shfl_sync(0xffffffffu, sum, lane & ~3) * 0.0009765625f;
+          y[2 * q2 + hh] = __shfl_sync(0xffffffffu, sum, (lane & ~3) + 1);
+        }
+      }
 #pragma unroll 1
       for (int q4 = 0; q4 < 4; ++q4) {                    // columns 64 (q4 / 2) .., rows 16 (q4 % 2) ..
         uint32_t o[32];
@@ -600,28 +617,16 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     if (p.splits > 1) {
       kv_cluster_barrier();
       // the CTAs of the cluster deal out the rows
-      for (int r = (int)crank + p.splits * warp; r < w.rows; r += p.splits * 8) {
-        float mm = -INFINITY;
-        for (int x = 0; x < p.splits; ++x) mm = fmaxf(mm, kv_peer_f32(kv_peer_addr(&sh.m[r], x)));
-        float ll = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int x = 0; x < p.splits; ++x) {
-          const float mx = kv_peer_f32(kv_peer_addr(&sh.m[r], x));
-          const float lx = kv_peer_f32(kv_peer_addr(&sh.l[r], x));
-          if (mx == -INFINITY && lx == 0.0f) continue;
-          const float f = ex2(mx - mm);
-          const float4 v = kv_peer_f32x4(kv_peer_addr(smem + at_part_off(r, lane), x));
-          ll = fmaf(lx, f, ll);
-          acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-        }
-        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-        const __half2 h0 = __floats2half2_rn(acc.x * inv, acc.y * inv), h1 = __floats2half2_rn(acc.z * inv, acc.w * inv);
-        uint2 out;
-        out.x = *reinterpret_cast<const uint32_t*>(&h0);
-        out.y = *reinterpret_cast<const uint32_t*>(&h1);
-        *reinterpret_cast<uint2*>(at_out_row(p, w, head_kv, r) + 4 * lane) = out;
-      }
-      kv_cluster_barrier();                                  // nobody leaves while its shared memory may still be read
+      kv_merge_rows<2>(p.splits, (int)crank + p.splits * warp, p.splits * 8, w.rows, lane, sh.m, sh.l,
+                       [&](int r) { return smem + at_part_off(r, lane); },
+                       [&](int r, float4 v, float inv) {
+                         const __half2 h0 = __floats2half2_rn(v.x * inv, v.y * inv), h1 = __floats2half2_rn(v.z * inv, v.w * inv);
+                         uint2 out;
+                         out.x = *reinterpret_cast<const uint32_t*>(&h0);
+                         out.y = *reinterpret_cast<const uint32_t*>(&h1);
+                         *reinterpret_cast<uint2*>(at_out_row(p, w, head_kv, r) + 4 * lane) = out;
+                       });
+      kv_cluster_barrier();                               // nobody leaves while its shared memory may still be read
     }
   } else if (warp < 16) {
     // ---------------------------------------------------------------- unpacking: warps 8 - 11 keys and parameters, 12 - 15 values
@@ -636,17 +641,17 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     const size_t row_0 = row_k + (what ? v_rows : 0);
     auto page_id = [&](int j) -> int {
       const int t = kv_block_index(blk, begin + j) * kAtTok + tid;
-      return t < tokens ? __ldg(p.indices + first_page + fast_div(t, p.page_div)) : 0;
+      return tid < kAtTok && t < tokens ? __ldg(p.indices + first_page + fast_div(t, p.page_div)) : 0;
     };
     auto put_rows = [&](int j, int id) -> long long {
       const int t = kv_block_index(blk, begin + j) * kAtTok + tid;
       long long row = -1;
-      if (t < tokens) {
+      if (tid < kAtTok && t < tokens) {
         const int slot = t - fast_div(t, p.page_div) * p.page_size;
         const size_t page = min((size_t)(uint32_t)id, (size_t)p.num_pages - 1);        // an index outside the pool reads its last page
         row = (long long)(page * page_rows + row_0 + slot);
       }
-      sh.row[what][j & 1][tid] = row;
+      if (tid < kAtTok) sh.row[what][j & 1][tid] = row;
       asm volatile("bar.sync %0, 128;" ::"r"(1 + what) : "memory");
       return row;
     };
@@ -656,11 +661,11 @@ kv_attend_tc_kernel(const KvAttendParams p) {
       // row (lane & 7) + 8 (warp + 4 it), 16-byte chunk lane / 8
       const float sm_scale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
       const int kr = (lane & 7) + 8 * pw, kc = lane >> 3;
-      uint4 kw[4];
+      uint4 kw[3];
       uint32_t kp = 0, vp = 0;
       auto load = [&](int j, long long mine) {
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
+        for (int it = 0; it < 3; ++it) {
           const long long row = sh.row[0][j & 1][kr + 32 * it];
           kw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.data + row * 64 + 16 * kc)) : make_uint4(0, 0, 0, 0);
         }
@@ -685,26 +690,19 @@ kv_attend_tc_kernel(const KvAttendParams p) {
           mbar_wait(k_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 74);
           __syncwarp();
         }
-        {
+        if (tid < kAtTok) {
           // parameters of token tid; the slot of the ring is free: the scores of block j - 2 were issued after the weights of
           // block j - 3 had been made
           const float2 k2 = __half22float2(*reinterpret_cast<const __half2*>(&kp));
-          float2 v2 = __half22float2(*reinterpret_cast<const __half2*>(&vp));
-          // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
-          if (v2.x < 9.31322575e-10f) v2.x = 9.31322575e-10f;
-          const float rv = __fdividef(1.0f, v2.x), ks = k2.x * sm_scale;
-          // x - x: 0, or NaN where it is not finite.  Then the weight of the token is NaN in the rows that see it, and its
-          // other numbers are 0, so that a weight 0 leaves the sums of the rows that do not see it alone.
-          const float bad = ((k2.x - k2.x) + (k2.y - k2.y)) + ((v2.x - v2.x) + (v2.y - v2.y));
-          const bool fine = bad == 0.0f;
+          const AtValue v = at_value(vp);
+          const float ks = k2.x * sm_scale;
           float* q = &sh.par[ring][tid >> 1][tid & 1];
           q[0] = ks;
           q[2] = -fmaf(16.0f, ks, k2.y * sm_scale);
-          q[4] = __log2f(v2.x) + bad;
-          q[8] = fine ? rv : 0.0f;
-          q[10] = fine ? fmaf(v2.y, rv, -7.5f) : 0.0f;
+          // x - x: 0, or NaN where it is not finite: the weight of such a token is NaN in the rows that see it
+          q[4] = __log2f(v.sigma) + ((k2.x - k2.x) + (k2.y - k2.y) + v.bad);
         }
-        const uint32_t dst = s_k + stage * kAtTile + (kc >> 1) * (kAtTile / 2);
+        const uint32_t dst = s_k + stage * kAtKTile + (kc >> 1) * (kAtKTile / 2);
 #pragma unroll 1
         for (int r = kr; r < kAtTok; r += 32) {           // the words of the next round move up: see the note on code size
           const uint32_t ww[4] = {kw[0].x, kw[0].y, kw[0].z, kw[0].w};
@@ -714,7 +712,7 @@ kv_attend_tc_kernel(const KvAttendParams p) {
             st_shared16(dst + r * 128 + ((ch ^ (r & 7)) << 4), code_pair<0>(ww[x]), code_pair<1>(ww[x]), code_pair<2>(ww[x]),
                         code_pair<3>(ww[x]));
           }
-          kw[0] = kw[1]; kw[1] = kw[2]; kw[2] = kw[3];
+          kw[0] = kw[1]; kw[1] = kw[2];
         }
         if (j + 1 < n) load(j + 1, mine);
         fence_proxy_async_smem();
@@ -725,52 +723,83 @@ kv_attend_tc_kernel(const KvAttendParams p) {
         }
       }
     } else {
-      // tokens 64 (warp & 1) + 8 (lane & 7) + 0 .. 7, 8 bytes (16 dimensions) at 32 (warp / 2) + 8 (lane / 8)
-      const int vt = 64 * (pw & 1) + 8 * (lane & 7), vb = 32 * (pw >> 1) + 8 * (lane >> 3);
+      // warps 0, 1: tokens 8 (lane & 7) + 0 .. 7 of the first atom, 8 bytes (16 dimensions) at 32 warp + 8 (lane / 8); warp 2:
+      // tokens 64 + 8 (lane & 3) + 0 .. 7, 8 bytes at 8 (lane / 4); thread t < 96: the rows of the sums for token t
+      const int tg = pw < 2 ? lane & 7 : lane & 3;
+      const int vt = pw < 2 ? 8 * tg : 64 + 8 * tg, vb = pw < 2 ? 32 * pw + 8 * (lane >> 3) : 8 * (lane >> 2);
       uint2 vw[8];
+      uint32_t vp = 0;
       auto load = [&](int j) {
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
-          const long long row = sh.row[1][j & 1][vt + it];
+          const long long row = pw < 3 ? sh.row[1][j & 1][vt + it] : -1;
           vw[it] = row >= 0 ? __ldg(reinterpret_cast<const uint2*>(p.data + row * 64 + vb)) : make_uint2(0, 0);
         }
       };
+      auto load_par = [&](long long mine) { vp = mine >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(p.param + mine)) : 0u; };
+      long long mine = -1;
       if (n > 0) {
-        put_rows(0, page_id(0));
+        mine = put_rows(0, page_id(0));
+        load_par(mine);
         load(0);
         if (n > 1) id = page_id(1);
       }
       for (int j = 0; j < n; ++j) {
         const int stage = j & 1;
+        const AtValue v = at_value(vp);
+        if (tid < kAtTok) sh.vscale[stage][tid] = __float2half_rn(v.down);
         if (j + 1 < n) {
-          put_rows(j + 1, id);
+          mine = put_rows(j + 1, id);                     // its barrier orders the scales as well
+          load_par(mine);
           if (j + 2 < n) id = page_id(j + 2);
+        } else {
+          asm volatile("bar.sync 2, 128;" ::: "memory");
         }
         if (j >= 2) {
           mbar_wait(v_empty + 8 * stage, ((j >> 1) + 1) & 1, abort_flag, p.status, 75);
           __syncwarp();
         }
-        const uint32_t dst = s_v + stage * kAtTile + (pw & 1) * (kAtTile / 2);
-        const int tg = lane & 7;
-#pragma unroll 1
-        for (int d0 = 2 * vb; d0 < 2 * vb + 16; d0 += 8) {  // eight dimensions: one word of each token
+        const uint32_t tile = s_v + stage * kAtVTile;
+        if (tid < kAtTok) {
+          // rows 128 .. 131: 2^10 / sigma and z' / sigma - .., each as the sum of two fp16 numbers; 0 where the token is bad
+          const float rv = v.bad == 0.0f ? __fdividef(1024.0f, v.sigma) : 0.0f, zv = v.bad == 0.0f ? v.z : 0.0f;
+          const __half rh = __float2half_rn(rv), zh = __float2half_rn(zv);
+          const __half part[4] = {rh, __float2half_rn(rv - __half2float(rh)), zh, __float2half_rn(zv - __half2float(zh))};
+          unsigned char* at = smem + (tile - base) + (tid >> 6) * kAtVAtom + 128 * 128 + (tid & 7) * 2;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t x[4];
+          for (int e = 0; e < 4; ++e)                     // row 128 + e: its number mod 8 is e
+            *reinterpret_cast<__half*>(at + e * 128 + (((((uint32_t)tid & 63) >> 3) ^ e) << 4)) = part[e];
+        }
+        if (pw < 3) {
+          const uint32_t dst = tile + (pw < 2 ? 0 : kAtVAtom);
+          __half2 sc[4], bi[4];
+          const uint4 raw = *reinterpret_cast<const uint4*>(&sh.vscale[stage][vt]);
+          const uint32_t rs[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __byte_perm(vw[2 * i].x, vw[2 * i + 1].x, half ? 0x7632u : 0x5410u);
-            const uint32_t at = dst + (d0 + 4 * half) * 128;                // d0 is a multiple of 8
-            st_shared16(at + ((tg ^ (4 * half)) << 4), at_centred_pair<0>(x[0]), at_centred_pair<0>(x[1]), at_centred_pair<0>(x[2]),
-                        at_centred_pair<0>(x[3]));
-            st_shared16(at + 128 + ((tg ^ (4 * half + 1)) << 4), at_centred_pair<1>(x[0]), at_centred_pair<1>(x[1]),
-                        at_centred_pair<1>(x[2]), at_centred_pair<1>(x[3]));
-            st_shared16(at + 256 + ((tg ^ (4 * half + 2)) << 4), at_centred_pair<2>(x[0]), at_centred_pair<2>(x[1]),
-                        at_centred_pair<2>(x[2]), at_centred_pair<2>(x[3]));
-            st_shared16(at + 384 + ((tg ^ (4 * half + 3)) << 4), at_centred_pair<3>(x[0]), at_centred_pair<3>(x[1]),
-                        at_centred_pair<3>(x[2]), at_centred_pair<3>(x[3]));
+          for (int i = 0; i < 4; ++i) {
+            sc[i] = *reinterpret_cast<const __half2*>(&rs[i]);
+            bi[i] = __hmul2(sc[i], __float2half2_rn(-23.5f));
           }
+#pragma unroll 1
+          for (int d0 = 2 * vb; d0 < 2 * vb + 16; d0 += 8) {  // eight dimensions: one word of each token
 #pragma unroll
-          for (int i = 0; i < 8; ++i) vw[i].x = vw[i].y;
+            for (int half = 0; half < 2; ++half) {
+              uint32_t x[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = __byte_perm(vw[2 * i].x, vw[2 * i + 1].x, half ? 0x7632u : 0x5410u);
+              const uint32_t at = dst + (d0 + 4 * half) * 128;              // d0 is a multiple of 8
+              st_shared16(at + ((tg ^ (4 * half)) << 4), at_centred_pair<0>(x[0], sc[0], bi[0]), at_centred_pair<0>(x[1], sc[1], bi[1]),
+                          at_centred_pair<0>(x[2], sc[2], bi[2]), at_centred_pair<0>(x[3], sc[3], bi[3]));
+              st_shared16(at + 128 + ((tg ^ (4 * half + 1)) << 4), at_centred_pair<1>(x[0], sc[0], bi[0]), at_centred_pair<1>(x[1], sc[1], bi[1]),
+                          at_centred_pair<1>(x[2], sc[2], bi[2]), at_centred_pair<1>(x[3], sc[3], bi[3]));
+              st_shared16(at + 256 + ((tg ^ (4 * half + 2)) << 4), at_centred_pair<2>(x[0], sc[0], bi[0]), at_centred_pair<2>(x[1], sc[1], bi[1]),
+                          at_centred_pair<2>(x[2], sc[2], bi[2]), at_centred_pair<2>(x[3], sc[3], bi[3]));
+              st_shared16(at + 384 + ((tg ^ (4 * half + 3)) << 4), at_centred_pair<3>(x[0], sc[0], bi[0]), at_centred_pair<3>(x[1], sc[1], bi[1]),
+                          at_centred_pair<3>(x[2], sc[2], bi[2]), at_centred_pair<3>(x[3], sc[3], bi[3]));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vw[i].x = vw[i].y;
+          }
         }
         if (j + 1 < n) load(j + 1);
         fence_proxy_async_smem();
@@ -785,17 +814,15 @@ kv_attend_tc_kernel(const KvAttendParams p) {
     const int i = warp - 16;                              // a warp per row tile: they do not wait for each other
     if (i < tiles && n > 0) {
       const uint32_t lead = elect_lane();
-      const uint32_t t_s = kTmem + i * 128, t_o = kTmem + 256 + i * 128;
-      const uint32_t q = desc_lo(s_q) + i * (kAtTile >> 4);
-      bool ok = mbar_wait(k_full, 0, abort_flag, p.status, 76);
+      const uint32_t t_s = kTmemS + i * (2 * kAtHalf), t_o = kTmemO + i * kAtVRows;
+      const uint32_t q = desc_lo(s_q) + i * (kAtQTile >> 4);
+      bool ok = mbar_wait(q_full + 8 * i, 0, abort_flag, p.status, 74) && mbar_wait(k_full, 0, abort_flag, p.status, 76);
       // scores of a half of the block in K stage `stage`
       auto scores = [&](int buf, int stage) {
-        const uint32_t b = desc_lo(s_k) + stage * (kAtTile >> 4) + buf * (64 * 128 >> 4), d = t_s + buf * 64;
+        const uint32_t b = desc_lo(s_k) + stage * (kAtKTile >> 4) + buf * (kAtHalf * 128 >> 4), d = t_s + buf * kAtHalf;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = ((ks >> 2) * (kAtTile / 2) + (ks & 3) * 32) >> 4;
-          umma_f16_ss(lead, d, q + off, b + off, ks > 0);
-        }
+        for (int ks = 0; ks < 8; ++ks)
+          umma_f16_ss(lead, d, q + (ks >> 2) * (kAtQTile / 2 >> 4) + (ks & 3) * 2, b + (ks >> 2) * (kAtKTile / 2 >> 4) + (ks & 3) * 2, ks > 0);
         umma_commit_lead(lead, s_full + 16 * i + 8 * buf);
       };
       if (ok) {
@@ -815,10 +842,12 @@ kv_attend_tc_kernel(const KvAttendParams p) {
           ok = mbar_wait(p_full + 16 * i + 8 * buf, j & 1, abort_flag, p.status, 79);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = desc_lo(s_v) + stage * (kAtTile >> 4) + buf * (kAtTile / 2 >> 4);
+          // 16 tokens at 48 buf + 16 ks: the first four steps lie in the first atom
+          const uint32_t b = desc_lo(s_v) + stage * (kAtVTile >> 4), b0 = b + buf * 6, b1 = buf ? b + (kAtVAtom >> 4) : b + 2;
           const uint32_t first = buf | j;
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_f16_ts(lead, t_o, t_s + buf * 64 + ks * 8, b + ks * 2, ks > 0 ? 1u : first);
+          umma_f16_ts(lead, t_o, t_s + buf * kAtHalf, b0, first);
+          umma_f16_ts(lead, t_o, t_s + buf * kAtHalf + 8, b1, 1u);
+          umma_f16_ts(lead, t_o, t_s + buf * kAtHalf + 16, b1 + 2, 1u);
           // scores of half h imply the products of half h - 2: the softmax is at most one phase of pv_done behind
           umma_commit_lead(lead, (more || !buf ? pv_done : o_full) + 8 * i);
           if (more) scores(buf, stage ^ 1);                 // over the weights, which the products before it have read
@@ -848,11 +877,11 @@ int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
+  QR_CUDA(cudaFuncSetAttribute(kv_attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAtSmem));
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= num_sms()) splits *= 2;
+  if (const int rc = kv_pick_splits((const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, units, visible_blocks(p, max_rows, kAtTok), &splits)) return rc;
   p.splits = splits;
   if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
-  QR_CUDA(cudaFuncSetAttribute(kv_attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAtSmem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

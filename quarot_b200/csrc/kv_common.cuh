@@ -120,7 +120,67 @@ struct KvAttendParams {
   int* status;
 };
 
+// Upper bound, where the host knows one, of the blocks of T tokens that a tile of rows sees.
+static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, int T) {
+  if (p.window <= 0) return 1ll << 40;
+  return ((int64_t)p.window + max_rows / p.group + T - 1) / T + 1 + ((int64_t)p.sinks + T - 1) / T;
+}
+
 #ifdef __CUDACC__
+// CTAs of a cluster that share the token axis of a unit of work (a tile of rows of one KV head), 1 .. 16: the number s for
+// which ceil(units / clusters of s that fit on the device) rounds of 1 / s of the work, with a share lost to each round,
+// cost least.  How many clusters fit is asked once per kernel, device and size (clusters lie within a GPC, whose SMs they
+// do not divide evenly: 15 clusters of 8 fit, 16 do not).  At most `most`: parts of the work that there are.
+int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, int64_t most, int* splits);
+
+// fp32 shares [rows][128] (addr(r): offset of row r at the lane's four columns) of the CTAs of a cluster joined into one row.
+// Up to 16 shares: lane x looks at the statistics of CTA x, then all lanes walk over the shares.
+template <int U, class Addr, class Store>
+__device__ __forceinline__ void kv_merge_rows(int splits, int first, int step, int rows, int lane, const float* s_m, const float* s_l,
+                                              Addr addr, Store store) {
+  for (int r0 = first; r0 < rows; r0 += U * step) {
+    float f[U], inv[U];
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * step;
+      const bool on = lane < splits && r < rows;
+      f[u] = on ? kv_peer_f32(kv_peer_addr(s_m + r, lane)) : -INFINITY;
+      inv[u] = on ? kv_peer_f32(kv_peer_addr(s_l + r, lane)) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float mm = f[u];
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+      // a share that saw no token of the row has l = 0 (its statistics say nothing); NaN stays NaN
+      f[u] = f[u] == -INFINITY && inv[u] == 0.0f ? 0.0f : ex2(f[u] - mm);
+      float ll = inv[u] * f[u];
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+      inv[u] = ll != 0.0f ? 1.0f / ll : 0.0f;             // a row that sees nothing gives zeros
+      acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int x = 0; x < splits; ++x) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float fx = __shfl_sync(0xffffffffu, f[u], x);
+        const int r = r0 + u * step;
+        if (r < rows && fx != 0.0f) {
+          const float4 v = kv_peer_f32x4(kv_peer_addr(addr(r), x));
+          acc[u].x = fmaf(v.x, fx, acc[u].x); acc[u].y = fmaf(v.y, fx, acc[u].y);
+          acc[u].z = fmaf(v.z, fx, acc[u].z); acc[u].w = fmaf(v.w, fx, acc[u].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      inv[u] = __shfl_sync(0xffffffffu, inv[u], 0);
+      if (r0 + u * step < rows) store(r0 + u * step, acc[u], inv[u]);
+    }
+  }
+}
+
 // The tile of query rows that a CTA works on.  Row r of a sequence is (new token r / group, head r % group of the KV head).
 struct KvTile {
   int b, row0, rows;            // sequence, first row, rows (0: nothing to do)
