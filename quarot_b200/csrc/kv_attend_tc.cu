@@ -342,46 +342,60 @@ __device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
 // and sixteen dimensions to a lane, so that the rotation needs three exchanges between lanes instead of five.  8 dimensions
 // 8 i .. 8 i + 7 lie as 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart.
 // (A call: inlined, its registers cost the loop of the softmax 5 %.)
-__device__ __noinline__ void at_load_rows(const KvAttendParams& p, int w_row0, int w_rows, int w_pos0, int64_t w_tok0, int head_kv, int row0,
-                                          int lane, unsigned char* tile, float* s_sum, int* s_pos) {
+struct AtQuery {
+  const __half* q;                                        // first new token of the sequence, first query head of the group
+  int64_t ts, hs;                                         // strides of tokens and heads
+  FastDiv group_div;
+  int group, row0, rows, pos0, hadamard;
+};
+__device__ __noinline__ void at_load_rows(const AtQuery a, int row0, int lane, unsigned char* tile, float* s_sum, int* s_pos) {
   const int sub = lane >> 3, l8 = lane & 7;
-  uint2 raw[4], ahead[4];
-  int pos = -1, pos_ahead = -1;
-  auto fetch = [&](int r) {
-    pos_ahead = -1;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ahead[e] = make_uint2(0, 0);
-    if (r < w_rows) {
-      const int row = w_row0 + r;
-      const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
-      pos_ahead = w_pos0 + tok;
-      const uint2* src = reinterpret_cast<const uint2*>(p.q + (w_tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs) + 4 * l8;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ahead[e] = src[e];
+  // all rows on their way at once, each to its place in the two atoms, in their natural order; two at a time where they are
+  // 16-byte aligned
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.ts & 7) | (a.hs & 7)) == 0;
+  const int per = wide ? 2 : 1, piece = wide ? lane & 15 : lane, bytes = wide ? 16 : 8;
+  {
+    int r = row0 + (wide ? lane >> 4 : 0);
+    int tok = fast_div(a.row0 + r, a.group_div), hh = a.row0 + r - tok * a.group;
+    const __half* src = a.q + tok * a.ts + hh * a.hs + piece * (bytes / 2);
+    const int64_t step = per * a.hs, wrap = a.ts - a.group * a.hs;
+    uint32_t dst = smem_u32(tile) + (piece * bytes >> 7) * (kAtQTile / 2) + (r & 127) * 128 + (piece * bytes & 127);
+#pragma unroll 1
+    for (; r < row0 + 32; r += per) {
+      const bool on = r < a.rows;
+      if (wide) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(on ? src : a.q), "r"(on ? 16 : 0) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(on ? src : a.q), "r"(on ? 8 : 0) : "memory");
+      if (piece == 0) s_pos[r] = on ? a.pos0 + tok : -1;
+      dst += per * 128;
+      src += step;
+      hh += per;
+      while (hh >= a.group) { hh -= a.group; ++tok; src += wrap; }
     }
-  };
-  fetch(row0 + sub);
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
 #pragma unroll 1
   for (int r = row0 + sub; r < row0 + 32; r += 4) {
+    uint2 raw[4];
+    unsigned char* mine = tile + (l8 >> 2) * (kAtQTile / 2) + (r & 127) * 128 + (l8 & 3) * 32;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) raw[e] = ahead[e];
-    pos = pos_ahead;
-    if (r + 4 < row0 + 32) fetch(r + 4);
+    for (int e = 0; e < 4; ++e) raw[e] = *reinterpret_cast<const uint2*>(mine + 8 * e);
+    __syncwarp();                                         // the row is read before it is written
     float x[16];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].y));
       x[4 * e] = lo.x; x[4 * e + 1] = lo.y; x[4 * e + 2] = hi.x; x[4 * e + 3] = hi.y;
     }
-    if (p.hadamard_q) {
+    if (a.hadamard) {
 #pragma unroll
       for (int h = 1; h < 16; h <<= 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if ((e & h) == 0) {
-            const float a = x[e], b = x[e + h];
-            x[e] = a + b;
-            x[e + h] = a - b;
+            const float u = x[e], v = x[e + h];
+            x[e] = u + v;
+            x[e + h] = u - v;
           }
 #pragma unroll 1
       for (int s = 1; s < 8; s <<= 1) {
@@ -392,9 +406,10 @@ __device__ __noinline__ void at_load_rows(const KvAttendParams& p, int w_row0, i
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
     }
-    float sum = 0.0f;
+    float part[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sum += x[e];
+    for (int e = 0; e < 4; ++e) part[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
+    float sum = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
     for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     const int rr = r & 127;
@@ -409,7 +424,7 @@ __device__ __noinline__ void at_load_rows(const KvAttendParams& p, int w_row0, i
       const int ch = 2 * l8 + v;
       *reinterpret_cast<uint4*>(tile + (ch >> 3) * (kAtQTile / 2) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    if (l8 == 0) { s_sum[r] = sum; s_pos[r] = pos; }
+    if (l8 == 0) s_sum[r] = sum;
   }
 }
 
@@ -470,7 +485,9 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
     const int row0 = i * 128 + (warp & 3) * 32;                           // the lane's rows: row0 + g + 8 x, x = 0 .. 3
     const int* pos = &sh.pos[row0 + g];
     if (i < tiles) {
-      at_load_rows(p, w.row0, w.rows, w.pos0, w.tok0, head_kv, row0, lane, smem + i * kAtQTile, sh.qsum, sh.pos);
+      const AtQuery a = {p.q + w.tok0 * p.q_ts + (int64_t)(head_kv * p.group) * p.q_hs, p.q_ts, p.q_hs, p.group_div, p.group, w.row0, w.rows,
+                         w.pos0, p.hadamard_q};
+      at_load_rows(a, row0, lane, smem + i * kAtQTile, sh.qsum, sh.pos);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full + 8 * i);
@@ -617,7 +634,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
     if (p.splits > 1) {
       kv_cluster_barrier();
       // the CTAs of the cluster deal out the rows
-      kv_merge_rows<2>(p.splits, (int)crank + p.splits * warp, p.splits * 8, w.rows, lane, sh.m, sh.l,
+      kv_merge_rows<4>(p.splits, (int)crank + p.splits * warp, p.splits * 8, w.rows, lane, sh.m, sh.l,
                        [&](int r) { return smem + at_part_off(r, lane); },
                        [&](int r, float4 v, float inv) {
                          const __half2 h0 = __floats2half2_rn(v.x * inv, v.y * inv), h1 = __floats2half2_rn(v.z * inv, v.w * inv);

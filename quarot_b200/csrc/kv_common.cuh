@@ -133,20 +133,23 @@ static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, 
 // do not divide evenly: 15 clusters of 8 fit, 16 do not).  At most `most`: parts of the work that there are.
 int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, int64_t most, int* splits);
 
-// fp32 shares [rows][128] (addr(r): offset of row r at the lane's four columns) of the CTAs of a cluster joined into one row.
-// Up to 16 shares: lane x looks at the statistics of CTA x, then all lanes walk over the shares.
+// fp32 shares [rows][128] (addr(r): the lane's four columns of row r) of the CTAs of a cluster joined into one row, U rows
+// at a time.  Lane x looks at the statistics of CTA x; the first two shares are asked for before that.
 template <int U, class Addr, class Store>
 __device__ __forceinline__ void kv_merge_rows(int splits, int first, int step, int rows, int lane, const float* s_m, const float* s_l,
                                               Addr addr, Store store) {
+#pragma unroll 1
   for (int r0 = first; r0 < rows; r0 += U * step) {
     float f[U], inv[U];
-    float4 acc[U];
+    float4 acc[U], v[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * step;
-      const bool on = lane < splits && r < rows;
-      f[u] = on ? kv_peer_f32(kv_peer_addr(s_m + r, lane)) : -INFINITY;
-      inv[u] = on ? kv_peer_f32(kv_peer_addr(s_l + r, lane)) : 0.0f;
+      const int r = r0 + u * step < rows ? r0 + u * step : r0;
+      f[u] = lane < splits ? kv_peer_f32(kv_peer_addr(s_m + r, lane)) : -INFINITY;
+      inv[u] = lane < splits ? kv_peer_f32(kv_peer_addr(s_l + r, lane)) : 0.0f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) v[u][x] = kv_peer_f32x4(kv_peer_addr(addr(r), x));
+      acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -159,18 +162,26 @@ __device__ __forceinline__ void kv_merge_rows(int splits, int first, int step, i
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
       inv[u] = ll != 0.0f ? 1.0f / ll : 0.0f;             // a row that sees nothing gives zeros
-      acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    for (int x = 0; x < splits; ++x) {
+#pragma unroll 1
+    for (int x0 = 0; x0 < splits; x0 += 2) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float fx = __shfl_sync(0xffffffffu, f[u], x);
-        const int r = r0 + u * step;
-        if (r < rows && fx != 0.0f) {
-          const float4 v = kv_peer_f32x4(kv_peer_addr(addr(r), x));
-          acc[u].x = fmaf(v.x, fx, acc[u].x); acc[u].y = fmaf(v.y, fx, acc[u].y);
-          acc[u].z = fmaf(v.z, fx, acc[u].z); acc[u].w = fmaf(v.w, fx, acc[u].w);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float fx = __shfl_sync(0xffffffffu, f[u], x0 + x);        // 0 beyond the last share
+          if (fx != 0.0f) {
+            acc[u].x = fmaf(v[u][x].x, fx, acc[u].x); acc[u].y = fmaf(v[u][x].y, fx, acc[u].y);
+            acc[u].z = fmaf(v[u][x].z, fx, acc[u].z); acc[u].w = fmaf(v[u][x].w, fx, acc[u].w);
+          }
         }
+      }
+      if (x0 + 2 < splits) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            v[u][x] = kv_peer_f32x4(kv_peer_addr(addr(r0 + u * step < rows ? r0 + u * step : r0), x0 + 2 + x < splits ? x0 + 2 + x : 0));
       }
     }
 #pragma unroll
