@@ -52,9 +52,15 @@ struct RwShared {
   __half q[8 * NT][kHeadDim];                           // rows in fragment order
   float qsum[8 * NT];
   int pos[8 * NT];                                      // position of the row, -1: not a row
+  union {
+    struct {                                            // of a warp's block, per token:
+      float4 par4[kRwWarps][kRwTok];                    // s, -(z + 16 s) (both times log2(e) / sqrt(d)), log2 s', 1 / s'
+      float par1[kRwWarps][kRwTok];                     // z' / s' - 7.5
+    };
+    float part_o[8 * NT][kHeadDim];                     // after the loop: the CTA's share
+  };
   float m[kRwWarps][8 * NT], l[kRwWarps][8 * NT];
   float part_m[8 * NT], part_l[8 * NT];
-  float part_o[8 * NT][kHeadDim];
 };
 
 __device__ __forceinline__ void rw_cp16(uint32_t dst, const void* src, int bytes) {
@@ -127,23 +133,33 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   const uint32_t last_page = (uint32_t)(p.num_pages - 1);
   const uint32_t my_ring = smem_u32(ring) + warp * (kStages * kRwStageBytes);
 
-  // lane copies chunk c of the rows g + 8 i of a block
+  // Lane copies chunk c of the rows g + 8 i of a block.  Where pages hold a multiple of 16 tokens the rows i = 0, 1 and
+  // 2, 3 lie in one page each, eight slots apart.
+  const bool by16 = (p.page_size & 15) == 0;
   auto page_ids = [&](int bi, int (&id)[4]) {
     const int t0 = kv_block_index(blk, bi) * kRwTok + g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = t0 + 8 * i < tokens ? __ldg(pages + fast_div(t0 + 8 * i, p.page_div)) : 0;
+    for (int i = 0; i < 4; ++i) {
+      if ((i & 1) && by16) continue;
+      id[i] = t0 + 8 * i < tokens ? __ldg(pages + fast_div(t0 + 8 * i, p.page_div)) : 0;
+    }
   };
   auto issue = [&](int bi, int stage, const int (&id)[4]) {
     const int t0 = kv_block_index(blk, bi) * kRwTok + g;
     const uint32_t st = my_ring + stage * kRwStageBytes + g * 64 + ((c ^ rw_swz(g)) << 4);
     const uint32_t sp = my_ring + stage * kRwStageBytes + kRwTok * 128 + (c & 1) * (kRwTok * 4) + g * 4;
+    uint32_t row = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = t0 + 8 * i;
       const bool ok = t < tokens;
-      const int slot = t - fast_div(t, p.page_div) * p.page_size;
-      // an index outside the pool reads its last page
-      const uint32_t row = min((uint32_t)id[i], last_page) * page_rows + row_k + (ok ? slot : 0);
+      if ((i & 1) && by16) {
+        row += ok ? 8 : 0;
+      } else {
+        const int slot = t - fast_div(t, p.page_div) * p.page_size;
+        // an index outside the pool reads its last page
+        row = min((uint32_t)id[i], last_page) * page_rows + row_k + (ok ? slot : 0);
+      }
       const uint8_t* src = p.data + (uint64_t)row * 64 + 16 * c;
       rw_cp16(st + 512 * i, src, ok ? 16 : 0);
       rw_cp16(st + 512 * i + kRwTok * 64, src + (uint64_t)v_rows * 64, ok ? 16 : 0);
@@ -189,7 +205,6 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   // query fragments: in registers for eight or sixteen rows, from shared memory where they are used for more
   uint32_t qf[NT <= 2 ? NT : 1][16];
   float qs[NT][2];
-  int ps[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (NT <= 2) {
@@ -201,7 +216,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       }
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; ps[n][k] = sh.pos[8 * n + 2 * c + k]; }
+    for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; }
   }
 
   float o[NT][8][4], ws[NT][4], l[NT][2], y[NT][2], m[NT][2];
@@ -234,6 +249,21 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     const unsigned char* st = ring + warp * (kStages * kRwStageBytes) + stage * kRwStageBytes;
     const int t0 = kv_block_index(blk, bi) * kRwTok;
     const bool edge = t0 + kRwTok - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kRwTok - 1 >= p.sinks);
+    {
+      // the numbers of token `lane`
+      const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 128 + lane * 4));
+      float2 vp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 132 + lane * 4));
+      // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
+      if (vp.x < 9.31322575e-10f) vp.x = 9.31322575e-10f;
+      // x - x: 0, or NaN where it is not finite.  Then the weight of the token is NaN in the rows that see it, and its other
+      // numbers are 0, so that a weight 0 leaves the sums of the rows that do not see it alone.
+      const float bad = ((kp.x - kp.x) + (kp.y - kp.y)) + ((vp.x - vp.x) + (vp.y - vp.y));
+      const bool fine = bad == 0.0f;
+      const float rv = __fdividef(1.0f, vp.x), ks = kp.x * sm_scale;
+      sh.par4[warp][lane] = make_float4(ks, -fmaf(16.0f, ks, kp.y * sm_scale), __log2f(vp.x) + bad, fine ? rv : 0.0f);
+      sh.par1[warp][lane] = fine ? fmaf(vp.y, rv, -7.5f) : 0.0f;
+    }
+    __syncwarp();
 #pragma unroll 1
     for (int a0 = 0; a0 < 2; a0 += TA) {
     float s[TA][NT][4];
@@ -263,36 +293,43 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       }
     }
     float rv[TA][2], zv[TA][2];                         // 1 / s', z' / s' - 7.5 of the lane's tokens
-    float top = -INFINITY;                              // largest exponent relative to M
+    float e[TA][NT][4];                                 // exponents relative to M
+    float top = -INFINITY;
 #pragma unroll
     for (int a = 0; a < TA; ++a)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = 16 * (a0 + a) + 8 * h + tau;
-        const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 128 + r * 4));
-        float2 vp = __half22float2(*reinterpret_cast<const __half2*>(st + kRwTok * 132 + r * 4));
-        // scales of a cache are positive; below 2^-30 the codes of a token cannot move an fp16 result
-        if (vp.x < 9.31322575e-10f) vp.x = 9.31322575e-10f;
-        rv[a][h] = __fdividef(1.0f, vp.x);
-        zv[a][h] = fmaf(vp.y, rv[a][h], -7.5f);
-        // x - x: 0, or NaN where key parameters are not finite (the score of such a token may not end up at -infinity)
-        const float lv = __log2f(vp.x) + ((kp.x - kp.x) + (kp.y - kp.y));
-        const float ks = kp.x * sm_scale, kz = fmaf(16.0f, ks, kp.y * sm_scale);
-        const int t = t0 + r;
+        const float4 pr = sh.par4[warp][r];
+        rv[a][h] = pr.w;
+        zv[a][h] = sh.par1[warp][r];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float v = fmaf(ks, s[a][n][2 * h + k], fmaf(-kz, qs[n][k], lv));
-            if (edge) {
-              const bool see = t <= ps[n][k] && (p.window <= 0 || t > ps[n][k] - p.window || t < p.sinks);
-              v = see ? v : -INFINITY;
-            }
-            s[a][n][2 * h + k] = v;
-            top = fmaxf(top, v - m[n][k]);
+            s[a][n][2 * h + k] = fmaf(pr.x, s[a][n][2 * h + k], fmaf(pr.y, qs[n][k], pr.z));
+            e[a][n][2 * h + k] = s[a][n][2 * h + k] - m[n][k];          // +infinity before the row has seen a token
+            top = fmaxf(top, e[a][n][2 * h + k]);
           }
       }
-    if (__any_sync(0xffffffffu, top > kRwTop)) {
+    if (__builtin_expect(edge, 0)) {
+      top = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < TA; ++a)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t = t0 + 16 * (a0 + a) + 8 * h + tau;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int pos = sh.pos[8 * n + 2 * c + k];
+              if (t > pos || (p.window > 0 && t <= pos - p.window && t >= p.sinks)) s[a][n][2 * h + k] = e[a][n][2 * h + k] = -INFINITY;
+              top = fmaxf(top, e[a][n][2 * h + k]);
+            }
+        }
+    }
+    if (__builtin_expect(__any_sync(0xffffffffu, top > kRwTop), 0)) {
       // a weight would pass 2^15, or a row sees its first token: M moves, and what has been summed up is multiplied through
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -309,32 +346,30 @@ kv_attend_rows_kernel(const KvAttendParams p) {
           m[n][k] = move ? to : m[n][k];
           l[n][k] *= f[k];
           y[n][k] *= f[k];
+#pragma unroll
+          for (int a = 0; a < TA; ++a)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              e[a][n][2 * h + k] = s[a][n][2 * h + k] == -INFINITY ? -INFINITY : s[a][n][2 * h + k] - m[n][k];
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][t][e] *= f[e & 1];
+          for (int x = 0; x < 4; ++x) o[n][t][x] *= f[x & 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ws[n][e] *= f[e & 1];
+        for (int x = 0; x < 4; ++x) ws[n][x] *= f[x & 1];
       }
     }
     uint32_t pb[TA][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
 #pragma unroll
       for (int a = 0; a < TA; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float w0 = ex2(s[a][n][2 * h] - m0), w1 = ex2(s[a][n][2 * h + 1] - m1);
-          if (edge) {
-            // a hidden token leaves the sums alone whatever its parameters hold
-            if (w0 != 0.0f) { l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]); }
-            if (w1 != 0.0f) { l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]); }
-          } else {
-            l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]);
-            l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]);
-          }
+          const float w0 = ex2(e[a][n][2 * h]), w1 = ex2(e[a][n][2 * h + 1]);
+          l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]);
+          l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]);
           const __half2 wh = __floats2half2_rn(w0, w1);
           pb[a][n][h] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&wh));
         }
