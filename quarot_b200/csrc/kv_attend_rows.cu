@@ -3,16 +3,18 @@
 //
 // Mathematics.  With key codes c, scale s and zero z per (token, head), the score of row r and token t is
 //   s_t <q_r, c_t> - z_t sum(q_r),   and value = s' c' - z'  (s', z' the value parameters).
-// The tensor cores see only small whole numbers: a code is put into the mantissa of 16.0 (fp16 0x4C00 | c << 6 is exactly
-// 16 + c), two logical instructions per pair of codes and no arithmetic, and the 16 is taken out of the sums in fp32.
+// The tensor cores see the codes as they stand: four bits masked out of a word are the subnormal fp16 number c 2^-24 (bits
+// 0 .. 3) or c 2^-20 (bits 4 .. 7), exact, so that a pair of codes takes one logical instruction and four pairs one shift.
+// The powers of two are taken back in the query (brought to 2^10 .. 2^15 by powers of two per row, in which no bit is lost)
+// and in the output, where the two kinds lie in different registers.
 // Weights: w_t = exp2(score_t + log2 s'_t - M) so that the value scale is inside the weight.  M does not follow the
 // maximum: it is set 1 below the first one and moves, in whole steps, only where a weight would pass 2^15, so that sums
 // are rarely multiplied through and no maximum is looked for across lanes.  Rounding w to fp16 (the B operand of the second
 // product) is a relative error of at most 2^-11 down to 2^-14 of the largest; the sums
 //   l = sum w / s'_t  (the softmax denominator)  and  y = sum w (z'_t / s'_t - 7.5)
 // are of the unrounded w in fp32, and the centre 7.5 of the codes is taken out with the ROUNDED weights (one more MMA
-// row of ones), so that a rounding error of w meets c' - 7.5 and not 16 + c':
-//   o = (sum w~ (16 + c') - 23.5 sum w~ - y) / l.
+// row of ones), so that a rounding error of w meets c' - 7.5:
+//   o = (sum w~ c' - 7.5 sum w~ - y) / l.
 //
 // Mapping.  A warp takes blocks of 32 tokens.  Scores: S^T = K Q^T with mma.m16n8k16, 16 tokens as M, 8 rows as N; lane
 // (g, c) = (lane / 4, lane % 4) reads 16 bytes of each of its token rows (32 codes), and since the order of the 128
@@ -27,39 +29,41 @@
 #include "kv_common.cuh"
 
 #include <math.h>
-#include <map>
-#include <mutex>
-#include <utility>
+#include <atomic>
 
 namespace qr {
 
-constexpr int kRwWarps = 8;
 constexpr int kRwTok = 32;                              // tokens per block
 constexpr int kRwStageBytes = kRwTok * (64 + 64 + 4 + 4);
 constexpr int kRwORow = kHeadDim + 4;                   // floats per row of the merge buffers
+constexpr uint32_t kRwLow = 0x000F000Fu, kRwHigh = 0x00F000F0u;   // codes as they stand in subnormal fp16: c 2^-24 and c 2^-20
 constexpr float kRwTop = 15.0f;                         // weights are at most 2^15
 
-// Eight rows: two CTAs per SM with three stages per warp; more rows: one CTA (registers) with four.
+// Warps work on two 16-token tiles at once (TA), which hides more latency than further warps would: eight rows take 128
+// registers a thread, four CTAs of four warps per SM; sixteen rows 232, two CTAs.  CTAs of four warps balance better than
+// larger ones, and smaller ones have too much beside the loop.
 template <int NT>
 struct RwConfig {
-  static constexpr int kStages = NT == 1 ? 3 : 4;
-  static constexpr int kCtas = NT == 1 ? 2 : 1;
-  static constexpr int kRing = kRwWarps * kStages * kRwStageBytes;
+  static constexpr int kWarps = 4;
+  static constexpr int kStages = NT == 1 ? 2 : 3;
+  static constexpr int kCtas = NT == 1 ? 4 : 2;                  // per SM
+  static constexpr int kRing = kWarps * kStages * kRwStageBytes;
 };
 
 template <int NT>
 struct RwShared {
+  static constexpr int kWarps = RwConfig<NT>::kWarps;
   __half q[8 * NT][kHeadDim];                           // rows in fragment order
-  float qsum[8 * NT];
+  float qsum[8 * NT], qmul[8 * NT];                     // sum of the row's elements; the power of two that its products lack
   int pos[8 * NT];                                      // position of the row, -1: not a row
   union {
     struct {                                            // of a warp's block, per token:
-      float4 par4[kRwWarps][kRwTok];                    // s, -(z + 16 s) (both times log2(e) / sqrt(d)), log2 s', 1 / s'
-      float par1[kRwWarps][kRwTok];                     // z' / s' - 7.5
+      float4 par4[kWarps][kRwTok];                    // s, -(z + 16 s) (both times log2(e) / sqrt(d)), log2 s', 1 / s'
+      float par1[kWarps][kRwTok];                     // z' / s' - 7.5
     };
     float part_o[8 * NT][kHeadDim];                     // after the loop: the CTA's share
   };
-  float m[kRwWarps][8 * NT], l[kRwWarps][8 * NT];
+  float m[kWarps][8 * NT], l[kWarps][8 * NT];
   float part_m[8 * NT], part_l[8 * NT];
 };
 
@@ -101,11 +105,12 @@ __device__ __forceinline__ void rw_store_row(const KvAttendParams& p, const KvTi
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * kRwWarps, RwConfig<NT>::kCtas)
+__global__ void __launch_bounds__(32 * RwConfig<NT>::kWarps, RwConfig<NT>::kCtas)
 kv_attend_rows_kernel(const KvAttendParams p) {
   constexpr int R = 8 * NT;
   constexpr int kStages = RwConfig<NT>::kStages;
-  constexpr int TA = NT == 1 ? 2 : 1;                   // 16-token tiles worked on together: two hide the MMA chains of one row group
+  constexpr int kWarps = RwConfig<NT>::kWarps;
+  constexpr int TA = 2;                                 // 16-token tiles of a block worked on together
   extern __shared__ __align__(128) unsigned char s_dyn[];
   unsigned char* ring = s_dyn;
   RwShared<NT>& sh = *reinterpret_cast<RwShared<NT>*>(s_dyn + RwConfig<NT>::kRing);
@@ -124,12 +129,13 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   const int per = (blk.count + p.splits - 1) / p.splits;
   const int begin = (int)crank * per + warp, end = min((int)(crank + 1) * per, blk.count);
 
-  const int32_t* pages = p.indices + p.indptr[w.b];
+  const int32_t* pages = p.indices + w.first;
   const int tokens = min(p_max + 1, w.seq_len);         // tokens from here on are not read
   // a pool has fewer than 2^32 rows of 64 bytes
   const uint32_t page_rows = (uint32_t)p.layers * 2 * p.kv_heads * p.page_size;
   const uint32_t row_k = ((uint32_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
   const uint32_t v_rows = (uint32_t)p.kv_heads * p.page_size;
+  const uint64_t v_bytes = (uint64_t)v_rows * 64;
   const uint32_t last_page = (uint32_t)(p.num_pages - 1);
   const uint32_t my_ring = smem_u32(ring) + warp * (kStages * kRwStageBytes);
 
@@ -148,75 +154,90 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     const int t0 = kv_block_index(blk, bi) * kRwTok + g;
     const uint32_t st = my_ring + stage * kRwStageBytes + g * 64 + ((c ^ rw_swz(g)) << 4);
     const uint32_t sp = my_ring + stage * kRwStageBytes + kRwTok * 128 + (c & 1) * (kRwTok * 4) + g * 4;
-    uint32_t row = 0;
+    const uint8_t* src = nullptr;
+    const __half2* num = nullptr;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = t0 + 8 * i;
       const bool ok = t < tokens;
       if ((i & 1) && by16) {
-        row += ok ? 8 : 0;
+        src += 8 * 64;
+        num += 8;
       } else {
-        const int slot = t - fast_div(t, p.page_div) * p.page_size;
         // an index outside the pool reads its last page
-        row = min((uint32_t)id[i], last_page) * page_rows + row_k + (ok ? slot : 0);
+        const uint32_t row = min((uint32_t)id[i], last_page) * page_rows + row_k + (t - fast_div(t, p.page_div) * p.page_size);
+        src = p.data + (uint64_t)row * 64 + 16 * c;
+        num = p.param + (row + (c ? v_rows : 0u));
       }
-      const uint8_t* src = p.data + (uint64_t)row * 64 + 16 * c;
       rw_cp16(st + 512 * i, src, ok ? 16 : 0);
-      rw_cp16(st + 512 * i + kRwTok * 64, src + (uint64_t)v_rows * 64, ok ? 16 : 0);
-      if (c < 2) rw_cp4(sp + 32 * i, p.param + (row + (c ? v_rows : 0u)), ok ? 4 : 0);
+      rw_cp16(st + 512 * i + kRwTok * 64, src + v_bytes, ok ? 16 : 0);
+      if (c < 2) rw_cp4(sp + 32 * i, num, ok ? 4 : 0);
     }
   };
-  int id[4];
+  // the query rows are on their way while the first pages are looked up
+  uint2 raw[R / kWarps];
+  int pos[R / kWarps];
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    const int bi = begin + s * kRwWarps;
-    if (bi < end) { page_ids(bi, id); issue(bi, s, id); }
-    rw_commit();
-  }
-  if (begin + (kStages - 1) * kRwWarps < end) page_ids(begin + (kStages - 1) * kRwWarps, id);
-
-  for (int r = warp; r < R; r += kRwWarps) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int pos = -1;
+  for (int i = 0; i < R / kWarps; ++i) {
+    const int r = warp + i * kWarps;
+    raw[i] = make_uint2(0, 0);
+    pos[i] = -1;
     if (r < w.rows) {
       const int row = w.row0 + r;
       const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
-      pos = w.pos0 + tok;
-      load4_f16(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane, x);
-      if (p.hadamard_q) {
-        fwht128_warp(x, lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
-      }
+      pos[i] = w.pos0 + tok;
+      raw[i] = *reinterpret_cast<const uint2*>(p.q + (w.tok0 + tok) * p.q_ts + (int64_t)(head_kv * p.group + hh) * p.q_hs + 4 * lane);
     }
-    float sum = x[0] + x[1] + x[2] + x[3];
+  }
+  int id[4];
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  for (int s = 0; s < kStages - 1; ++s) {
+    const int bi = begin + s * kWarps;
+    if (bi < end) { page_ids(bi, id); issue(bi, s, id); }
+    rw_commit();
+  }
+  if (begin + (kStages - 1) * kWarps < end) page_ids(begin + (kStages - 1) * kWarps, id);
+
+#pragma unroll
+  for (int i = 0; i < R / kWarps; ++i) {
+    const int r = warp + i * kWarps;
+    float x[4];
+    half4_to_f32(raw[i], x);
+    if (p.hadamard_q) {
+      fwht128_warp(x, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
+    }
+    float sum = x[0] + x[1] + x[2] + x[3], big = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+    }
+    // a power of two that brings the largest element to 2^10 .. 2^11 (fp16 elements: no bit is lost in [2^-24, 2^11])
+    const int eb = big > 0.0f && big <= 65504.0f ? (int)(__float_as_uint(big) >> 23) - 127 : 10;
+    const float down = __uint_as_float((uint32_t)(127 + 10 - eb) << 23);
     // dimension d = 32 cc + 8 wi + e sits in register (2 wi + e % 4 / 2, e % 2), half e / 4, of lane column cc
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const int d = 4 * lane + e4, e = d & 7;
-      sh.q[r][(d >> 5) * 32 + ((d >> 3) & 3) * 8 + (e & 3) * 2 + (e >> 2)] = __float2half_rn(x[e4]);
+      sh.q[r][(d >> 5) * 32 + ((d >> 3) & 3) * 8 + (e & 3) * 2 + (e >> 2)] = __float2half_rn(x[e4] * (e & 1 ? down : down * 16.0f));
     }
-    if (lane == 0) { sh.qsum[r] = sum; sh.pos[r] = pos; }
+    if (lane == 0) { sh.qsum[r] = sum; sh.qmul[r] = __uint_as_float((uint32_t)(127 + 10 + eb) << 23); sh.pos[r] = pos[i]; }
   }
   __syncthreads();
 
-  // query fragments: in registers for eight or sixteen rows, from shared memory where they are used for more
-  uint32_t qf[NT <= 2 ? NT : 1][16];
-  float qs[NT][2];
+  uint32_t qf[NT][16];                                  // query fragments
+  float qs[NT][2], qm[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (NT <= 2) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 u = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * i]);
-        qf[NT <= 2 ? n : 0][4 * i] = u.x; qf[NT <= 2 ? n : 0][4 * i + 1] = u.y;
-        qf[NT <= 2 ? n : 0][4 * i + 2] = u.z; qf[NT <= 2 ? n : 0][4 * i + 3] = u.w;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * i]);
+      qf[n][4 * i] = u.x; qf[n][4 * i + 1] = u.y; qf[n][4 * i + 2] = u.z; qf[n][4 * i + 3] = u.w;
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; }
+    for (int k = 0; k < 2; ++k) { qs[n][k] = sh.qsum[8 * n + 2 * c + k]; qm[n][k] = sh.qmul[8 * n + 2 * c + k]; }
   }
 
   float o[NT][8][4], ws[NT][4], l[NT][2], y[NT][2], m[NT][2];
@@ -237,12 +258,12 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   // slots of a 16-token tile -> tokens, see rw_token_even: rows g, g + 8 of a K fragment; 2 c, 2 c + 1 (+ 8) of a V fragment
   const int tau = (g & 1) ? rw_token_odd(g >> 1) : rw_token_even(g >> 1), ta = rw_token_even(c), tb = rw_token_odd(c);
 #pragma unroll 1
-  for (int bi = begin; bi < end; bi += kRwWarps) {
+  for (int bi = begin; bi < end; bi += kWarps) {
     {
-      const int ahead = bi + (kStages - 1) * kRwWarps;
+      const int ahead = bi + (kStages - 1) * kWarps;
       if (ahead < end) issue(ahead, stage == 0 ? kStages - 1 : stage - 1, id);
       rw_commit();
-      if (ahead + kRwWarps < end) page_ids(ahead + kRwWarps, id);
+      if (ahead + kWarps < end) page_ids(ahead + kWarps, id);
     }
     rw_wait<kStages - 1>();
     __syncwarp();
@@ -260,17 +281,15 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       const float bad = ((kp.x - kp.x) + (kp.y - kp.y)) + ((vp.x - vp.x) + (vp.y - vp.y));
       const bool fine = bad == 0.0f;
       const float rv = __fdividef(1.0f, vp.x), ks = kp.x * sm_scale;
-      sh.par4[warp][lane] = make_float4(ks, -fmaf(16.0f, ks, kp.y * sm_scale), __log2f(vp.x) + bad, fine ? rv : 0.0f);
+      sh.par4[warp][lane] = make_float4(ks, -kp.y * sm_scale, __log2f(vp.x) + bad, fine ? rv : 0.0f);
       sh.par1[warp][lane] = fine ? fmaf(vp.y, rv, -7.5f) : 0.0f;
     }
     __syncwarp();
-#pragma unroll 1
-    for (int a0 = 0; a0 < 2; a0 += TA) {
     float s[TA][NT][4];
 #pragma unroll
     for (int a = 0; a < TA; ++a) {
       // fragment rows g and g + 8: tokens tau and 8 + tau of the tile
-      const unsigned char* sk = st + (16 * (a0 + a) + tau) * 64 + ((c ^ rw_swz(tau)) << 4);
+      const unsigned char* sk = st + (16 * a + tau) * 64 + ((c ^ rw_swz(tau)) << 4);
       const uint4 x = *reinterpret_cast<const uint4*>(sk);
       const uint4 z = *reinterpret_cast<const uint4*>(sk + 8 * 64);
 #pragma unroll
@@ -280,15 +299,13 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
       for (int wi = 0; wi < 4; ++wi) {
-        const uint32_t f0 = code_pair<0>(xw[wi]), f1 = code_pair<0>(zw[wi]), f2 = code_pair<1>(xw[wi]), f3 = code_pair<1>(zw[wi]);
-        const uint32_t h0 = code_pair<2>(xw[wi]), h1 = code_pair<2>(zw[wi]), h2 = code_pair<3>(xw[wi]), h3 = code_pair<3>(zw[wi]);
+        const uint32_t xh = xw[wi] >> 8, zh = zw[wi] >> 8;
+        const uint32_t f0 = xw[wi] & kRwLow, f1 = zw[wi] & kRwLow, f2 = xw[wi] & kRwHigh, f3 = zw[wi] & kRwHigh;
+        const uint32_t h0 = xh & kRwLow, h1 = zh & kRwLow, h2 = xh & kRwHigh, h3 = zh & kRwHigh;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint4 q4;
-          if (NT <= 2) q4 = make_uint4(qf[NT <= 2 ? n : 0][4 * wi], qf[NT <= 2 ? n : 0][4 * wi + 1], qf[NT <= 2 ? n : 0][4 * wi + 2], qf[NT <= 2 ? n : 0][4 * wi + 3]);
-          else q4 = *reinterpret_cast<const uint4*>(&sh.q[8 * n + g][32 * c + 8 * wi]);
-          mma_f16(s[a][n], f0, f1, f2, f3, q4.x, q4.y);
-          mma_f16(s[a][n], h0, h1, h2, h3, q4.z, q4.w);
+          mma_f16(s[a][n], f0, f1, f2, f3, qf[n][4 * wi], qf[n][4 * wi + 1]);
+          mma_f16(s[a][n], h0, h1, h2, h3, qf[n][4 * wi + 2], qf[n][4 * wi + 3]);
         }
       }
     }
@@ -299,7 +316,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     for (int a = 0; a < TA; ++a)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = 16 * (a0 + a) + 8 * h + tau;
+        const int r = 16 * a + 8 * h + tau;
         const float4 pr = sh.par4[warp][r];
         rv[a][h] = pr.w;
         zv[a][h] = sh.par1[warp][r];
@@ -307,7 +324,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            s[a][n][2 * h + k] = fmaf(pr.x, s[a][n][2 * h + k], fmaf(pr.y, qs[n][k], pr.z));
+            s[a][n][2 * h + k] = fmaf(pr.x * qm[n][k], s[a][n][2 * h + k], fmaf(pr.y, qs[n][k], pr.z));
             e[a][n][2 * h + k] = s[a][n][2 * h + k] - m[n][k];          // +infinity before the row has seen a token
             top = fmaxf(top, e[a][n][2 * h + k]);
           }
@@ -318,7 +335,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       for (int a = 0; a < TA; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int t = t0 + 16 * (a0 + a) + 8 * h + tau;
+          const int t = t0 + 16 * a + 8 * h + tau;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -337,7 +354,8 @@ kv_attend_rows_kernel(const KvAttendParams p) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float up = fmaxf(s[0][n][k], s[0][n][2 + k]);
-          if (TA == 2) up = fmaxf(up, fmaxf(s[TA - 1][n][k], s[TA - 1][n][2 + k]));
+#pragma unroll
+          for (int a = 1; a < TA; ++a) up = fmaxf(up, fmaxf(s[a][n][k], s[a][n][2 + k]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, x));
           const bool move = up - m[n][k] > kRwTop;
@@ -377,7 +395,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
 #pragma unroll
     for (int a = 0; a < TA; ++a) {
       // slots 2c, 2c + 1, 2c + 8, 2c + 9: tokens of the tile
-      const unsigned char* sv = st + kRwTok * 64 + (16 * (a0 + a)) * 64 + (g & 1) * 8;
+      const unsigned char* sv = st + kRwTok * 64 + (16 * a) * 64 + (g & 1) * 8;
       const unsigned char* sa = sv + ta * 64 + (((g >> 1) ^ rw_swz(ta)) << 4);
       const unsigned char* sb = sv + tb * 64 + (((g >> 1) ^ rw_swz(tb)) << 4);
       const uint2 va = *reinterpret_cast<const uint2*>(sa), vb = *reinterpret_cast<const uint2*>(sb);
@@ -387,8 +405,9 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         const uint32_t sel = (q4 & 1) ? 0x7632u : 0x5410u;
         const uint32_t ab = __byte_perm(q4 < 2 ? va.x : va.y, q4 < 2 ? vb.x : vb.y, sel);
         const uint32_t cd = __byte_perm(q4 < 2 ? vc.x : vc.y, q4 < 2 ? vd.x : vd.y, sel);
-        const uint32_t f0 = code_pair<0>(ab), f1 = code_pair<1>(ab), f2 = code_pair<0>(cd), f3 = code_pair<1>(cd);
-        const uint32_t h0 = code_pair<2>(ab), h1 = code_pair<3>(ab), h2 = code_pair<2>(cd), h3 = code_pair<3>(cd);
+        const uint32_t ah = ab >> 8, ch = cd >> 8;
+        const uint32_t f0 = ab & kRwLow, f1 = ab & kRwHigh, f2 = cd & kRwLow, f3 = cd & kRwHigh;
+        const uint32_t h0 = ah & kRwLow, h1 = ah & kRwHigh, h2 = ch & kRwLow, h3 = ch & kRwHigh;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma_f16(o[n][2 * q4], f0, f1, f2, f3, pb[a][n][0], pb[a][n][1]);
@@ -397,7 +416,6 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16(ws[n], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[a][n][0], pb[a][n][1]);
-    }
     }
     __syncwarp();                                       // the stage is filled again in the next round
     stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -416,23 +434,23 @@ kv_attend_rows_kernel(const KvAttendParams p) {
         y[n][k] += __shfl_xor_sync(0xffffffffu, y[n][k], x);
       }
       const int r = 8 * n + 2 * c + k;
-      const float off = fmaf(23.5f, ws[n][k], y[n][k]);
+      const float off = fmaf(7.5f, ws[n][k], y[n][k]);
       float* dst = merge + ((size_t)warp * R + r) * kRwORow + 16 * g;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        *reinterpret_cast<float4*>(dst + 4 * t) = make_float4(o[n][2 * t][k] - off, o[n][2 * t][2 + k] - off,
-                                                              o[n][2 * t + 1][k] - off, o[n][2 * t + 1][2 + k] - off);
+        *reinterpret_cast<float4*>(dst + 4 * t) = make_float4(fmaf(o[n][2 * t][k], 16777216.0f, -off), fmaf(o[n][2 * t][2 + k], 1048576.0f, -off),
+                                                              fmaf(o[n][2 * t + 1][k], 16777216.0f, -off), fmaf(o[n][2 * t + 1][2 + k], 1048576.0f, -off));
       if (g == 0) { sh.m[warp][r] = m[n][k]; sh.l[warp][r] = l[n][k]; }
     }
   __syncthreads();
-  for (int r = warp; r < w.rows; r += kRwWarps) {
+  for (int r = warp; r < w.rows; r += kWarps) {
     float mm = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < kRwWarps; ++x) mm = fmaxf(mm, sh.m[x][r]);
+    for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, sh.m[x][r]);
     float ll = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int x = 0; x < kRwWarps; ++x) {
+    for (int x = 0; x < kWarps; ++x) {
       if (sh.m[x][r] == -INFINITY && sh.l[x][r] == 0.0f) continue;     // a warp that saw no token of the row
       const float f = ex2(sh.m[x][r] - mm);
       const float4 v = *reinterpret_cast<const float4*>(merge + ((size_t)x * R + r) * kRwORow + 4 * lane);
@@ -449,54 +467,67 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   if (p.splits > 1) {
     kv_cluster_barrier();
     // the CTAs of the cluster deal out the rows
-    kv_merge_rows<1>(p.splits, (int)crank + p.splits * warp, p.splits * kRwWarps, w.rows, lane, sh.part_m, sh.part_l,
+    kv_merge_rows<1>(p.splits, (int)crank + p.splits * warp, p.splits * kWarps, w.rows, lane, sh.part_m, sh.part_l,
                      [&](int r) { return &sh.part_o[r][4 * lane]; },
                      [&](int r, float4 v, float inv) { rw_store_row(p, w, head_kv, r, 4 * lane, v, inv); });
     kv_cluster_barrier();
   }
 }
 
-int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, int64_t most, int* splits) {
-  constexpr int kMost = 16;
-  struct Known { int fit[kMost + 1]; };
-  static std::mutex mu;
-  static std::map<std::pair<const void*, int>, Known> cache;
+namespace {
+// Clusters of s CTAs that fit on a device, for s = 1 .. 16.  Two threads that ask first write the same numbers.
+struct KvFit {
+  std::atomic<int> known, per_sm, fit[17];
+};
+constexpr int kKvDevices = 32;
+KvFit g_kv_fit[kKvKernels][kKvDevices];
+
+int kv_ask_fit(KvFit& k, const void* kernel, int threads, size_t smem) {
+  QR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  QR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  int per_sm = 0;
+  QR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+  k.per_sm.store(per_sm, std::memory_order_relaxed);
+  k.fit[1].store(per_sm * num_sms(), std::memory_order_relaxed);
+  for (int s = 2; s <= 16; ++s) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)s);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+    k.fit[s].store(n, std::memory_order_relaxed);
+  }
+  k.known.store(1, std::memory_order_release);
+  return QR_OK;
+}
+}  // namespace
+
+int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
+                   double joined, int* splits) {
   int dev = 0;
   QR_CUDA(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lk(mu);
-  auto it = cache.find({kernel, dev});
-  if (it == cache.end()) {
-    Known k = {};
-    QR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    int per_sm = 0;
-    QR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-    k.fit[1] = per_sm * num_sms();
-    for (int s = 2; s <= kMost; ++s) {
-      cudaLaunchConfig_t cfg = {};
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)s;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3((unsigned)s);
-      cfg.blockDim = dim3((unsigned)threads);
-      cfg.dynamicSmemBytes = smem;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-      k.fit[s] = n;
-    }
-    it = cache.emplace(std::make_pair(kernel, dev), k).first;
+  if (dev < 0 || dev >= kKvDevices) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: device %d (at most %d)", dev, kKvDevices - 1);
+  KvFit& k = g_kv_fit[which][dev];
+  if (!k.known.load(std::memory_order_acquire)) {
+    if (const int rc = kv_ask_fit(k, kernel, threads, smem)) return rc;
   }
-  // cost in parts of one unit's work: a round costs 1/16 of a unit beside its share of the work, twice that where shares
-  // have to be joined, so that a split has to pay
+  const int per_sm = k.per_sm.load(std::memory_order_relaxed);
   double best = 0.0;
   *splits = 1;
-  for (int s = 1; s <= kMost && s <= most; ++s) {
-    const int fit = it->second.fit[s];
+  for (int s = 1; s <= 16 && s <= most; ++s) {
+    const int fit = k.fit[s].load(std::memory_order_relaxed);
     if (fit < 1) continue;
-    const double cost = (double)((units + fit - 1) / fit) * (1.0 / s + (s > 1 ? 2.0 : 1.0) / 16);
+    // CTAs that the fullest SM works through, against those that it holds: an SM that is not full takes as long as a full one
+    const int64_t load = (units * per_sm + fit - 1) / fit;
+    const double cost = (double)(load < per_sm ? per_sm : load) / per_sm * (1.0 / s + (s > 1 ? joined : alone));
     if (s == 1 || cost < best * 0.98) { best = cost; *splits = s; }
   }
   return QR_OK;
@@ -504,9 +535,9 @@ int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, 
 
 template <int NT>
 static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
-  constexpr int R = 8 * NT;
+  constexpr int R = 8 * NT, kWarps = RwConfig<NT>::kWarps;
   constexpr size_t smem = RwConfig<NT>::kRing + sizeof(RwShared<NT>);
-  static_assert(kRwWarps * R * kRwORow * sizeof(float) <= RwConfig<NT>::kRing, "the merge buffer lies in the ring");
+  static_assert(kWarps * R * kRwORow * sizeof(float) <= RwConfig<NT>::kRing, "the merge buffer lies in the ring");
   static_assert(RwConfig<NT>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory");
   // tiles: at most one ragged tile per sequence beyond the full ones; a grid of equal shares per sequence needs no search
   const int64_t per_seq = (max_rows + R - 1) / R;
@@ -515,9 +546,13 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
-  QR_CUDA(cudaFuncSetAttribute(kv_attend_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int splits = 1;
-  if (const int rc = kv_pick_splits((const void*)kv_attend_rows_kernel<NT>, 32 * kRwWarps, smem, units, (visible_blocks(p, max_rows, kRwTok) + kRwWarps - 1) / kRwWarps, &splits)) return rc;
+  // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
+  // more; where no window says how long a unit is, 64 blocks are assumed
+  const int64_t blocks = visible_blocks(p, max_rows, kRwTok), parts = (blocks + kWarps - 1) / kWarps;
+  const double length = (double)(p.window > 0 ? blocks : 64) / kWarps;
+  if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
+                                    smem, units, parts, 2.0 / length, 2.5 / length, &splits)) return rc;
   p.splits = splits;
   if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   cudaLaunchConfig_t cfg = {};
@@ -527,7 +562,7 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(units * splits));
-  cfg.blockDim = dim3(32 * kRwWarps);
+  cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -538,8 +573,7 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
 
 int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   if (max_rows <= 8) return launch_rows<1>(p, max_rows, st);
-  if (max_rows <= 16) return launch_rows<2>(p, max_rows, st);
-  return launch_rows<4>(p, max_rows, st);
+  return launch_rows<2>(p, max_rows, st);
 }
 
 }  // namespace qr
@@ -582,6 +616,9 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
   p.page_div = make_fastdiv((uint32_t)page_size); p.group_div = make_fastdiv((uint32_t)group);
   p.window = window; p.sinks = window > 0 ? sink_tokens : 0; p.hadamard_q = hadamard_q;
   p.status = kernel_status_ptr();
+  // Up to 64 rows per KV head: mma.sync, 16 rows at a time; above: tcgen05, 256 rows at a time, at a cost that hardly depends
+  // on the rows.  32 sequences of 8192 tokens, 8 KV heads: 32 rows 194 us here, 378 there; 48 rows 289 and 378; 64 rows 382
+  // and 378; 96 rows 569 and 379.  One sequence of 16384 tokens: 64 rows 33 and 51, 96 rows 46 and 53.
   const int64_t rows = max_q_len * group;
   return rows > 64 ? launch_kv_attend_tc(p, rows, (cudaStream_t)stream) : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
 }

@@ -650,7 +650,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
     regs_dec<64>();
     const int tid = threadIdx.x & 127, pw = warp & 3;
     const int what = warp >= 12;
-    const int first_page = p.indptr[w.b];
+    const int first_page = w.first;
     const int tokens = min(p_max + 1, w.seq_len);
     const size_t page_rows = (size_t)p.layers * 2 * p.kv_heads * p.page_size;
     const size_t row_k = ((size_t)p.layer * 2 * p.kv_heads + head_kv) * p.page_size;
@@ -894,9 +894,9 @@ int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
-  QR_CUDA(cudaFuncSetAttribute(kv_attend_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAtSmem));
   int splits = 1;
-  if (const int rc = kv_pick_splits((const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, units, visible_blocks(p, max_rows, kAtTok), &splits)) return rc;
+  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, units, visible_blocks(p, max_rows, kAtTok),
+                                    1.0 / 16, 2.0 / 16, &splits)) return rc;
   p.splits = splits;
   if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   cudaLaunchConfig_t cfg = {};

@@ -25,12 +25,12 @@ __device__ __forceinline__ void fwht128_warp(float (&x)[4], int lane) {
   }
 }
 
-__device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ void half4_to_f32(uint2 u, float (&x)[4]) {
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
+__device__ __forceinline__ void load4_f16(const __half* p, float (&x)[4]) { half4_to_f32(*reinterpret_cast<const uint2*>(p), x); }
 #endif
 
 #ifdef __CUDACC__
@@ -127,11 +127,14 @@ static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, 
 }
 
 #ifdef __CUDACC__
-// CTAs of a cluster that share the token axis of a unit of work (a tile of rows of one KV head), 1 .. 16: the number s for
-// which ceil(units / clusters of s that fit on the device) rounds of 1 / s of the work, with a share lost to each round,
-// cost least.  How many clusters fit is asked once per kernel, device and size (clusters lie within a GPC, whose SMs they
-// do not divide evenly: 15 clusters of 8 fit, 16 do not).  At most `most`: parts of the work that there are.
-int kv_pick_splits(const void* kernel, int threads, size_t smem, int64_t units, int64_t most, int* splits);
+// Splitting the token axis of a unit of work (a tile of rows of one KV head) over a cluster of s = 1 .. 16 CTAs.  The cost of
+// s, in parts of a unit, is (rounds of CTAs that an SM goes through) * (1 / s + what a CTA costs beside its share of the
+// tokens); `most` is the number of parts that there are.  `alone` and `joined`: that cost without and with other CTAs to
+// join.  How many clusters fit is asked once per kernel, device and size (clusters lie within a GPC, whose SMs they do not
+// divide evenly: 15 clusters of 8 fit, 16 do not); the kernel's attributes are set then too.
+enum { kKvKernelRows8, kKvKernelRows16, kKvKernelTc, kKvKernels };
+int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
+                   double joined, int* splits);
 
 // fp32 shares [rows][128] (addr(r): the lane's four columns of row r) of the CTAs of a cluster joined into one row, U rows
 // at a time.  Lane x looks at the statistics of CTA x; the first two shares are asked for before that.
@@ -195,6 +198,7 @@ __device__ __forceinline__ void kv_merge_rows(int splits, int first, int step, i
 // The tile of query rows that a CTA works on.  Row r of a sequence is (new token r / group, head r % group of the KV head).
 struct KvTile {
   int b, row0, rows;            // sequence, first row, rows (0: nothing to do)
+  int first;                    // the sequence's first entry of the page list
   int64_t tok0;                 // first new token of the sequence in q and o
   int seq_len, pos0;            // cached tokens with the new ones; position of new token 0
 };
@@ -202,7 +206,7 @@ struct KvTile {
 // Sequence and tile of rows behind tile index `tile`, by all lanes of a warp.
 __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile, int tile_rows, int lane) {
   KvTile w;
-  w.rows = 0; w.b = 0; w.row0 = 0; w.tok0 = 0; w.seq_len = 0; w.pos0 = 0;
+  w.rows = 0; w.b = 0; w.first = 0; w.row0 = 0; w.tok0 = 0; w.seq_len = 0; w.pos0 = 0;
   int j = -1, b = 0;
   if (p.tiles_per_seq > 0) {
     b = tile / p.tiles_per_seq;
@@ -234,16 +238,15 @@ __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile
     if (j < 0) return w;
   }
   if (b >= p.batch) return w;
-  long long tok0 = b, len = 1;
-  if (p.qo_indptr) {
-    tok0 = p.qo_indptr[b];
-    len = p.qo_indptr[b + 1] - tok0;
-  }
+  // one round trip for all of them
+  const int qo0 = p.qo_indptr ? __ldg(p.qo_indptr + b) : b, qo1 = p.qo_indptr ? __ldg(p.qo_indptr + b + 1) : b + 1;
+  const int first = __ldg(p.indptr + b), behind = __ldg(p.indptr + b + 1), last = __ldg(p.last_page_offset + b);
+  const long long tok0 = qo0, len = (long long)qo1 - qo0;
   if (tok0 < 0 || tok0 + len > p.total_q) return w;       // rows beyond q are not touched
   const long long rows = len * p.group, row0 = (long long)j * tile_rows;
   if (row0 >= rows) return w;
-  const int first = p.indptr[b];
-  const long long seq = (long long)(p.indptr[b + 1] - first - 1) * p.page_size + p.last_page_offset[b];
+  const long long seq = ((long long)behind - first - 1) * p.page_size + last;
+  w.first = first;
   w.b = b;
   w.row0 = (int)row0;
   w.rows = (int)(rows - row0 < tile_rows ? rows - row0 : tile_rows);
