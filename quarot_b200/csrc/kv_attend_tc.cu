@@ -50,6 +50,7 @@ constexpr uint32_t kTmem = 0;                             // the CTA owns all 51
 constexpr uint32_t kTmemO = kTmem, kTmemS = kTmem + 2 * kAtVRows;     // O_0 O_1 (144 columns each), then S of (tile, half)
 constexpr int kAtParStages = 3;
 constexpr float kAtTop = 15.0f;                           // weights are at most 2^15
+constexpr float kAtMove = 2.0f;                           // where one row has to move, all that have grown by this much do
 constexpr uint32_t kAtIdescS = (1u << 4) | ((48u >> 3) << 17) | ((128u >> 4) << 24);    // fp16 x fp16 -> fp32, K-major, 128 x 48
 constexpr uint32_t kAtIdescO = (1u << 4) | ((144u >> 3) << 17) | ((128u >> 4) << 24);   // 128 x 144
 
@@ -128,6 +129,13 @@ __device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x256_x4(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_16x256_x2(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
@@ -322,18 +330,37 @@ __device__ __forceinline__ void at_tops(uint32_t (&s)[2][24], const float* par, 
   }
 }
 
-// Multiplies O, the columns of the sums included, by the factors of the four rows.
-__device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
-#pragma unroll 1
-  for (int q = 0; q < 2 * kAtVRows / 16; ++q) {
-    uint32_t o[8];
-    const uint32_t at = t_o + (q >> 1) * 16 + ((uint32_t)(q & 1) << 20);
-    tmem_ld_16x256_x2(at, o);
-    tmem_ld_done<8>(o);
-    const float fa = q & 1 ? f[2] : f[0], fb = q & 1 ? f[3] : f[1];
+// The largest of the exponents that at_scores left, per row.
+__device__ __forceinline__ void at_largest(const uint32_t (&s)[2][24], float (&top)[4]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? fb : fa));
-    tmem_st_16x256_x2(at, o);
+  for (int x = 0; x < 4; ++x) {
+    top[x] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
+      top[x] = max3(top[x], __uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+  }
+}
+
+// Multiplies O, the columns of the sums included, by the factors of the four rows, 48 columns at a time.
+__device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
+  static_assert(kAtVRows % 48 == 0, "columns of O");
+#pragma unroll 1
+  for (int q = 0; q < kAtVRows / 48; ++q, t_o += 48) {
+    uint32_t o[2][24];
+    at_fetch(o, t_o);
+    tmem_ld_done<24>(o[0]);
+    tmem_ld_done<24>(o[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int e = 0; e < 24; ++e) o[h][e] = __float_as_uint(__uint_as_float(o[h][e]) * f[2 * h + ((e >> 1) & 1)]);
+      tmem_st_16x256_x4(t_o + ((uint32_t)h << 20), o[h]);
+      tmem_st_16x256_x2(t_o + 32 + ((uint32_t)h << 20), o[h] + 16);
+    }
   }
   tmem_st_done();
 }
@@ -522,25 +549,48 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
       if (__builtin_expect(edge, 0)) top = at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
       if (__builtin_expect(__any_sync(0xffffffffu, top > kAtTop), 0)) {
         // a weight would pass 2^15, or a row sees its first token: M moves, O follows by powers of two (or 0)
-        at_fetch(s, t_sb);
-        tmem_ld_done<24>(s[0]);
-        tmem_ld_done<24>(s[1]);
         float mn[4], f[4];
-        at_tops(s, par, rw, mn, edge, pos, t0 + 2 * c, p.window, p.sinks);
+        const bool fresh = __any_sync(0xffffffffu, fminf(fminf(rw.m[0], rw.m[1]), fminf(rw.m[2], rw.m[3])) == -INFINITY);
+        if (fresh) {                                      // no exponents yet: the scores are looked at once more
+          at_fetch(s, t_sb);
+          tmem_ld_done<24>(s[0]);
+          tmem_ld_done<24>(s[1]);
+          at_tops(s, par, rw, mn, edge, pos, t0 + 2 * c, p.window, p.sinks);
+        } else {
+          at_largest(s, mn);
+        }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const bool move = mn[x] - rw.m[x] > kAtTop;
-          const float to = ceilf(mn[x]) - 1.0f;
-          f[x] = !move ? 1.0f : rw.m[x] == -INFINITY ? 0.0f : ex2(rw.m[x] - to);
-          rw.m[x] = move ? to : rw.m[x];
+          if (fresh) {
+            const bool move = mn[x] - rw.m[x] > kAtMove;
+            const float to = ceilf(mn[x]) - 1.0f;
+            f[x] = !move ? 1.0f : rw.m[x] == -INFINITY ? 0.0f : ex2(rw.m[x] - to);
+            rw.m[x] = move ? to : rw.m[x];
+          } else {
+            mn[x] = mn[x] > kAtMove ? ceilf(mn[x]) - 1.0f : 0.0f;
+            f[x] = ex2(-mn[x]);
+            rw.m[x] += mn[x];
+          }
         }
         if (h > 0) {                                      // the products of half h - 1 may still be on their way
           ok = mbar_wait(pv_done + 8 * i, (h - 1) & 1, abort_flag, p.status, 73) && ok;
           tc_fence_after();
           at_scale_o(t_o, f);
         }
-        at_scores(s, par, rw);
-        if (edge) at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
+        if (fresh) {
+          at_scores(s, par, rw);
+          if (edge) at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int k = 0; k < 6; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t& v = s[x >> 1][4 * k + 2 * (x & 1) + e];
+                v = __float_as_uint(__uint_as_float(v) - mn[x]);
+              }
+        }
       }
       at_weights(s, t_sb);                                // in place of S, which is in registers
       tmem_st_done();

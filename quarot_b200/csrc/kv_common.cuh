@@ -256,10 +256,12 @@ __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile
   return w;
 }
 
-// Blocks of T tokens that the rows at positions p_min .. p_max see: `head` blocks from token 0 on (the sinks), then the
-// blocks first .. end.  Without a window, or where the two ranges meet, head = 0 and first = 0.
+// Blocks of T tokens that the rows at positions p_min .. p_max see: first .. first + body - 1, and with a window that does
+// not reach the sinks the blocks 0 .. count - body - 1 that hold these.  Where rows see only parts of the first block (a
+// window begins in it) it comes after the others, and the sinks last: the reference of a row's weights is set by the tokens
+// that it sees first, and moves the less the more of them there are.
 struct KvBlocks {
-  int head, first, count;
+  int first, body, turn, count;
 };
 template <int T>
 __device__ __forceinline__ KvBlocks kv_blocks(int p_min, int p_max, int window, int sinks) {
@@ -267,12 +269,16 @@ __device__ __forceinline__ KvBlocks kv_blocks(int p_min, int p_max, int window, 
   const int end = p_max >= 0 ? p_max / T + 1 : 0;
   const int lo = window > 0 ? max(0, p_min - window + 1) : 0;
   k.first = min(lo / T, end);
-  k.head = (max(min(sinks, p_max + 1), 0) + T - 1) / T;
-  if (window <= 0 || k.head >= k.first) { k.head = 0; k.first = 0; }
-  k.count = k.head + end - k.first;
+  int head = (max(min(sinks, p_max + 1), 0) + T - 1) / T;
+  if (window <= 0 || head >= k.first) { head = 0; k.first = 0; }
+  k.body = end - k.first;
+  k.turn = k.first > 0 && k.body > 1 ? 1 : 0;
+  k.count = head + k.body;
   return k;
 }
-__device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) { return i < k.head ? i : k.first + i - k.head; }
+__device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) {
+  return i < k.body - k.turn ? k.first + k.turn + i : i < k.body ? k.first : i - k.body;
+}
 #endif
 
 int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
