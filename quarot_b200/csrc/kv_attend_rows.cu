@@ -511,7 +511,7 @@ int kv_ask_fit(KvFit& k, const void* kernel, int threads, size_t smem) {
 }  // namespace
 
 int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
-                   double joined, int* splits) {
+                   double joined, int* splits, double* cost_out) {
   int dev = 0;
   QR_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kKvDevices) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: device %d (at most %d)", dev, kKvDevices - 1);
@@ -530,6 +530,7 @@ int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int6
     const double cost = (double)(load < per_sm ? per_sm : load) / per_sm * (1.0 / s + (s > 1 ? joined : alone));
     if (s == 1 || cost < best * 0.98) { best = cost; *splits = s; }
   }
+  if (cost_out) *cost_out = best;
   return QR_OK;
 }
 
@@ -548,9 +549,9 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
   int splits = 1;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
-  // more; where no window says how long a unit is, 64 blocks are assumed
+  // more; where no window says how long a unit is, at most 64 blocks are assumed
   const int64_t blocks = visible_blocks(p, max_rows, kRwTok), parts = (blocks + kWarps - 1) / kWarps;
-  const double length = (double)(p.window > 0 ? blocks : 64) / kWarps;
+  const double length = (double)(p.window > 0 || blocks < 64 ? blocks : 64) / kWarps;
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
                                     smem, units, parts, 2.0 / length, 2.5 / length, &splits)) return rc;
   p.splits = splits;
@@ -583,7 +584,7 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
                                const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_offset,
                                const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
                                int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
-                               int hadamard_q, void* stream) {
+                               int hadamard_q, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace qr;
   if (batch < 0 || total_q < 0 || max_q_len < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative size");
   if (batch == 0 || total_q == 0 || max_q_len == 0) return QR_OK;
@@ -603,6 +604,7 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
   const int group = num_q_heads / num_kv_heads;
   if (total_q * group > 0x3fffffffll || (int64_t)batch * max_q_len * group > 0xffffffffffll)
     return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many query rows");
+  if (workspace && ((uintptr_t)workspace & 15)) return fail(QR_EALIGN, "qr_kv_attend_i4: workspace must be 16-byte aligned");
   if (((uintptr_t)q & 7) || ((uintptr_t)o & 7) || ((uintptr_t)kv_data & 15) || ((uintptr_t)kv_param & 3) || (q_token_stride & 3) ||
       (q_head_stride & 3) || (o_token_stride & 3) || (o_head_stride & 3))
     return fail(QR_EALIGN, "qr_kv_attend_i4: q and o must be 8-byte aligned with strides that are multiples of 4, the pages 16-byte aligned");
@@ -620,5 +622,20 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
   // on the rows.  32 sequences of 8192 tokens, 8 KV heads: 32 rows 194 us here, 378 there; 48 rows 289 and 378; 64 rows 382
   // and 378; 96 rows 569 and 379.  One sequence of 16384 tokens: 64 rows 33 and 51, 96 rows 46 and 53.
   const int64_t rows = max_q_len * group;
-  return rows > 64 ? launch_kv_attend_tc(p, rows, (cudaStream_t)stream) : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
+  return rows > kKvRowsMost ? launch_kv_attend_tc(p, rows, workspace, workspace_bytes, (cudaStream_t)stream)
+                            : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
+}
+
+extern "C" size_t qr_kv_attend_workspace_bytes(int64_t num_pages, int page_size, int64_t total_q, int64_t max_q_len, int batch,
+                                               int num_q_heads, int num_kv_heads, int window, int sink_tokens) {
+  using namespace qr;
+  if (num_pages < 1 || page_size < 1 || total_q < 1 || max_q_len < 1 || batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads ||
+      num_q_heads % num_kv_heads || window < 0 || sink_tokens < 0 || max_q_len > total_q)
+    return 0;
+  KvAttendParams p = {};
+  p.num_pages = num_pages; p.page_size = page_size; p.total_q = total_q; p.batch = batch; p.kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads; p.window = window; p.sinks = window > 0 ? sink_tokens : 0;
+  size_t bytes = 0;
+  if (max_q_len * p.group <= kKvRowsMost || kv_attend_tc_workspace(p, max_q_len * p.group, &bytes) != QR_OK) return 0;
+  return bytes;
 }

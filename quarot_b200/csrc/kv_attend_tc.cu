@@ -470,8 +470,9 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   volatile int* abort_flag = &sh.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t crank = 0;
-  if (p.splits > 1) crank = kv_cluster_rank();
   const int unit = blockIdx.x / p.splits;
+  const bool joined = p.splits > 1, clustered = joined && !p.part;
+  if (joined) crank = blockIdx.x - unit * p.splits;       // also the rank within a cluster
   const int head_kv = unit % p.kv_heads;
   // the last tiles of a sequence see the most tokens: they start first
   const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
@@ -617,7 +618,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
       ok = __all_sync(0xffffffffu, ok);
     }
     // the merge area of one row tile lies over operands of the other, whose MMAs may still be running
-    if (p.splits > 1) asm volatile("bar.sync 3, 256;" ::: "memory");
+    if (clustered) asm volatile("bar.sync 3, 256;" ::: "memory");
     if (ok) {
       tc_fence_after();
       // the sums: columns 128, 129 (2^10 w / sigma, in two parts) in lane c = 0, 130, 131 (w (z' / sigma - ..)) in lane c = 1
@@ -653,13 +654,15 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         for (int hh = 0; hh < 2; ++hh) {
           const float ll = q4 & 1 ? l[2 + hh] : l[hh], yy = q4 & 1 ? y[2 + hh] : y[hh];
           const int r = row0 + 16 * (q4 & 1) + 8 * hh + g;
-          const float inv = p.splits > 1 ? 1.0f : (ll != 0.0f ? 1.0f / ll : 0.0f);      // a row that sees nothing gives zeros
+          const float inv = joined ? 1.0f : (ll != 0.0f ? 1.0f / ll : 0.0f);      // a row that sees nothing gives zeros
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float e0 = (__uint_as_float(o[4 * k + 2 * hh]) - yy) * inv, e1 = (__uint_as_float(o[4 * k + 2 * hh + 1]) - yy) * inv;
             const int col = 64 * (q4 >> 1) + 8 * k + 2 * c;
-            if (p.splits > 1) {
+            if (clustered) {
               *reinterpret_cast<float2*>(smem + at_part_off(r, col >> 2) + (col & 2) * 4) = make_float2(e0, e1);
+            } else if (joined) {
+              if (n > 0) *reinterpret_cast<float2*>(p.part + ((size_t)blockIdx.x * kAtRows + r) * kHeadDim + col) = make_float2(e0, e1);
             } else {
               const __half2 hv = __floats2half2_rn(e0, e1);
               *reinterpret_cast<__half2*>(smem + r * 256 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2) = hv;
@@ -667,10 +670,12 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
           }
         }
       }
-      if (p.splits > 1) {
+      if (joined) {
+        float* m_out = clustered ? sh.m : p.part + (size_t)gridDim.x * kAtRows * kHeadDim + (size_t)blockIdx.x * (2 * kAtRows);
+        float* l_out = clustered ? sh.l : m_out + kAtRows;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (c == 0) { sh.m[row0 + g + 8 * x] = rw.m[x]; sh.l[row0 + g + 8 * x] = l[x]; }
+          if (c == 0) { m_out[row0 + g + 8 * x] = rw.m[x]; l_out[row0 + g + 8 * x] = l[x]; }
       } else {
         __syncwarp();
         for (int rr = 0; rr < 32; ++rr) {                 // a row is 256 contiguous bytes
@@ -681,7 +686,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         }
       }
     }
-    if (p.splits > 1) {
+    if (clustered) {
       kv_cluster_barrier();
       // the CTAs of the cluster deal out the rows
       kv_merge_rows<4>(p.splits, (int)crank + p.splits * warp, p.splits * 8, w.rows, lane, sh.m, sh.l,
@@ -874,7 +879,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         if (lane == 0) mbar_arrive(v_full + 8 * stage);
       }
     }
-    if (p.splits > 1) { kv_cluster_barrier(); kv_cluster_barrier(); }
+    if (clustered) { kv_cluster_barrier(); kv_cluster_barrier(); }
   } else {
     // ---------------------------------------------------------------- MMA issue
     regs_dec<32>();
@@ -926,7 +931,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
       }
       __syncwarp();
     }
-    if (p.splits > 1) { kv_cluster_barrier(); kv_cluster_barrier(); }
+    if (clustered) { kv_cluster_barrier(); kv_cluster_barrier(); }
   }
   drain_after_abort(abort_flag);
   tc_fence_before();
@@ -937,31 +942,93 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   }
 }
 
-int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
+// Shares of the CTAs of a unit that went to global memory joined into the result: a warp per row.
+__global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = blockIdx.x / (kAtRows / 8), r = (blockIdx.x % (kAtRows / 8)) * 8 + warp;
+  const int head_kv = unit % p.kv_heads;
+  const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
+  if (r >= w.rows) return;
+  const int cta = unit * p.splits;
+  const float* stat = p.part + (size_t)p.max_tiles * p.kv_heads * p.splits * kAtRows * kHeadDim + (size_t)cta * (2 * kAtRows) + r;
+  const float* part = p.part + ((size_t)cta * kAtRows + r) * kHeadDim + 4 * lane;
+  float f = lane < p.splits ? stat[lane * (2 * kAtRows)] : -INFINITY;
+  const float l = lane < p.splits ? stat[lane * (2 * kAtRows) + kAtRows] : 0.0f;
+  float mm = f;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+  f = f == -INFINITY && l == 0.0f ? 0.0f : ex2(f - mm);   // a share that saw no token of the row
+  float ll = l * f;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int x = 0; x < p.splits; ++x) {
+    const float fx = __shfl_sync(0xffffffffu, f, x);
+    if (fx == 0.0f) continue;                             // may not have been written
+    const float4 v = *reinterpret_cast<const float4*>(part + (size_t)x * (kAtRows * kHeadDim));
+    acc.x = fmaf(v.x, fx, acc.x); acc.y = fmaf(v.y, fx, acc.y); acc.z = fmaf(v.z, fx, acc.z); acc.w = fmaf(v.w, fx, acc.w);
+  }
+  const __half2 h0 = __floats2half2_rn(acc.x * inv, acc.y * inv), h1 = __floats2half2_rn(acc.z * inv, acc.w * inv);
+  uint2 out;
+  out.x = *reinterpret_cast<const uint32_t*>(&h0);
+  out.y = *reinterpret_cast<const uint32_t*>(&h1);
+  *reinterpret_cast<uint2*>(at_out_row(p, w, head_kv, r) + 4 * lane) = out;
+}
+
+// Tiles, split and, where the CTAs of a unit are to meet in global memory, the bytes for it.
+static int at_plan(KvAttendParams& p, int64_t max_rows, int64_t* units, size_t* bytes) {
   const int64_t per_seq = (max_rows + kAtRows - 1) / kAtRows;
   const int64_t bound = p.total_q * p.group / kAtRows + p.batch;
-  const bool uniform = !p.qo_indptr || p.batch * per_seq <= 2 * bound;
+  const bool uniform = p.batch * per_seq <= 2 * bound;
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
-  const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
-  int splits = 1;
-  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, units, visible_blocks(p, max_rows, kAtTok),
-                                    1.0 / 16, 2.0 / 16, &splits)) return rc;
-  p.splits = splits;
-  if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
+  *units = (int64_t)p.max_tiles * p.kv_heads;
+  *bytes = 0;
+  const int64_t blocks = visible_blocks(p, max_rows, kAtTok);
+  double cost = 0.0;
+  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, *units, blocks, 1.0 / 16, 2.0 / 16,
+                                    &p.splits, &cost)) return rc;
+  // Clusters lie within a GPC and leave SMs over: 16 units get 6 CTAs each from them, 9 without.
+  int64_t s = num_sms() / *units;
+  if (s > blocks) s = blocks;
+  if (s > 32) s = 32;
+  if (s > p.splits && 1.0 / s + 2.0 / 16 < 0.9 * cost) *bytes = (size_t)(*units * s) * kAtRows * (kHeadDim + 2) * sizeof(float);
+  return QR_OK;
+}
+
+int kv_attend_tc_workspace(KvAttendParams& p, int64_t max_rows, size_t* bytes) {
+  int64_t units = 0;
+  return at_plan(p, max_rows, &units, bytes);
+}
+
+int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  int64_t units = 0;
+  size_t bytes = 0;
+  if (const int rc = at_plan(p, max_rows, &units, &bytes)) return rc;
+  if (bytes > 0 && workspace && workspace_bytes >= bytes) {
+    p.part = reinterpret_cast<float*>(workspace);
+    p.splits = (int)(bytes / (kAtRows * (kHeadDim + 2) * sizeof(float)) / units);
+  }
+  if (units * p.splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.x = (unsigned)p.splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(units * splits));
+  cfg.gridDim = dim3((unsigned)(units * p.splits));
   cfg.blockDim = dim3(kAtThreads);
   cfg.dynamicSmemBytes = kAtSmem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cfg.numAttrs = p.splits > 1 && !p.part ? 1 : 0;
   QR_CUDA(cudaLaunchKernelEx(&cfg, kv_attend_tc_kernel, (const KvAttendParams)p));
+  if (p.part) {
+    kv_attend_join_kernel<<<(unsigned)(units * (kAtRows / 8)), 256, 0, st>>>(p);
+    QR_LAUNCH_CHECK("kv_attend_join_kernel");
+  }
   return QR_OK;
 }
 

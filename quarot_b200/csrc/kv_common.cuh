@@ -114,16 +114,20 @@ struct KvAttendParams {
   FastDiv page_div, group_div;
   int window, sinks;            // window 0: none
   int hadamard_q;
-  int splits;                   // CTAs (one cluster) that share the tokens of a tile of rows
+  int splits;                   // CTAs (one cluster, or joined through `part`) that share the tokens of a tile of rows
+  float* part;                  // tcgen05 kernel: shares of the CTAs in global memory, or NULL
   int tiles_per_seq;            // > 0: tile index = sequence * tiles_per_seq + tile; 0: found by a search in qo_indptr
   int max_tiles;                // tiles that the grid holds per KV head
   int* status;
 };
 
-// Upper bound, where the host knows one, of the blocks of T tokens that a tile of rows sees.
+// Upper bound of the blocks of T tokens that a tile of rows sees, from the window and the pool (a page that is listed more
+// than once for a sequence may lead beyond it; only the split suffers).
 static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, int T) {
-  if (p.window <= 0) return 1ll << 40;
-  return ((int64_t)p.window + max_rows / p.group + T - 1) / T + 1 + ((int64_t)p.sinks + T - 1) / T;
+  const int64_t pool = (p.num_pages * p.page_size + T - 1) / T;
+  if (p.window <= 0) return pool;
+  const int64_t seen = ((int64_t)p.window + max_rows / p.group + T - 1) / T + 1 + ((int64_t)p.sinks + T - 1) / T;
+  return seen < pool ? seen : pool;
 }
 
 #ifdef __CUDACC__
@@ -134,7 +138,7 @@ static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, 
 // divide evenly: 15 clusters of 8 fit, 16 do not); the kernel's attributes are set then too.
 enum { kKvKernelRows8, kKvKernelRows16, kKvKernelTc, kKvKernels };
 int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
-                   double joined, int* splits);
+                   double joined, int* splits, double* cost = nullptr);
 
 // fp32 shares [rows][128] (addr(r): the lane's four columns of row r) of the CTAs of a cluster joined into one row, U rows
 // at a time.  Lane x looks at the statistics of CTA x; the first two shares are asked for before that.
@@ -282,6 +286,8 @@ __device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) {
 #endif
 
 int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
-int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
+int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, size_t workspace_bytes, cudaStream_t st);
+int kv_attend_tc_workspace(KvAttendParams& p, int64_t max_rows, size_t* bytes);
+constexpr int64_t kKvRowsMost = 64;   // query rows per KV head up to which the mma.sync kernel runs
 
 }  // namespace qr
