@@ -326,8 +326,8 @@ int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, cons
                     int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
                     int hadamard_q, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace with which qr_kv_attend_i4 spreads a call of these sizes over more SMs (few tiles of rows over long
- * sequences: the CTAs of a tile meet in memory instead of in a cluster); 0 where it needs none.  The workspace is 16-byte
+/* Bytes of workspace with which qr_kv_attend_i4 spreads a call of these sizes over more SMs (the CTAs of a tile of
+ * rows meet in memory instead of in a cluster); 0 where it needs none.  The workspace is 16-byte
  * aligned device memory of any content that no other work uses at the same time; without it (NULL, or fewer bytes) the call
  * is slower and rounds differently in the last bits. */
 size_t qr_kv_attend_workspace_bytes(int64_t num_pages, int page_size, int64_t total_q, int64_t max_q_len, int batch,

@@ -544,9 +544,10 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   const int64_t per_seq = (max_rows + R - 1) / R;
   const int64_t bound = p.total_q * p.group / R + p.batch;
   const bool uniform = !p.qo_indptr || p.batch * per_seq <= 2 * bound;
+  const int64_t tiles = uniform ? p.batch * per_seq : bound, units = tiles * p.kv_heads;
+  if (units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
-  p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
-  const int64_t units = (int64_t)p.max_tiles * p.kv_heads;
+  p.max_tiles = (int)tiles;
   int splits = 1;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
   // more; where no window says how long a unit is, at most 64 blocks are assumed
@@ -555,7 +556,6 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
                                     smem, units, parts, 2.0 / length, 2.5 / length, &splits)) return rc;
   p.splits = splits;
-  if (units * splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

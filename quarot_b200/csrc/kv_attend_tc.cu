@@ -470,9 +470,11 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   volatile int* abort_flag = &sh.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t crank = 0;
-  const int unit = blockIdx.x / p.splits;
-  const bool joined = p.splits > 1, clustered = joined && !p.part;
-  if (joined) crank = blockIdx.x - unit * p.splits;       // also the rank within a cluster
+  const int share = blockIdx.x - p.whole;                 // of the units that are split
+  const int splits = share < 0 ? 1 : p.splits;
+  const int unit = share < 0 ? blockIdx.x : p.whole + share / p.splits;
+  const bool joined = splits > 1, clustered = joined && !p.part;
+  if (joined) crank = share % p.splits;                   // also the rank within a cluster
   const int head_kv = unit % p.kv_heads;
   // the last tiles of a sequence see the most tokens: they start first
   const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
@@ -480,7 +482,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   const int tiles = w.rows > 128 ? 2 : 1;
   const int p_min = w.pos0 + fast_div(w.row0, p.group_div), p_max = w.pos0 + fast_div(w.row0 + w.rows - 1, p.group_div);
   const KvBlocks blk = kv_blocks<kAtTok>(p_min, p_max, p.window, p.sinks);
-  const int per = (blk.count + p.splits - 1) / p.splits;
+  const int per = (blk.count + splits - 1) / splits;
   const int begin = (int)crank * per;
   const int n = max(min(begin + per, blk.count) - begin, 0);
 
@@ -662,7 +664,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
             if (clustered) {
               *reinterpret_cast<float2*>(smem + at_part_off(r, col >> 2) + (col & 2) * 4) = make_float2(e0, e1);
             } else if (joined) {
-              if (n > 0) *reinterpret_cast<float2*>(p.part + ((size_t)blockIdx.x * kAtRows + r) * kHeadDim + col) = make_float2(e0, e1);
+              if (n > 0) *reinterpret_cast<float2*>(p.part + ((size_t)share * kAtRows + r) * kHeadDim + col) = make_float2(e0, e1);
             } else {
               const __half2 hv = __floats2half2_rn(e0, e1);
               *reinterpret_cast<__half2*>(smem + r * 256 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2) = hv;
@@ -671,7 +673,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         }
       }
       if (joined) {
-        float* m_out = clustered ? sh.m : p.part + (size_t)gridDim.x * kAtRows * kHeadDim + (size_t)blockIdx.x * (2 * kAtRows);
+        float* m_out = clustered ? sh.m : p.part + (size_t)(gridDim.x - p.whole) * kAtRows * kHeadDim + (size_t)share * (2 * kAtRows);
         float* l_out = clustered ? sh.l : m_out + kAtRows;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -945,12 +947,12 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
 // Shares of the CTAs of a unit that went to global memory joined into the result: a warp per row.
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int unit = blockIdx.x / (kAtRows / 8), r = (blockIdx.x % (kAtRows / 8)) * 8 + warp;
+  const int split = blockIdx.x / (kAtRows / 8), unit = p.whole + split, r = (blockIdx.x % (kAtRows / 8)) * 8 + warp;
   const int head_kv = unit % p.kv_heads;
   const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
   if (r >= w.rows) return;
-  const int cta = unit * p.splits;
-  const float* stat = p.part + (size_t)p.max_tiles * p.kv_heads * p.splits * kAtRows * kHeadDim + (size_t)cta * (2 * kAtRows) + r;
+  const int cta = split * p.splits;
+  const float* stat = p.part + (size_t)(gridDim.x / (kAtRows / 8)) * p.splits * kAtRows * kHeadDim + (size_t)cta * (2 * kAtRows) + r;
   const float* part = p.part + ((size_t)cta * kAtRows + r) * kHeadDim + 4 * lane;
   float f = lane < p.splits ? stat[lane * (2 * kAtRows)] : -INFINITY;
   const float l = lane < p.splits ? stat[lane * (2 * kAtRows) + kAtRows] : 0.0f;
@@ -977,48 +979,63 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParam
   *reinterpret_cast<uint2*>(at_out_row(p, w, head_kv, r) + 4 * lane) = out;
 }
 
-// Tiles, split and, where the CTAs of a unit are to meet in global memory, the bytes for it.
-static int at_plan(KvAttendParams& p, int64_t max_rows, int64_t* units, size_t* bytes) {
+// How the work is cut: tiles, CTAs per tile and, where these are to meet in global memory, the bytes for it.
+struct AtPlan {
+  int64_t units;
+  int whole, splits;                                      // with memory to meet in
+  size_t bytes;                                           // 0: of no use
+};
+static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   const int64_t per_seq = (max_rows + kAtRows - 1) / kAtRows;
   const int64_t bound = p.total_q * p.group / kAtRows + p.batch;
   const bool uniform = p.batch * per_seq <= 2 * bound;
+  const int64_t tiles = uniform ? p.batch * per_seq : bound;
+  plan->units = tiles * p.kv_heads;
+  plan->bytes = 0;
+  if (plan->units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
-  p.max_tiles = (int)(uniform ? p.batch * per_seq : bound);
-  *units = (int64_t)p.max_tiles * p.kv_heads;
-  *bytes = 0;
+  p.max_tiles = (int)tiles;
   const int64_t blocks = visible_blocks(p, max_rows, kAtTok);
   double cost = 0.0;
-  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, *units, blocks, 1.0 / 16, 2.0 / 16,
-                                    &p.splits, &cost)) return rc;
-  // Clusters lie within a GPC and leave SMs over: 16 units get 6 CTAs each from them, 9 without.
-  int64_t s = num_sms() / *units;
+  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, plan->units, blocks, 1.0 / 16,
+                                    2.0 / 16, &p.splits, &cost)) return rc;
+  // Clusters lie within a GPC and leave SMs over (16 units get 6 CTAs each from them, 9 without), and they split all units
+  // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.
+  const int64_t sms = num_sms(), rounds = plan->units / sms, rest = plan->units % sms;
+  int64_t s = rest ? sms / rest : 1;
   if (s > blocks) s = blocks;
   if (s > 32) s = 32;
-  if (s > p.splits && 1.0 / s + 2.0 / 16 < 0.9 * cost) *bytes = (size_t)(*units * s) * kAtRows * (kHeadDim + 2) * sizeof(float);
+  if (s > 1 && rounds * (1.0 + 1.0 / 16) + 1.0 / s + 2.0 / 16 < 0.95 * cost) {
+    plan->whole = (int)(rounds * sms);
+    plan->splits = (int)s;
+    plan->bytes = (size_t)(rest * s) * kAtRows * (kHeadDim + 2) * sizeof(float);
+  }
   return QR_OK;
 }
 
 int kv_attend_tc_workspace(KvAttendParams& p, int64_t max_rows, size_t* bytes) {
-  int64_t units = 0;
-  return at_plan(p, max_rows, &units, bytes);
+  AtPlan plan = {};
+  const int rc = at_plan(p, max_rows, &plan);
+  *bytes = plan.bytes;
+  return rc;
 }
 
 int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, size_t workspace_bytes, cudaStream_t st) {
-  int64_t units = 0;
-  size_t bytes = 0;
-  if (const int rc = at_plan(p, max_rows, &units, &bytes)) return rc;
-  if (bytes > 0 && workspace && workspace_bytes >= bytes) {
+  AtPlan plan = {};
+  if (const int rc = at_plan(p, max_rows, &plan)) return rc;
+  if (plan.bytes > 0 && workspace && workspace_bytes >= plan.bytes) {
     p.part = reinterpret_cast<float*>(workspace);
-    p.splits = (int)(bytes / (kAtRows * (kHeadDim + 2) * sizeof(float)) / units);
+    p.whole = plan.whole;
+    p.splits = plan.splits;
   }
-  if (units * p.splits > 0x7fffffffll) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
+  const int64_t split = plan.units - p.whole;             // units that p.splits CTAs share
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)p.splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(units * p.splits));
+  cfg.gridDim = dim3((unsigned)(p.whole + split * p.splits));
   cfg.blockDim = dim3(kAtThreads);
   cfg.dynamicSmemBytes = kAtSmem;
   cfg.stream = st;
@@ -1026,7 +1043,7 @@ int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, si
   cfg.numAttrs = p.splits > 1 && !p.part ? 1 : 0;
   QR_CUDA(cudaLaunchKernelEx(&cfg, kv_attend_tc_kernel, (const KvAttendParams)p));
   if (p.part) {
-    kv_attend_join_kernel<<<(unsigned)(units * (kAtRows / 8)), 256, 0, st>>>(p);
+    kv_attend_join_kernel<<<(unsigned)(split * (kAtRows / 8)), 256, 0, st>>>(p);
     QR_LAUNCH_CHECK("kv_attend_join_kernel");
   }
   return QR_OK;

@@ -116,6 +116,7 @@ struct KvAttendParams {
   int hadamard_q;
   int splits;                   // CTAs (one cluster, or joined through `part`) that share the tokens of a tile of rows
   float* part;                  // tcgen05 kernel: shares of the CTAs in global memory, or NULL
+  int whole;                    // with `part`: units before this one have a CTA each
   int tiles_per_seq;            // > 0: tile index = sequence * tiles_per_seq + tile; 0: found by a search in qo_indptr
   int max_tiles;                // tiles that the grid holds per KV head
   int* status;
