@@ -577,6 +577,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         }
         if (h > 0) {                                      // the products of half h - 1 may still be on their way
           ok = mbar_wait(pv_done + 8 * i, (h - 1) & 1, abort_flag, p.status, 73) && ok;
+          __syncwarp();
           tc_fence_after();
           at_scale_o(t_o, f);
         }
@@ -620,6 +621,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
       ok = __all_sync(0xffffffffu, ok);
     }
     // the merge area of one row tile lies over operands of the other, whose MMAs may still be running
+    __syncwarp();
     if (clustered) asm volatile("bar.sync 3, 256;" ::: "memory");
     if (ok) {
       tc_fence_after();
@@ -726,6 +728,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
         row = (long long)(page * page_rows + row_0 + slot);
       }
       if (tid < kAtTok) sh.row[what][j & 1][tid] = row;
+      __syncwarp();
       asm volatile("bar.sync %0, 128;" ::"r"(1 + what) : "memory");
       return row;
     };
@@ -827,6 +830,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
           load_par(mine);
           if (j + 2 < n) id = page_id(j + 2);
         } else {
+          __syncwarp();
           asm volatile("bar.sync 2, 128;" ::: "memory");
         }
         if (j >= 2) {

@@ -208,6 +208,7 @@ struct KvTile {
   int seq_len, pos0;            // cached tokens with the new ones; position of new token 0
 };
 
+constexpr int kKvMostTokens = 0x7fff0000;
 // Sequence and tile of rows behind tile index `tile`, by all lanes of a warp.
 __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile, int tile_rows, int lane) {
   KvTile w;
@@ -250,7 +251,11 @@ __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile
   if (tok0 < 0 || tok0 + len > p.total_q) return w;       // rows beyond q are not touched
   const long long rows = len * p.group, row0 = (long long)j * tile_rows;
   if (row0 >= rows) return w;
-  const long long seq = ((long long)behind - first - 1) * p.page_size + last;
+  // not beyond the pages that are listed, whatever the last page's offset says
+  const long long listed = ((long long)behind - first) * p.page_size;
+  long long seq = listed - p.page_size + last;
+  if (seq > listed) seq = listed;
+  if (seq > kKvMostTokens) return w;                      // tokens are counted in 32 bits
   w.first = first;
   w.b = b;
   w.row0 = (int)row0;
@@ -272,7 +277,8 @@ template <int T>
 __device__ __forceinline__ KvBlocks kv_blocks(int p_min, int p_max, int window, int sinks) {
   KvBlocks k;
   const int end = p_max >= 0 ? p_max / T + 1 : 0;
-  const int lo = window > 0 ? max(0, p_min - window + 1) : 0;
+  // p_min < 0: a row before the sequence (more new tokens than cached ones), which sees nothing
+  const int lo = window > 0 ? max(0, max(p_min, 0) - window + 1) : 0;
   k.first = min(lo / T, end);
   int head = (max(min(sinks, p_max + 1), 0) + T - 1) / T;
   if (window <= 0 || head >= k.first) { head = 0; k.first = 0; }
