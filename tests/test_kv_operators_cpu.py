@@ -1,4 +1,6 @@
 """Argument checks of the cache operators that are made before anything touches a GPU, and the CPU side of the cache."""
+import threading
+
 import pytest
 import torch
 
@@ -10,13 +12,22 @@ from oracle import quarot_oracle as O
 P = 1 << 20                                                         # stands for an aligned pointer; nothing reads it
 
 
+def _call(name, *args):
+    """(status, error text) of a C entry, from a thread of its own: the text of the last error is kept per thread."""
+    out = []
+    t = threading.Thread(target=lambda: out.append((getattr(_lib.lib, name)(*args), _lib.last_error())))
+    t.start()
+    t.join()
+    return out[0]
+
+
 def _attend(**kw):
     a = dict(o=P, ots=1024, ohs=128, q=P, qts=1024, qhs=128, data=P, param=P, pages=10, indptr=P, indices=P, last=P, qo=P, total=8,
              most=8, batch=1, layers=1, layer=0, heads=8, kv_heads=8, page=16, dim=128, window=0, sinks=0, rotate=0, work=None, bytes=0,
              stream=None)
     assert not set(kw) - set(a)
     a.update(kw)
-    return _lib.lib.qr_kv_attend_i4(*a.values())
+    return _call("qr_kv_attend_i4", *a.values())
 
 
 @pytest.mark.parametrize("kw,words", [
@@ -29,12 +40,12 @@ def _attend(**kw):
     (dict(o=P + 4), "aligned"), (dict(q=P + 2), "aligned"), (dict(data=P + 8), "aligned"), (dict(param=P + 2), "aligned"),
     (dict(qts=1022), "aligned"), (dict(ohs=130), "aligned"), (dict(work=P + 8, bytes=64), "aligned")])
 def test_attention_entry_refuses(kw, words):
-    assert _attend(**kw) != 0
-    assert words in _lib.last_error()
+    rc, text = _attend(**kw)
+    assert rc != 0 and words in text
 
 
 def test_empty_calls_do_nothing():
-    assert _attend(batch=0) == 0 and _attend(total=0) == 0 and _attend(most=0) == 0
+    assert [_attend(**kw)[0] for kw in (dict(batch=0), dict(total=0), dict(most=0))] == [0, 0, 0]
     assert _lib.lib.qr_kv_page_table(None, None, 0, 0, 16, 4, None, None, 0, None, None, None, None, None, None, None, None, None) == 0
 
 
@@ -44,7 +55,8 @@ def test_page_table_entry_refuses(change):
     a = [P, P, 4, 8, 16, 4, P, P, 4, P, P, P, P, P, P, P, P, None]
     for i, v in change.items():
         a[i] = v
-    assert _lib.lib.qr_kv_page_table(*a) != 0 and "qr_kv_page_table" in _lib.last_error()
+    rc, text = _call("qr_kv_page_table", *a)
+    assert rc != 0 and "qr_kv_page_table" in text
 
 
 @pytest.mark.parametrize("change", [{0: None}, {1: None}, {3: None}, {4: None}, {7: None}, {2: 0}, {10: -1}, {11: 0}, {12: 5}, {13: 0}, {14: 0},
@@ -53,7 +65,8 @@ def test_append_by_slot_map_entry_refuses(change):
     a = [P, P, 10, P, P, 1024, 128, P, 1024, 128, 4, 2, 1, 8, 16, 128, 0, None]
     for i, v in change.items():
         a[i] = v
-    assert _lib.lib.qr_kv_append_slots_i4(*a) != 0 and "qr_kv_append_slots_i4" in _lib.last_error()
+    rc, text = _call("qr_kv_append_slots_i4", *a)
+    assert rc != 0 and "qr_kv_append_slots_i4" in text
 
 
 def test_tensors_of_the_cpu_are_refused():
