@@ -365,9 +365,8 @@ __device__ __forceinline__ void at_scale_o(uint32_t t_o, const float (&f)[4]) {
   tmem_st_done();
 }
 
-// The 32 query rows of a softmax warp: into the Q tile, their sums and positions.  Four rows at a time, eight lanes to a row
-// and sixteen dimensions to a lane, so that the rotation needs three exchanges between lanes instead of five.  8 dimensions
-// 8 i .. 8 i + 7 lie as 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart.
+// The 32 query rows of a softmax warp: into the Q tile, their sums and positions.  8 dimensions 8 i .. 8 i + 7 lie as
+// 0 4 1 5 2 6 3 7, the order in which a word of key codes comes apart.
 // (A call: inlined, its registers cost the loop of the softmax 5 %.)
 struct AtQuery {
   const __half* q;                                        // first new token of the sequence, first query head of the group
@@ -376,82 +375,72 @@ struct AtQuery {
   int group, row0, rows, pos0, hadamard;
 };
 __device__ __noinline__ void at_load_rows(const AtQuery a, int row0, int lane, unsigned char* tile, float* s_sum, int* s_pos) {
-  const int sub = lane >> 3, l8 = lane & 7;
-  // all rows on their way at once, each to its place in the two atoms, in their natural order; two at a time where they are
+  // all rows on their way at once, each to its place in the two swizzled atoms, in their natural order; two at a time where they are
   // 16-byte aligned
   const bool wide = ((reinterpret_cast<uintptr_t>(a.q) & 15) | (a.ts & 7) | (a.hs & 7)) == 0;
   const int per = wide ? 2 : 1, piece = wide ? lane & 15 : lane, bytes = wide ? 16 : 8;
   {
     int r = row0 + (wide ? lane >> 4 : 0);
-    int tok = fast_div(a.row0 + r, a.group_div), hh = a.row0 + r - tok * a.group;
-    const __half* src = a.q + tok * a.ts + hh * a.hs + piece * (bytes / 2);
-    const int64_t step = per * a.hs, wrap = a.ts - a.group * a.hs;
-    uint32_t dst = smem_u32(tile) + (piece * bytes >> 7) * (kAtQTile / 2) + (r & 127) * 128 + (piece * bytes & 127);
-#pragma unroll 1
+    const uint32_t at = smem_u32(tile) + (piece * bytes >> 7) * (kAtQTile / 2) + (piece * bytes & 15), ch = (piece * bytes >> 4) & 7;
+    const __half* mine = a.q + piece * (bytes / 2);
+#pragma unroll 2
     for (; r < row0 + 32; r += per) {
+      const uint32_t dst = at + (r & 127) * 128 + ((ch ^ (r & 7)) << 4);
       const bool on = r < a.rows;
-      if (wide) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(on ? src : a.q), "r"(on ? 16 : 0) : "memory");
-      else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(on ? src : a.q), "r"(on ? 8 : 0) : "memory");
+      const int tok = fast_div(a.row0 + r, a.group_div), hh = a.row0 + r - tok * a.group;
+      const __half* src = on ? mine + tok * a.ts + hh * a.hs : a.q;
+      if (wide) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
       if (piece == 0) s_pos[r] = on ? a.pos0 + tok : -1;
-      dst += per * 128;
-      src += step;
-      hh += per;
-      while (hh >= a.group) { hh -= a.group; ++tok; src += wrap; }
     }
   }
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
   __syncwarp();
+  // a lane has 64 dimensions of a row, lane ^ 16 the others: one exchange (shuffles are what this would otherwise wait for)
 #pragma unroll 1
-  for (int r = row0 + sub; r < row0 + 32; r += 4) {
-    uint2 raw[4];
-    unsigned char* mine = tile + (l8 >> 2) * (kAtQTile / 2) + (r & 127) * 128 + (l8 & 3) * 32;
+  for (int r = row0 + (lane & 15); r < row0 + 32; r += 16) {
+    unsigned char* mine = tile + (lane >> 4) * (kAtQTile / 2) + (r & 127) * 128;
+    float x[64];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) raw[e] = *reinterpret_cast<const uint2*>(mine + 8 * e);
-    __syncwarp();                                         // the row is read before it is written
-    float x[16];
+    for (int c = 0; c < 8; ++c) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(mine + ((c ^ (r & 7)) << 4));
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw[e].y));
-      x[4 * e] = lo.x; x[4 * e + 1] = lo.y; x[4 * e + 2] = hi.x; x[4 * e + 3] = hi.y;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        x[8 * c + 2 * e] = f.x; x[8 * c + 2 * e + 1] = f.y;
+      }
     }
     if (a.hadamard) {
 #pragma unroll
-      for (int h = 1; h < 16; h <<= 1)
+      for (int h = 1; h < 64; h <<= 1)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int e = 0; e < 64; ++e)
           if ((e & h) == 0) {
-            const float u = x[e], v = x[e + h];
-            x[e] = u + v;
-            x[e + h] = u - v;
+            const float p = x[e], m = x[e + h];
+            x[e] = p + m;
+            x[e + h] = p - m;
           }
-#pragma unroll 1
-      for (int s = 1; s < 8; s <<= 1) {
-        const float sg = (lane & s) ? -1.0f : 1.0f;
+      const float sg = (lane & 16) ? -1.0f : 1.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], sg, __shfl_xor_sync(0xffffffffu, x[e], s));
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = __half2float(__float2half_rn(x[e] * 0.08838834764831845f));
+      for (int e = 0; e < 64; ++e)
+        x[e] = __half2float(__float2half_rn(fmaf(x[e], sg, __shfl_xor_sync(0xffffffffu, x[e], 16)) * 0.08838834764831845f));
     }
-    float part[4];
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
-    float sum = (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-    for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    const int rr = r & 127;
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
+    for (int c = 0; c < 8; ++c) {
       uint32_t h[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const __half2 hv = __floats2half2_rn(x[8 * v + e], x[8 * v + e + 4]);
+        part[e] += x[8 * c + e] + x[8 * c + e + 4];
+        const __half2 hv = __floats2half2_rn(x[8 * c + e], x[8 * c + e + 4]);
         h[e] = *reinterpret_cast<const uint32_t*>(&hv);
       }
-      const int ch = 2 * l8 + v;
-      *reinterpret_cast<uint4*>(tile + (ch >> 3) * (kAtQTile / 2) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(mine + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    if (l8 == 0) s_sum[r] = sum;
+    float sum = (part[0] + part[1]) + (part[2] + part[3]);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    if (lane < 16) s_sum[r] = sum;
   }
 }
 
