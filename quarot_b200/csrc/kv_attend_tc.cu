@@ -184,9 +184,11 @@ __device__ __forceinline__ uint32_t at_centred_pair(uint32_t w, __half2 scale, _
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), scale, bias);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Value parameters of a token.  The weight of a token carries sigma = s' 2^k, its codes 2^-k, with the smallest k >= 0 for
-// which 2^10 / sigma and z' / sigma lie in the range of fp16 (k = 0 unless a row is all but constant or tiny; k <= 23, so
-// that (c - 7.5) 2^-k is exact).
+// Value parameters of a token.  The weight of a token carries sigma = s' 2^k in [1, 2), its codes 2^-k, so that weights compare
+// as the softmax does: with s' itself in them, the weights of tokens with small scales would be rounded at the fp16 numbers'
+// lower end next to a token with a large one.  k lies in -11 .. 23, where (c - 7.5) 2^-k is exact (and 23.5 2^11 finite);
+// scales above 2^12 then give a sigma of up to 4.3.  The centre z' / sigma - 7.5 2^-k is a value of the row over sigma: in
+// the range of fp16 as the row is.
 struct AtValue {
   float sigma, down, z, bad;                              // sigma, 2^-k, z' / sigma - 7.5 2^-k, 0 or NaN
 };
@@ -197,9 +199,7 @@ __device__ __forceinline__ AtValue at_value(uint32_t raw) {
   // scales of a cache are positive; below 2^-22 the codes of a token cannot move an fp16 result by more than 2^-18
   if (!(v.x >= 2.384185791015625e-07f)) v.x = 2.384185791015625e-07f;
   if (r.bad != 0.0f) v = make_float2(1.0f, 0.0f);
-  const float need = __fdividef(fmaxf(0.03125f, fabsf(v.y) * 6.103515625e-05f), v.x);
-  int k = ((__float_as_int(need) + 0x7fffff) >> 23) - 127;
-  k = min(max(k, 0), 23);
+  const int k = max(127 - (__float_as_int(v.x) >> 23), -11);
   r.down = __int_as_float((127 - k) << 23);
   r.sigma = v.x * __int_as_float((127 + k) << 23);
   r.z = fmaf(-7.5f, r.down, __fdividef(v.y, r.sigma));
@@ -989,16 +989,20 @@ static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
   const int64_t blocks = visible_blocks(p, max_rows, kAtTok);
+  // beside its blocks (2.8 us each) a CTA has about 11 us, and 8 us more where there are others to join; where neither the
+  // window nor the pool says how long a unit is, 64 blocks are assumed
+  const double length = (double)(blocks < 64 ? blocks : 64), alone = 4.0 / length, joined = 7.0 / length;
   double cost = 0.0;
-  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, plan->units, blocks, 1.0 / 16,
-                                    2.0 / 16, &p.splits, &cost)) return rc;
+  if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, plan->units, blocks, alone, joined,
+                                    &p.splits, &cost)) return rc;
   // Clusters lie within a GPC and leave SMs over (16 units get 6 CTAs each from them, 9 without), and they split all units
-  // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.
+  // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.  At the same split a second kernel
+  // that joins is no slower than the cluster (64 units in two: 57.4 us both; 32 in four: 40.1 and 42.0).
   const int64_t sms = num_sms(), rounds = plan->units / sms, rest = plan->units % sms;
   int64_t s = rest ? sms / rest : 1;
   if (s > blocks) s = blocks;
   if (s > 32) s = 32;
-  if (s > 1 && rounds * (1.0 + 1.0 / 16) + 1.0 / s + 2.0 / 16 < 0.95 * cost) {
+  if (s > 1 && rounds * (1.0 + alone) + 1.0 / s + joined <= cost) {
     plan->whole = (int)(rounds * sms);
     plan->splits = (int)s;
     plan->bytes = (size_t)(rest * s) * kAtRows * (kHeadDim + 2) * sizeof(float);
