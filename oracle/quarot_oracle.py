@@ -317,7 +317,9 @@ def paged_attention(q, pages, params, layer, kv_indptr, kv_indices, last_page_of
         a change d of weight t moves the result by d (c_t - 7.5).  Or the weights p_t g_t (g_t the scale brought to
         [1, 2), for scales above 2^12 s_t / 2^11), in front of all sums, the denominator among them: with p_t + d_t for p_t,
           sum (p_t + d_t) v_t / sum (p_t + d_t) - o = sum d_t (v_t - o) / (1 + sum d_t),
-        |d_t| <= max(2^-11 p_t, 2^-25 max(p g) / g_t); the larger of the two,
+        |d_t| <= max(2^-11 p_t, 2^-25 max(p g) / g_t); weights cut to 11 bits, p_t (1 - c_t) with 0 <= c_t < 2^-10, are
+        (1 - 2^-11) p_t (1 + d_t / p_t) with |d_t| <= 2^-11 (1 + 2^-10) p_t, and the common factor drops out.  What such an
+        evaluation rounds once more, below 2^-14 of the largest, meets c - 7.5 with 2^-25 of the largest.  The larger of the two,
       * has scores that are off by at most e_t = 2^-19 (31 |s_t| sum|q| + |z_t| |sum q|) / sqrt(d): products of a query with
         codes 16 + c <= 31 summed in fp32 (128 terms and the corrections, each off by 2^-23 of the sum of magnitudes at
         most), which changes weight t by the factor exp(e_t): sum p_t (exp(e_t) - 1) |v_t - o|, twice for the denominator's
@@ -369,8 +371,8 @@ def paged_attention(q, pages, params, layer, kv_indptr, kv_indices, last_page_of
                     rounding = torch.maximum(2.0 ** -11 * w, 2.0 ** -25 * w.max())
                     sv = s.clamp(min=2.0 ** -22)
                     size = sv / 2.0 ** torch.floor(torch.log2(sv)).clamp(max=11)
-                    dp = torch.maximum(2.0 ** -11 * p[:, None], 2.0 ** -25 * (p[:, None] * size).max() / size)
-                    moved = (dp * (v - o).abs()).sum(0) / (1 - dp.sum())
+                    dp = torch.maximum(2.0 ** -11 * (1 + 2.0 ** -10) * p[:, None], 2.0 ** -25 * (p[:, None] * size).max() / size)
+                    moved = (dp * (v - o).abs()).sum(0) / (1 - dp.sum()) + (2.0 ** -25 * w.max() * off).sum(0)
                     bound[r0 + i, e] = ((2.0 ** -11 * o.abs()).clamp(min=2.0 ** -25) + torch.maximum((rounding * off).sum(0), moved)
                                         + 2 * ((p * torch.expm1(es))[:, None] * (v - o).abs()).sum(0) + 2.0 ** -18 * v.abs().max())
     return out, bound

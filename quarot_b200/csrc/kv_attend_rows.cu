@@ -9,12 +9,12 @@
 // and in the output, where the two kinds lie in different registers.
 // Weights: w_t = exp2(score_t + log2 s'_t - M) so that the value scale is inside the weight.  M does not follow the
 // maximum: it is set 1 below the first one and moves, in whole steps, only where a weight would pass 2^15, so that sums
-// are rarely multiplied through and no maximum is looked for across lanes.  Rounding w to fp16 (the B operand of the second
-// product) is a relative error of at most 2^-11 down to 2^-14 of the largest; the sums
-//   l = sum w / s'_t  (the softmax denominator)  and  y = sum w (z'_t / s'_t - 7.5)
-// are of the unrounded w in fp32, and the centre 7.5 of the codes is taken out with the ROUNDED weights (one more MMA
-// row of ones), so that a rounding error of w meets c' - 7.5:
-//   o = (sum w~ c' - 7.5 sum w~ - y) / l.
+// are rarely multiplied through and no maximum is looked for across lanes.  Weights are cut to the 11 bits of fp16 before
+// all sums,
+//   l = sum w / s'_t  (the softmax denominator),   y = sum w (z'_t / s'_t - 7.5),   o = (sum w~ c' - 7.5 sum w~ - y) / l,
+// so that a cut of weight t moves the result by its difference from v_t - o only (a row that looks at one token has
+// nothing of it) and their common part not at all.  l and y are fp32 sums of w; w~ (the B operand) differs from w below
+// 2^-14 of the largest, by at most 2^-25, and meets the centred codes c' - 7.5 with it (sum w~: one more MMA row of ones).
 //
 // Mapping.  A warp takes blocks of 32 tokens.  Scores: S^T = K Q^T with mma.m16n8k16, 16 tokens as M, 8 rows as N; lane
 // (g, c) = (lane / 4, lane % 4) reads 16 bytes of each of its token rows (32 codes), and since the order of the 128
@@ -87,6 +87,8 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+// The 11 leading bits of a weight, those of a normal fp16 number.
+__device__ __forceinline__ float rw_cut(float w) { return __uint_as_float(__float_as_uint(w) & 0xffffe000u); }
 // Row of a block's stage that holds 64 bytes of codes: 16-byte chunk ch of row r lies at chunk ch ^ rw_swz(r).
 __device__ __forceinline__ int rw_swz(int r) { return (r & 2); }
 // Token of a 16-token tile in fragment slot s: the four tokens that a V fragment reads at once, and the two of a K
@@ -385,7 +387,7 @@ kv_attend_rows_kernel(const KvAttendParams p) {
       for (int a = 0; a < TA; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float w0 = ex2(e[a][n][2 * h]), w1 = ex2(e[a][n][2 * h + 1]);
+          const float w0 = rw_cut(ex2(e[a][n][2 * h])), w1 = rw_cut(ex2(e[a][n][2 * h + 1]));
           l[n][0] = fmaf(w0, rv[a][h], l[n][0]); y[n][0] = fmaf(w0, zv[a][h], y[n][0]);
           l[n][1] = fmaf(w1, rv[a][h], l[n][1]); y[n][1] = fmaf(w1, zv[a][h], y[n][1]);
           const __half2 wh = __floats2half2_rn(w0, w1);
