@@ -513,7 +513,7 @@ int kv_ask_fit(KvFit& k, const void* kernel, int threads, size_t smem) {
 }  // namespace
 
 int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
-                   double joined, int* splits, double* cost_out) {
+                   double joined, int* splits, int* resident, double* cost_out) {
   int dev = 0;
   QR_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kKvDevices) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: device %d (at most %d)", dev, kKvDevices - 1);
@@ -522,6 +522,7 @@ int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int6
     if (const int rc = kv_ask_fit(k, kernel, threads, smem)) return rc;
   }
   const int per_sm = k.per_sm.load(std::memory_order_relaxed);
+  *resident = k.fit[1].load(std::memory_order_relaxed);
   double best = 0.0;
   *splits = 1;
   for (int s = 1; s <= 16 && s <= most; ++s) {
@@ -550,13 +551,15 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   if (units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
-  int splits = 1;
+  int splits = 1, resident = 0;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
   // more; where no window says how long a unit is, at most 64 blocks are assumed
   const int64_t blocks = visible_blocks(p, max_rows, kRwTok), parts = (blocks + kWarps - 1) / kWarps;
   const double length = (double)(p.window > 0 || blocks < 64 ? blocks : 64) / kWarps;
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
-                                    smem, units, parts, 2.0 / length, 2.5 / length, &splits)) return rc;
+                                    smem, units, parts, 2.0 / length, 2.5 / length, &splits, &resident)) return rc;
+  // more than one round: the longest sequences first (32 of ragged lengths: 87 us -> 75); a window makes them alike
+  p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && units * splits > resident;
   p.splits = splits;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -2,34 +2,42 @@
 // 5th-generation tensor cores.  Same operator, masks and layouts as kv_attend_rows.cu.
 //
 // One CTA takes up to 256 query rows of one (sequence, KV head) -- row = (new token, query head of the group), so a
-// group shares the tokens it reads -- as two tiles of 128, and walks over the visible tokens in blocks of 128:
-//   S_i = Q_i (16 + Ck)^T          tcgen05.mma 128 x 64 x 128 twice, Q and the key codes in shared memory
+// group shares the tokens it reads -- as two tiles of 128, and walks over the visible tokens in blocks of 96:
+//   S_i = Q_i (16 + Ck)^T          tcgen05.mma 128 x 48 x 128 twice, Q and the key codes in shared memory
 //   P_i = softmax weights          S from tensor memory to registers and back as fp16
-//   O_i += P_i (Cv - 7.5)          P from tensor memory, the value codes, transposed, in shared memory
+//   O_i += P_i Cv                  tcgen05.mma 128 x 144 x 48 twice, P from tensor memory, the value codes in shared memory
 // The tensor cores see the codes, which are exact in fp16, never dequantised keys or values: scales and zero points
-// of a token are folded into its column of S and into its weight, as described in kv_attend_rows.cu:
-//   score_t = s_t S_t - (z_t + 16 s_t) sum(q),   w_t = exp2(score_t + log2 s'_t - M),
-//   l = sum w / s',   y = sum w (z' / s' - 7.5),   o = (O - y) / l,
-// which leaves the fp16 rounding of w as the only one in front of the result's own (7.5 is the centre of the codes: the
-// rounding meets at most 7.5).  M does not follow the maximum: it is set 6 below the first one, so that the largest weight
-// is about 2^6, and moves only where a weight would pass 2^15 (everything summed up is then multiplied through, by powers
-// of two, which round nothing).  So weights are made in one pass, without looking for a maximum first, and the normal
-// fp16 range reaches down to at least 2^-20 of the largest.
+// of a token are folded into its column of S and into its weight.  With s' = sigma 2^-k, sigma in [1, 2),
+//   score_t = s_t S_t - (z_t + 16 s_t) sum(q),   w_t = exp2(score_t + log2 sigma_t - M),   Cv = (c' - 7.5) 2^-k,
+//   l = sum w / sigma,   y = sum w (z' / sigma - 7.5 2^-k),   o = (O - y) / l.
+// l and y are four more rows of the transposed values (128 .. 131: 2^10 / sigma and z' / sigma - .., each as the sum of two
+// fp16 numbers, which is exact to 2^-22), so the same rounded weights are in all sums and the softmax has no sums to make;
+// 144 is the next multiple of 16.  The fp16 rounding of w is the only one in front of the result's own, and a rounding d of
+// weight t moves the result by d (v_t - o) / l.
+// M does not follow the maximum: it is set 1 below the first one and moves, in whole steps, only where a weight would pass
+// 2^15 (all rows of the warp that have grown by 2 move then; what is summed up in tensor memory is multiplied through, by
+// powers of two, which round nothing).  So weights are made in one pass, without looking for a maximum first, and the
+// normal fp16 range reaches down to 2^-14 of the first largest or further.
 //
-// S is made and used in halves of 64 tokens with a buffer each, the weights lie over the half of S they came from: while
+// S is made and used in halves of 48 tokens with a buffer each, the weights lie over the half of S they came from: while
 // the softmax is on one half, the tensor cores make the products of the other and then its next scores.
 //
-// Warps: two warpgroups make the softmax of one row tile each, four warps unpack keys, four unpack values, two issue the
-// MMAs of a row tile each.  A token's
-// five numbers are per COLUMN of S, so a thread that owned a whole row would have to read all of them: S is read
+// Warps: two warpgroups make the softmax of one row tile each, four warps unpack keys and make the numbers of a token, four
+// unpack values, two issue the MMAs of a row tile each.  A token's
+// numbers are per COLUMN of S, so a thread that owned a whole row would have to read all of them: S is read
 // with the 16x256b shape instead, which gives a lane two neighbouring columns of eight in four rows, the numbers of
 // a column pair serve four rows, and a row's maximum is two shuffles away.  Unpacking: keys as they stand (two
 // logical instructions per pair of codes; the query follows their order), values transposed by byte permutes over
 // eight tokens, so that both operands are K-major 128-byte-swizzled tiles written by conflict-free 16-byte stores.
-// Few tiles: a cluster shares the token axis and merges through distributed shared memory.
+// Few tiles: several CTAs share the token axis of a tile and meet in a workspace, or in a cluster where there is none.
 //
 // Registers: 20 warps, five per scheduler, start with 96 each; the softmax warps go up to 160, the unpacking warps down to
 // 64 and the MMA warpgroup to 32 (per scheduler 2 x 160 + 2 x 64 + 32 = 5 x 96).  All waits are bounded (tc_ptx.cuh).
+//
+// Measured (2048 tokens x 64 heads over 10240 tokens, 8 KV heads): 845 us, 733 TFLOP/s.  A block of 96 tokens takes 4900
+// cycles: in each half the softmax of a warp takes 2300 -- 325 until S has arrived, 750 for scores, 760 for weights (exp2
+// alone would take 384 of a scheduler's special function unit per warp, and there are two), 450 waiting -- which is what
+// bounds it; the tensor cores are busy half of the time.  A CTA takes 15000 cycles before its first scores.
 #include "kv_common.cuh"
 #include "tc_ptx.cuh"
 
@@ -215,6 +223,14 @@ __device__ __forceinline__ __half* at_out_row(const KvAttendParams& p, const KvT
   const int row = w.row0 + r;
   const int tok = fast_div(row, p.group_div), hh = row - tok * p.group;
   return p.o + (w.tok0 + tok) * p.o_ts + (int64_t)(head_kv * p.group + hh) * p.o_hs;
+}
+
+// Tile of rows of a unit.  The last tiles of a sequence see the most tokens: they start first.
+__device__ __forceinline__ int at_tile(const KvAttendParams& p, int unit) {
+  const int x = unit / p.kv_heads;
+  if (!p.sorted) return p.max_tiles - 1 - x;
+  const int rank = x / p.tiles_per_seq;
+  return rank * p.tiles_per_seq + p.tiles_per_seq - 1 - (x - rank * p.tiles_per_seq);
 }
 
 // What a lane of a softmax warp keeps of its four rows (g + 8 x of the warp's 32).
@@ -465,8 +481,7 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
   const bool joined = splits > 1, clustered = joined && !p.part;
   if (joined) crank = share % p.splits;                   // also the rank within a cluster
   const int head_kv = unit % p.kv_heads;
-  // the last tiles of a sequence see the most tokens: they start first
-  const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
+  const KvTile w = kv_find_tile(p, at_tile(p, unit), kAtRows, lane);
   if (w.rows == 0) return;                                // the whole cluster has the same tile
   const int tiles = w.rows > 128 ? 2 : 1;
   const int p_min = w.pos0 + fast_div(w.row0, p.group_div), p_max = w.pos0 + fast_div(w.row0 + w.rows - 1, p.group_div);
@@ -942,7 +957,7 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const KvAttendParam
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x / (kAtRows / 8), unit = p.whole + split, r = (blockIdx.x % (kAtRows / 8)) * 8 + warp;
   const int head_kv = unit % p.kv_heads;
-  const KvTile w = kv_find_tile(p, p.max_tiles - 1 - unit / p.kv_heads, kAtRows, lane);
+  const KvTile w = kv_find_tile(p, at_tile(p, unit), kAtRows, lane);
   if (r >= w.rows) return;
   const int cta = split * p.splits;
   const float* stat = p.part + (size_t)(gridDim.x / (kAtRows / 8)) * p.splits * kAtRows * kHeadDim + (size_t)cta * (2 * kAtRows) + r;
@@ -993,8 +1008,10 @@ static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   // window nor the pool says how long a unit is, 64 blocks are assumed
   const double length = (double)(blocks < 64 ? blocks : 64), alone = 4.0 / length, joined = 7.0 / length;
   double cost = 0.0;
+  int resident = 0;
   if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, plan->units, blocks, alone, joined,
-                                    &p.splits, &cost)) return rc;
+                                    &p.splits, &resident, &cost)) return rc;
+  p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && plan->units > resident;
   // Clusters lie within a GPC and leave SMs over (16 units get 6 CTAs each from them, 9 without), and they split all units
   // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.  At the same split a second kernel
   // that joins is no slower than the cluster (64 units in two: 57.4 us both; 32 in four: 40.1 and 42.0).

@@ -119,6 +119,7 @@ struct KvAttendParams {
   int whole;                    // with `part`: units before this one have a CTA each
   int tiles_per_seq;            // > 0: tile index = sequence * tiles_per_seq + tile; 0: found by a search in qo_indptr
   int max_tiles;                // tiles that the grid holds per KV head
+  int sorted;                   // tiles_per_seq > 0, at most 64 sequences: the longest sequences come first
   int* status;
 };
 
@@ -134,12 +135,13 @@ static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, 
 #ifdef __CUDACC__
 // Splitting the token axis of a unit of work (a tile of rows of one KV head) over a cluster of s = 1 .. 16 CTAs.  The cost of
 // s, in parts of a unit, is (rounds of CTAs that an SM goes through) * (1 / s + what a CTA costs beside its share of the
-// tokens); `most` is the number of parts that there are.  `alone` and `joined`: that cost without and with other CTAs to
+// tokens); `most` is the number of parts that there are.
+// `resident`: CTAs that the device holds at once.  `alone` and `joined`: that cost without and with other CTAs to
 // join.  How many clusters fit is asked once per kernel, device and size (clusters lie within a GPC, whose SMs they do not
 // divide evenly: 15 clusters of 8 fit, 16 do not); the kernel's attributes are set then too.
 enum { kKvKernelRows8, kKvKernelRows16, kKvKernelTc, kKvKernels };
 int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int64_t units, int64_t most, double alone,
-                   double joined, int* splits, double* cost = nullptr);
+                   double joined, int* splits, int* resident, double* cost = nullptr);
 
 // fp32 shares [rows][128] (addr(r): the lane's four columns of row r) of the CTAs of a cluster joined into one row, U rows
 // at a time.  Lane x looks at the statistics of CTA x; the first two shares are asked for before that.
@@ -214,39 +216,75 @@ __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile
   KvTile w;
   w.rows = 0; w.b = 0; w.first = 0; w.row0 = 0; w.tok0 = 0; w.seq_len = 0; w.pos0 = 0;
   int j = -1, b = 0;
-  if (p.tiles_per_seq > 0) {
-    b = tile / p.tiles_per_seq;
-    j = tile - b * p.tiles_per_seq;
-  } else {
-    int base = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      const int bb = b0 + lane;
-      int n = 0;
-      if (bb < p.batch) {
-        const long long rows = (long long)(p.qo_indptr[bb + 1] - p.qo_indptr[bb]) * p.group;
-        n = rows > 0 ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
-      }
-      int end = n;
+  int qo0, qo1, first, behind, last;
+  if (p.sorted) {
+    // a lane looks at two sequences and counts the longer ones; the sequence with as many as the tile asks for is the tile's
+    const int rank = tile / p.tiles_per_seq;
+    j = tile - rank * p.tiles_per_seq;
+    int v[2][5], len[2], ahead[2] = {0, 0};
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, end, s);
-        if (lane >= s) end += up;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, base + end > tile);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        b = b0 + src;
-        j = tile - base - (__shfl_sync(0xffffffffu, end, src) - __shfl_sync(0xffffffffu, n, src));
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, end, 31);
+    for (int k = 0; k < 2; ++k) {
+      const int bb = min(lane + 32 * k, p.batch - 1);
+      v[k][0] = p.qo_indptr ? __ldg(p.qo_indptr + bb) : bb;
+      v[k][1] = p.qo_indptr ? __ldg(p.qo_indptr + bb + 1) : bb + 1;
+      v[k][2] = __ldg(p.indptr + bb); v[k][3] = __ldg(p.indptr + bb + 1); v[k][4] = __ldg(p.last_page_offset + bb);
     }
-    if (j < 0) return w;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long long seq = ((long long)v[k][3] - v[k][2] - 1) * p.page_size + v[k][4];
+      // clamped: any order is right
+      len[k] = lane + 32 * k >= p.batch ? -1 : (int)(seq < 0 ? 0 : seq < 0x7fffffffll ? seq : 0x7fffffffll);
+    }
+#pragma unroll 8
+    for (int x = 0; x < 32; ++x) {
+      const int l0 = __shfl_sync(0xffffffffu, len[0], x), l1 = __shfl_sync(0xffffffffu, len[1], x);
+      ahead[0] += (l0 > len[0] || (l0 == len[0] && x < lane)) + (l1 > len[0]);
+      ahead[1] += (l0 >= len[1]) + (l1 > len[1] || (l1 == len[1] && x < lane));
+    }
+    const uint32_t hit0 = __ballot_sync(0xffffffffu, ahead[0] == rank), hit1 = __ballot_sync(0xffffffffu, ahead[1] == rank);
+    const int src = __ffs(hit0 ? hit0 : hit1) - 1;
+    b = hit0 ? src : src + 32;
+    qo0 = __shfl_sync(0xffffffffu, hit0 ? v[0][0] : v[1][0], src);
+    qo1 = __shfl_sync(0xffffffffu, hit0 ? v[0][1] : v[1][1], src);
+    first = __shfl_sync(0xffffffffu, hit0 ? v[0][2] : v[1][2], src);
+    behind = __shfl_sync(0xffffffffu, hit0 ? v[0][3] : v[1][3], src);
+    last = __shfl_sync(0xffffffffu, hit0 ? v[0][4] : v[1][4], src);
+  } else {
+    if (p.tiles_per_seq > 0) {
+      b = tile / p.tiles_per_seq;
+      j = tile - b * p.tiles_per_seq;
+    } else {
+      int base = 0;
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int bb = b0 + lane;
+        int n = 0;
+        if (bb < p.batch) {
+          const long long rows = (long long)(p.qo_indptr[bb + 1] - p.qo_indptr[bb]) * p.group;
+          n = rows > 0 ? (int)((rows + tile_rows - 1) / tile_rows) : 0;
+        }
+        int end = n;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, end, s);
+          if (lane >= s) end += up;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, base + end > tile);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          b = b0 + src;
+          j = tile - base - (__shfl_sync(0xffffffffu, end, src) - __shfl_sync(0xffffffffu, n, src));
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, end, 31);
+      }
+      if (j < 0) return w;
+    }
+    if (b >= p.batch) return w;
+    // one round trip for all of them
+    qo0 = p.qo_indptr ? __ldg(p.qo_indptr + b) : b;
+    qo1 = p.qo_indptr ? __ldg(p.qo_indptr + b + 1) : b + 1;
+    first = __ldg(p.indptr + b); behind = __ldg(p.indptr + b + 1); last = __ldg(p.last_page_offset + b);
   }
-  if (b >= p.batch) return w;
-  // one round trip for all of them
-  const int qo0 = p.qo_indptr ? __ldg(p.qo_indptr + b) : b, qo1 = p.qo_indptr ? __ldg(p.qo_indptr + b + 1) : b + 1;
-  const int first = __ldg(p.indptr + b), behind = __ldg(p.indptr + b + 1), last = __ldg(p.last_page_offset + b);
   const long long tok0 = qo0, len = (long long)qo1 - qo0;
   if (tok0 < 0 || tok0 + len > p.total_q) return w;       // rows beyond q are not touched
   const long long rows = len * p.group, row0 = (long long)j * tile_rows;

@@ -190,3 +190,19 @@ def test_refusals_of_the_c_entry_that_need_a_device():
     o = torch.empty_like(s["q"], device=DEV)
     work = torch.empty(64, dtype=torch.uint8, device=DEV)[8:]
     assert _raw(s, o, 100, work) != 0 and b"16-byte aligned" in ctypes.c_char_p(_lib.lib.qr_last_error()).value
+
+
+@pytest.mark.parametrize("batch,heads,group,new", [(33, 32, 1, 1), (64, 16, 4, 3), (65, 16, 1, 2), (40, 16, 1, 70)])
+def test_more_sequences_than_one_round_in_any_order_of_lengths(batch, heads, group, new):
+    """Sequences are served by length then (up to 64 of them), equal and empty ones among them."""
+    g = torch.Generator().manual_seed(64)
+    lens = (torch.randint(1, 6, (batch,), generator=g) ** 3 + new).tolist()
+    news = [new] * batch
+    lens[1], news[1] = 0, 0
+    s = _setup(lens, news, heads, group, 16, seed=65)
+    few = dict(s)                                                   # the oracle looks at four KV heads
+    pick = [0, 1, heads // 2, heads - 1]
+    few["pages"], few["params"] = s["pages"][:, :, :, pick], s["params"][:, :, :, pick]
+    cols = [h * group + e for h in pick for e in range(group)]
+    few["q"] = s["q"][:, cols]
+    _check(_attend(s, max_q=new)[:, cols], _oracle(few))
