@@ -78,7 +78,7 @@ template <int N>
 __device__ __forceinline__ void rw_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -288,29 +288,32 @@ kv_attend_rows_kernel(const KvAttendParams p) {
     }
     __syncwarp();
     float s[TA][NT][4];
+    uint4 xk[TA], zk[TA];
 #pragma unroll
     for (int a = 0; a < TA; ++a) {
       // fragment rows g and g + 8: tokens tau and 8 + tau of the tile
       const unsigned char* sk = st + (16 * a + tau) * 64 + ((c ^ rw_swz(tau)) << 4);
-      const uint4 x = *reinterpret_cast<const uint4*>(sk);
-      const uint4 z = *reinterpret_cast<const uint4*>(sk + 8 * 64);
+      xk[a] = *reinterpret_cast<const uint4*>(sk);
+      zk[a] = *reinterpret_cast<const uint4*>(sk + 8 * 64);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[a][n][e] = 0.0f;
-      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, zw[4] = {z.x, z.y, z.z, z.w};
+    }
 #pragma unroll
-      for (int wi = 0; wi < 4; ++wi) {
-        const uint32_t xh = xw[wi] >> 8, zh = zw[wi] >> 8;
-        const uint32_t f0 = xw[wi] & kRwLow, f1 = zw[wi] & kRwLow, f2 = xw[wi] & kRwHigh, f3 = zw[wi] & kRwHigh;
+    for (int wi = 0; wi < 4; ++wi)
+#pragma unroll
+      for (int a = 0; a < TA; ++a) {
+        const uint32_t xw = wi == 0 ? xk[a].x : wi == 1 ? xk[a].y : wi == 2 ? xk[a].z : xk[a].w;
+        const uint32_t zw = wi == 0 ? zk[a].x : wi == 1 ? zk[a].y : wi == 2 ? zk[a].z : zk[a].w;
+        const uint32_t xh = xw >> 8, zh = zw >> 8;
+        const uint32_t f0 = xw & kRwLow, f1 = zw & kRwLow, f2 = xw & kRwHigh, f3 = zw & kRwHigh;
         const uint32_t h0 = xh & kRwLow, h1 = zh & kRwLow, h2 = xh & kRwHigh, h3 = zh & kRwHigh;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_f16(s[a][n], f0, f1, f2, f3, qf[n][4 * wi], qf[n][4 * wi + 1]);
-          mma_f16(s[a][n], h0, h1, h2, h3, qf[n][4 * wi + 2], qf[n][4 * wi + 3]);
-        }
+        for (int n = 0; n < NT; ++n) mma_f16(s[a][n], f0, f1, f2, f3, qf[n][4 * wi], qf[n][4 * wi + 1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[a][n], h0, h1, h2, h3, qf[n][4 * wi + 2], qf[n][4 * wi + 3]);
       }
-    }
     float rv[TA][2], zv[TA][2];                         // 1 / s', z' / s' - 7.5 of the lane's tokens
     float e[TA][NT][4];                                 // exponents relative to M
     float top = -INFINITY;
