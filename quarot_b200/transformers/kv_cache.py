@@ -216,6 +216,7 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
         raise RuntimeError("%s: window must be positive (None: no window), sink_tokens not negative" % op)
     batch = last_page_offset.shape[0]
     window, sink_tokens = min(int(window), 0x7fffffff) if window else 0, min(int(sink_tokens), 0x7fffffff)
+    indptr = _check_i32(op, dev, "kv_indptr", kv_indptr, batch + 1)
     # the shares of CTAs that meet in memory; decode-sized calls have none
     work = None
     if max_q_len * heads > 64 * kv_heads:
@@ -224,7 +225,7 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
         if nbytes:
             work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(op, dev, _lib_c.qr_kv_attend_i4, o_p, ot, oh, q_p, qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), pages,
-            _check_i32(op, dev, "kv_indptr", kv_indptr, batch + 1), _check_i32(op, dev, "kv_indices", kv_indices, 0),
+            indptr, _check_i32(op, dev, "kv_indices", kv_indices, 0) or indptr,            # no page at all: not read
             _check_i32(op, dev, "last_page_offset", last_page_offset, batch), _check_i32(op, dev, "qo_indptr", qo_indptr, batch + 1),
             tokens, max_q_len, batch, layers, layer_idx, heads, kv_heads, page_size, 128, window, sink_tokens,
             1 if hadamard_q else 0, work.data_ptr() if work is not None else None, work.numel() if work is not None else 0)

@@ -206,3 +206,10 @@ def test_more_sequences_than_one_round_in_any_order_of_lengths(batch, heads, gro
     cols = [h * group + e for h in pick for e in range(group)]
     few["q"] = s["q"][:, cols]
     _check(_attend(s, max_q=new)[:, cols], _oracle(few))
+
+
+@pytest.mark.parametrize("new", [[2, 1], [80, 3]])
+def test_no_sequence_has_a_page(new):
+    s = _setup([0, 0], new, 1, 2, 16, seed=66)
+    assert s["indices"].numel() == 0
+    assert bool((_attend(s, max_q=max(new)) == 0).all())
