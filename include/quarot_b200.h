@@ -299,7 +299,8 @@ int qr_kv_page_table(const int32_t* seq_lens, const int32_t* new_lens, int batch
                      int64_t* slot_map, int32_t* positions, int32_t* seq_lens_out, int32_t* status, void* stream);
 
 /* qr_kv_append_slots_i4: qr_kv_append_i4 with the page slots taken from a slot map (qr_kv_page_table): the same bytes in
- * the same places.  A token whose slot lies outside the pool (-1 among others) is left out.  k and v [tokens, heads,
+ * the same places.  A token whose slot lies outside the pool (-1 among others) is left out; the slots of the others have
+ * to differ (of two tokens with one slot either may win, codes and parameters apart).  k and v [tokens, heads,
  * head_dim] fp16 with strides in elements (multiples of 4; the last axis is contiguous, 8-byte aligned). */
 int qr_kv_append_slots_i4(void* kv_data, void* kv_param, int64_t num_pages, const int64_t* slot_map, const void* k,
                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,

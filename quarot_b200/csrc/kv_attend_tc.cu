@@ -1014,12 +1014,13 @@ static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && plan->units > resident;
   // Clusters lie within a GPC and leave SMs over (16 units get 6 CTAs each from them, 9 without), and they split all units
   // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.  At the same split a second kernel
-  // that joins is no slower than the cluster (64 units in two: 57.4 us both; 32 in four: 40.1 and 42.0).
+  // that joins is no slower than the cluster (32 units in four: 40.1 and 42.0 us) unless there are but two (64 units: 59 and 60).
   const int64_t sms = num_sms(), rounds = plan->units / sms, rest = plan->units % sms;
   int64_t s = rest ? sms / rest : 1;
   if (s > blocks) s = blocks;
   if (s > 32) s = 32;
-  if (s > 1 && rounds * (1.0 + alone) + 1.0 / s + joined <= cost) {
+  const double here = rounds * (1.0 + alone) + 1.0 / s + joined;
+  if (s > 1 && (here < 0.999 * cost || (s > 2 && here <= cost))) {
     plan->whole = (int)(rounds * sms);
     plan->splits = (int)s;
     plan->bytes = (size_t)(rest * s) * kAtRows * (kHeadDim + 2) * sizeof(float);

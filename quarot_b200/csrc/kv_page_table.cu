@@ -12,6 +12,8 @@
 // memory) and then takes its share of the flat list of outputs; an entry finds its sequence by a binary search in
 // shared memory, 128 to 512 entries of kv_indices per search.  A new page is read from the free list by everyone, never from
 // the block table, whose new entries are written in the same launch: no CTA waits for another.
+// Measured: 16 requests 6.2 us, 2048 requests with 9 MB of table entries 12.6 us (3.4 us at the copy rate): latency of chained
+// reads and scans; a call from Python takes 18 us, a dozen torch operations for the same 600 us.
 #include "kv_common.cuh"
 
 namespace qr {

@@ -183,7 +183,8 @@ def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None
 
 def append_kv_slots_i4(kv_data, kv_param, slot_map, k, v, layer_idx, hadamard_k=True):
     """append_kv_i4 with the page slots from a slot map (build_page_table): slot_map int64 [tokens], k and v fp16 [tokens,
-    heads, 128] (strided views are fine).  Tokens whose slot lies outside the pool, -1 among others, are left out."""
+    heads, 128] (strided views are fine).  Tokens whose slot lies outside the pool, -1 among others, are left out; the other
+    slots have to differ."""
     op = "append_kv_slots_i4"
     layer_idx = int(layer_idx)
     dev, (pages, layers, _, heads, page_size, _) = _check_pages(op, kv_data, kv_param, layer_idx)
