@@ -89,7 +89,7 @@ def _check_i32(op, dev, name, t, n):
         return None
     if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
         raise RuntimeError("%s: %s must be a contiguous int32 tensor on %s" % (op, name, dev))
-    if t.numel() < n:
+    if n and t.numel() < n:
         raise RuntimeError("%s: %s has %d entries, %d are needed" % (op, name, t.numel(), n))
     return t.data_ptr()
 
@@ -101,9 +101,9 @@ def _check_pages(op, kv_data, kv_param, layer_idx):
         raise RuntimeError("%s: the pages and their parameters must be contiguous tensors on one CUDA device" % op)
     if kv_data.dtype is not torch.uint8 or kv_param.dtype is not torch.float16:
         raise RuntimeError("%s: the pages are uint8 and their parameters fp16" % op)
-    shape = tuple(kv_data.shape)
-    if len(shape) != 6 or shape[2] != 2 or tuple(kv_param.shape) != shape[:5] + (2,):
-        raise RuntimeError("%s: pages %s and parameters %s do not belong together" % (op, shape, tuple(kv_param.shape)))
+    shape = kv_data.shape
+    if len(shape) != 6 or shape[2] != 2 or kv_param.shape != shape[:5] + (2,):
+        raise RuntimeError("%s: pages %s and parameters %s do not belong together" % (op, tuple(shape), tuple(kv_param.shape)))
     if shape[5] != 64:
         raise RuntimeError("%s: head_dim must be 128" % op)
     if not 0 <= layer_idx < shape[1]:
@@ -112,7 +112,7 @@ def _check_pages(op, kv_data, kv_param, layer_idx):
 
 
 def _check_rows(op, dev, name, t):
-    """[tokens, heads, 128] fp16 on dev, last axis contiguous; address, strides of the other two."""
+    """[tokens, heads, 128] fp16 on dev, last axis contiguous; address, strides of the other two, shape."""
     shape = t.shape
     if t.dtype is not torch.float16 or t.device != dev or len(shape) != 3 or shape[2] != 128:
         raise RuntimeError("%s: %s must be fp16 [tokens, heads, 128] on %s" % (op, name, dev))
@@ -121,7 +121,7 @@ def _check_rows(op, dev, name, t):
     at = t.data_ptr()
     if (ds != 1 or ts % 4 or hs % 4 or at % 8) and t.numel():
         raise RuntimeError("%s: %s needs a contiguous last axis, 8-byte alignment and strides that are multiples of 4" % (op, name))
-    return at, ts, hs
+    return at, ts, hs, shape
 
 
 def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, free_pages=None, max_blocks=None):
@@ -188,11 +188,11 @@ def append_kv_slots_i4(kv_data, kv_param, slot_map, k, v, layer_idx, hadamard_k=
     op = "append_kv_slots_i4"
     layer_idx = int(layer_idx)
     dev, (pages, layers, _, heads, page_size, _) = _check_pages(op, kv_data, kv_param, layer_idx)
-    k_p, kt, kh = _check_rows(op, dev, "k", k)
-    v_p, vt, vh = _check_rows(op, dev, "v", v)
-    tokens = k.shape[0]
-    if k.shape != v.shape or k.shape[1] != heads:
-        raise RuntimeError("%s: k %s and v %s over %d heads" % (op, tuple(k.shape), tuple(v.shape), heads))
+    k_p, kt, kh, shape = _check_rows(op, dev, "k", k)
+    v_p, vt, vh, v_shape = _check_rows(op, dev, "v", v)
+    tokens = shape[0]
+    if shape != v_shape or shape[1] != heads:
+        raise RuntimeError("%s: k %s and v %s over %d heads" % (op, tuple(shape), tuple(v_shape), heads))
     if slot_map.dtype is not torch.int64 or slot_map.device != dev or not slot_map.is_contiguous() or slot_map.numel() != tokens:
         raise RuntimeError("%s: slot_map must be contiguous int64 on %s with one entry per token" % (op, dev))
     _launch(op, dev, _lib_c.qr_kv_append_slots_i4, kv_data.data_ptr(), kv_param.data_ptr(), pages, slot_map.data_ptr(), k_p, kt, kh,
@@ -203,11 +203,11 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
                window, sink_tokens):
     layer_idx = int(layer_idx)
     dev, (pages, layers, _, kv_heads, page_size, _) = _check_pages(op, kv_data, kv_param, layer_idx)
-    q_p, qt, qh = _check_rows(op, dev, "q", q)
-    o_p, ot, oh = _check_rows(op, dev, "o", o)
-    if o.shape != q.shape:
-        raise RuntimeError("%s: o %s, q %s" % (op, tuple(o.shape), tuple(q.shape)))
-    tokens, heads, _ = q.shape
+    q_p, qt, qh, shape = _check_rows(op, dev, "q", q)
+    o_p, ot, oh, o_shape = _check_rows(op, dev, "o", o)
+    if o_shape != shape:
+        raise RuntimeError("%s: o %s, q %s" % (op, tuple(o_shape), tuple(shape)))
+    tokens, heads, _ = shape
     if not ((heads < 2 or oh >= 128) and (tokens < 2 or ot >= 128) and
             (heads < 2 or tokens < 2 or ot >= oh * heads or oh >= ot * tokens)):
         raise RuntimeError("%s: the rows of o overlap" % op)
@@ -221,8 +221,12 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
     # the shares of CTAs that meet in memory; decode-sized calls have none
     work = None
     if max_q_len * heads > 64 * kv_heads:
-        with torch.cuda.device(dev):
-            nbytes = _lib_c.qr_kv_attend_workspace_bytes(pages, page_size, tokens, max_q_len, batch, heads, kv_heads, window, sink_tokens)
+        sizes = (pages, page_size, tokens, max_q_len, batch, heads, kv_heads, window, sink_tokens)
+        if torch.cuda.current_device() == dev.index:
+            nbytes = _lib_c.qr_kv_attend_workspace_bytes(*sizes)
+        else:
+            with torch.cuda.device(dev):
+                nbytes = _lib_c.qr_kv_attend_workspace_bytes(*sizes)
         if nbytes:
             work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(op, dev, _lib_c.qr_kv_attend_i4, o_p, ot, oh, q_p, qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), pages,
@@ -255,13 +259,14 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
     """o[b, h] = softmax(q[b, h] K^T / sqrt(d)) V over the packed pages, one new token per sequence
     (quarot/transformers/kv_cache.py:64-72); with hadamard_q the query is Hadamard-transformed first.  With a window only
     the last `window` tokens and the first sink_tokens are seen; the query may have a multiple of the cache's heads."""
-    if window is not None or q.dim() == 3 and q.shape[1] != kv_data.shape[3]:
-        if q.shape[0] != last_page_offset.shape[0]:
-            raise RuntimeError("batch_decode_i4: %d queries for %d sequences" % (q.shape[0], last_page_offset.shape[0]))
+    shape = q.shape
+    if window is not None or len(shape) == 3 and shape[1] != kv_data.shape[3]:
+        if shape[0] != last_page_offset.shape[0]:
+            raise RuntimeError("batch_decode_i4: %d queries for %d sequences" % (shape[0], last_page_offset.shape[0]))
         return _attend_i4("batch_decode_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, None, 1, layer_idx,
                           hadamard_q, window, sink_tokens)
-    batch, heads, head_dim = q.shape
-    assert o.shape == q.shape and q.dtype == o.dtype == torch.float16 and q.is_contiguous() and o.is_contiguous()
+    batch, heads, head_dim = shape
+    assert o.shape == shape and q.dtype == o.dtype == torch.float16 and q.is_contiguous() and o.is_contiguous()
     dev = kv_data.device
     with torch.cuda.device(dev):
         _lib.check(_lib_c.qr_kv_decode_i4(
