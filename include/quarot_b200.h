@@ -316,13 +316,16 @@ int qr_kv_append_slots_i4(void* kv_data, void* kv_param, int64_t num_pages, cons
  *   aligned); total_q rows exist, a sequence whose rows lie beyond them is left out, as are rows that belong to none.
  *   max_q_len: an upper bound of the new tokens of any sequence (it sets the grid and chooses the kernel; rows of a
  *   sequence beyond it may be left unwritten).  kv_indices outside 0 .. num_pages - 1 read the last page.
+ *   num_indices: entries of kv_indices; none beyond them is read, whatever kv_indptr says.  The grid is made for sequences
+ *   that share them evenly.
  *   hadamard_q: the query is Walsh-Hadamard transformed (and rounded to fp16) first.
  * Scales are positive, as qr_kv_append_i4 writes them; what lies in tokens that a row does not see, infinities and NaN
  * among it, does not reach it.  The sums are in fp32; the softmax weights, with the value scale in them, are rounded to
  * fp16 for the tensor cores, the codes are exact.  Same result from call to call. */
 int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, const void* q, int64_t q_token_stride,
                     int64_t q_head_stride, const void* kv_data, const void* kv_param, int64_t num_pages,
-                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_offset,
+                    const int32_t* kv_indptr, const int32_t* kv_indices, int64_t num_indices,
+                    const int32_t* last_page_offset,
                     const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
                     int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
                     int hadamard_q, void* workspace, size_t workspace_bytes, void* stream);
@@ -331,7 +334,7 @@ int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, cons
  * rows meet in memory instead of in a cluster); 0 where it needs none.  The workspace is 16-byte
  * aligned device memory of any content that no other work uses at the same time; without it (NULL, or fewer bytes) the call
  * is slower and rounds differently in the last bits. */
-size_t qr_kv_attend_workspace_bytes(int64_t num_pages, int page_size, int64_t total_q, int64_t max_q_len, int batch,
+size_t qr_kv_attend_workspace_bytes(int64_t num_indices, int page_size, int64_t total_q, int64_t max_q_len, int batch,
                                     int num_q_heads, int num_kv_heads, int window, int sink_tokens);
 
 #ifdef __cplusplus

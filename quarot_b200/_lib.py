@@ -41,7 +41,7 @@ SIGNATURES = {
     "qr_kv_decode_i4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _vp]),
     "qr_kv_page_table": (_int, [_vp, _vp, _int, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "qr_kv_append_slots_i4": (_int, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _int, _int, _int, _int, _int, _int, _vp]),
-    "qr_kv_attend_i4": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int,
+    "qr_kv_attend_i4": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _int, _int, _int,
                                _int, _int, _int, _int, _int, _int, _int, _vp, ctypes.c_size_t, _vp]),
     "qr_kv_attend_workspace_bytes": (ctypes.c_size_t, [_i64, _int, _i64, _i64, _int, _int, _int, _int, _int]),
     "qr_linear_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),

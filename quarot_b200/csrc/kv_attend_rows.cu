@@ -543,8 +543,9 @@ int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int6
   return QR_OK;
 }
 
+// Tiles and split of a call; the cost of kv_pick_splits.
 template <int NT>
-static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
+static int plan_rows(KvAttendParams& p, int64_t max_rows, int64_t* units, double* cost) {
   constexpr int R = 8 * NT, kWarps = RwConfig<NT>::kWarps;
   constexpr size_t smem = RwConfig<NT>::kRing + sizeof(RwShared<NT>);
   static_assert(kWarps * R * kRwORow * sizeof(float) <= RwConfig<NT>::kRing, "the merge buffer lies in the ring");
@@ -553,20 +554,40 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   const int64_t per_seq = (max_rows + R - 1) / R;
   const int64_t bound = p.total_q * p.group / R + p.batch;
   const bool uniform = !p.qo_indptr || p.batch * per_seq <= 2 * bound;
-  const int64_t tiles = uniform ? p.batch * per_seq : bound, units = tiles * p.kv_heads;
-  if (units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
+  const int64_t tiles = uniform ? p.batch * per_seq : bound;
+  *units = tiles * p.kv_heads;
+  if (*units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
-  int splits = 1, resident = 0;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
-  // more; where no window says how long a unit is, at most 64 blocks are assumed
-  const int64_t blocks = visible_blocks(p, max_rows, kRwTok), parts = (blocks + kWarps - 1) / kWarps;
-  const double length = (double)(p.window > 0 || blocks < 64 ? blocks : 64) / kWarps;
+  // more; a list of pages much longer than what the sequences use must not lead to splits that only pay for such lengths
+  const int64_t blocks = visible_blocks(p, max_rows, kRwTok, false), evenly = visible_blocks(p, max_rows, kRwTok, true);
+  const double length = (double)(evenly < 256 ? evenly : 256) / kWarps;
+  int resident = 0;
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
-                                    smem, units, parts, 2.0 / length, 2.5 / length, &splits, &resident)) return rc;
+                                    smem, *units, (blocks + kWarps - 1) / kWarps, 2.0 / length, 2.5 / length, &p.splits, &resident,
+                                    cost)) return rc;
   // more than one round: the longest sequences first (32 of ragged lengths: 87 us -> 75); a window makes them alike
-  p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && units * splits > resident;
-  p.splits = splits;
+  p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && *units * p.splits > resident;
+  return QR_OK;
+}
+
+int kv_attend_rows_time(const KvAttendParams& p, int64_t max_rows, double* us) {
+  KvAttendParams c = p;
+  int64_t units = 0;
+  double cost = 0.0;
+  if (const int rc = plan_rows<2>(c, max_rows, &units, &cost)) return rc;
+  *us = 5.0 + cost * (double)visible_blocks(c, max_rows, kRwTok, true) * 0.425;      // 13.3 ns per token of a unit
+  return QR_OK;
+}
+
+template <int NT>
+static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
+  constexpr int kWarps = RwConfig<NT>::kWarps;
+  constexpr size_t smem = RwConfig<NT>::kRing + sizeof(RwShared<NT>);
+  int64_t units = 0;
+  if (const int rc = plan_rows<NT>(p, max_rows, &units, nullptr)) return rc;
+  const int splits = p.splits;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -588,16 +609,32 @@ int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) 
   return launch_rows<2>(p, max_rows, st);
 }
 
+// Which kernel: mma.sync, 16 rows at a time, or tcgen05, 256 rows at a time at a cost that hardly depends on the rows and
+// with 11 us (18 where CTAs are joined) beside the tokens.  Measured, us in the one and in the other:
+//   32 sequences of 8192 tokens, 8 KV heads: 32 rows 194 and 378, 48 rows 289 and 378, 64 rows 382 and 378, 96 rows 569 and 379;
+//   one sequence, 8 KV heads, 128 rows: 300 tokens 11 and 23, 4000 tokens 22 and 28, 16000 tokens 55 and 41; 256 rows: 13 and 25,
+//   33 and 32, 99 and 47.
+// Up to 64 rows the first is never much behind; above, the estimates decide (both within about 15 % of the figures above).
+static int kv_pick_kernel(const KvAttendParams& p, int64_t rows, bool* tc, size_t* bytes) {
+  *tc = false;
+  if (g_tuning.kv_attend == 1 || (g_tuning.kv_attend == 0 && rows <= 64)) return QR_OK;
+  double a = 0.0, b = 0.0;
+  if (const int rc = kv_attend_tc_time(p, rows, &b, bytes)) return rc;
+  // more tiles than the first kernel's grid may have: the second takes them
+  *tc = g_tuning.kv_attend == 2 || kv_attend_rows_time(p, rows, &a) != QR_OK || b < a;
+  return QR_OK;
+}
+
 }  // namespace qr
 
 extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, const void* q, int64_t q_token_stride,
                                int64_t q_head_stride, const void* kv_data, const void* kv_param, int64_t num_pages,
-                               const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_offset,
-                               const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
+                               const int32_t* kv_indptr, const int32_t* kv_indices, int64_t num_indices,
+                               const int32_t* last_page_offset, const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
                                int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
                                int hadamard_q, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace qr;
-  if (batch < 0 || total_q < 0 || max_q_len < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative size");
+  if (batch < 0 || total_q < 0 || max_q_len < 0 || num_indices < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative size");
   if (batch == 0 || total_q == 0 || max_q_len == 0) return QR_OK;
   if (!o || !q || !kv_data || !kv_param || !kv_indptr || !kv_indices || !last_page_offset)
     return fail(QR_EINVAL, "qr_kv_attend_i4: null pointer");
@@ -625,28 +662,27 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
   p.indptr = kv_indptr; p.indices = kv_indices; p.last_page_offset = last_page_offset; p.qo_indptr = qo_indptr;
   p.q_ts = q_token_stride; p.q_hs = q_head_stride; p.o_ts = o_token_stride; p.o_hs = o_head_stride;
   p.total_q = total_q; p.batch = batch; p.layers = num_layers; p.layer = layer; p.kv_heads = num_kv_heads; p.group = group;
-  p.page_size = page_size; p.num_pages = num_pages;
+  p.page_size = page_size; p.num_pages = num_pages; p.num_indices = num_indices < 0x7fffffff ? num_indices : 0x7fffffff;
   p.page_div = make_fastdiv((uint32_t)page_size); p.group_div = make_fastdiv((uint32_t)group);
   p.window = window; p.sinks = window > 0 ? sink_tokens : 0; p.hadamard_q = hadamard_q;
   p.status = kernel_status_ptr();
-  // Up to 64 rows per KV head: mma.sync, 16 rows at a time; above: tcgen05, 256 rows at a time, at a cost that hardly depends
-  // on the rows.  32 sequences of 8192 tokens, 8 KV heads: 32 rows 194 us here, 378 there; 48 rows 289 and 378; 64 rows 382
-  // and 378; 96 rows 569 and 379.  One sequence of 16384 tokens: 64 rows 33 and 51, 96 rows 46 and 53.
   const int64_t rows = max_q_len * group;
-  return rows > kKvRowsMost ? launch_kv_attend_tc(p, rows, workspace, workspace_bytes, (cudaStream_t)stream)
-                            : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
+  bool tc = false;
+  size_t bytes = 0;
+  if (const int rc = kv_pick_kernel(p, rows, &tc, &bytes)) return rc;
+  return tc ? launch_kv_attend_tc(p, rows, workspace, workspace_bytes, (cudaStream_t)stream) : launch_kv_attend_rows(p, rows, (cudaStream_t)stream);
 }
 
-extern "C" size_t qr_kv_attend_workspace_bytes(int64_t num_pages, int page_size, int64_t total_q, int64_t max_q_len, int batch,
+extern "C" size_t qr_kv_attend_workspace_bytes(int64_t num_indices, int page_size, int64_t total_q, int64_t max_q_len, int batch,
                                                int num_q_heads, int num_kv_heads, int window, int sink_tokens) {
   using namespace qr;
-  if (num_pages < 1 || page_size < 1 || total_q < 1 || max_q_len < 1 || batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads ||
+  if (num_indices < 0 || page_size < 1 || total_q < 1 || max_q_len < 1 || batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads ||
       num_q_heads % num_kv_heads || window < 0 || sink_tokens < 0 || max_q_len > total_q)
     return 0;
   KvAttendParams p = {};
-  p.num_pages = num_pages; p.page_size = page_size; p.total_q = total_q; p.batch = batch; p.kv_heads = num_kv_heads;
+  p.num_indices = num_indices < 0x7fffffff ? num_indices : 0x7fffffff; p.page_size = page_size; p.total_q = total_q; p.batch = batch; p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads; p.window = window; p.sinks = window > 0 ? sink_tokens : 0;
+  bool tc = false;
   size_t bytes = 0;
-  if (max_q_len * p.group <= kKvRowsMost || kv_attend_tc_workspace(p, max_q_len * p.group, &bytes) != QR_OK) return 0;
-  return bytes;
+  return kv_pick_kernel(p, max_q_len * p.group, &tc, &bytes) == QR_OK && tc ? bytes : 0;
 }

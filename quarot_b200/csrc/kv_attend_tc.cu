@@ -992,6 +992,7 @@ struct AtPlan {
   int64_t units;
   int whole, splits;                                      // with memory to meet in
   size_t bytes;                                           // 0: of no use
+  double cost;                                            // of the better way, in parts of a unit and SM
 };
 static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   const int64_t per_seq = (max_rows + kAtRows - 1) / kAtRows;
@@ -1003,15 +1004,15 @@ static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
   if (plan->units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
-  const int64_t blocks = visible_blocks(p, max_rows, kAtTok);
-  // beside its blocks (2.8 us each) a CTA has about 11 us, and 8 us more where there are others to join; where neither the
-  // window nor the pool says how long a unit is, 64 blocks are assumed
-  const double length = (double)(blocks < 64 ? blocks : 64), alone = 4.0 / length, joined = 7.0 / length;
+  // beside its blocks a CTA has about four blocks' time, and three more where there are others to join
+  const int64_t blocks = visible_blocks(p, max_rows, kAtTok, false);
+  const double length = (double)visible_blocks(p, max_rows, kAtTok, true), alone = 4.0 / length, joined = 7.0 / length;
   double cost = 0.0;
   int resident = 0;
   if (const int rc = kv_pick_splits(kKvKernelTc, (const void*)kv_attend_tc_kernel, kAtThreads, kAtSmem, plan->units, blocks, alone, joined,
                                     &p.splits, &resident, &cost)) return rc;
   p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && plan->units > resident;
+  plan->cost = cost;
   // Clusters lie within a GPC and leave SMs over (16 units get 6 CTAs each from them, 9 without), and they split all units
   // alike.  Here full rounds of units have an SM each, what is left over shares all SMs.  At the same split a second kernel
   // that joins is no slower than the cluster (32 units in four: 40.1 and 42.0 us) unless there are but two (64 units: 59 and 60).
@@ -1024,15 +1025,18 @@ static int at_plan(KvAttendParams& p, int64_t max_rows, AtPlan* plan) {
     plan->whole = (int)(rounds * sms);
     plan->splits = (int)s;
     plan->bytes = (size_t)(rest * s) * kAtRows * (kHeadDim + 2) * sizeof(float);
+    plan->cost = here;
   }
   return QR_OK;
 }
 
-int kv_attend_tc_workspace(KvAttendParams& p, int64_t max_rows, size_t* bytes) {
+int kv_attend_tc_time(const KvAttendParams& p, int64_t max_rows, double* us, size_t* bytes) {
+  KvAttendParams c = p;
   AtPlan plan = {};
-  const int rc = at_plan(p, max_rows, &plan);
+  if (const int rc = at_plan(c, max_rows, &plan)) return rc;
+  *us = 3.0 + plan.cost * (double)visible_blocks(c, max_rows, kAtTok, true) * (max_rows <= 128 ? 2.3 : 2.6);
   *bytes = plan.bytes;
-  return rc;
+  return QR_OK;
 }
 
 int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, size_t workspace_bytes, cudaStream_t st) {

@@ -110,7 +110,7 @@ struct KvAttendParams {
   int64_t q_ts, q_hs, o_ts, o_hs;   // strides in elements between tokens and between heads
   int64_t total_q;
   int batch, layers, layer, kv_heads, group, page_size;
-  int64_t num_pages;
+  int64_t num_pages, num_indices;   // pages of the pool, entries of indices
   FastDiv page_div, group_div;
   int window, sinks;            // window 0: none
   int hadamard_q;
@@ -123,13 +123,14 @@ struct KvAttendParams {
   int* status;
 };
 
-// Upper bound of the blocks of T tokens that a tile of rows sees, from the window and the pool (a page that is listed more
-// than once for a sequence may lead beyond it; only the split suffers).
-static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, int T) {
-  const int64_t pool = (p.num_pages * p.page_size + T - 1) / T;
-  if (p.window <= 0) return pool;
+// Blocks of T tokens that a tile of rows sees: at most (`all` entries of the page list), or as many as each of the
+// sequences has where they share the list evenly.
+static inline int64_t visible_blocks(const KvAttendParams& p, int64_t max_rows, int T, bool evenly) {
+  const int64_t pages = evenly ? (p.num_indices + p.batch - 1) / p.batch : p.num_indices;
+  const int64_t all = (pages * p.page_size + T - 1) / T;
+  if (p.window <= 0) return all > 0 ? all : 1;
   const int64_t seen = ((int64_t)p.window + max_rows / p.group + T - 1) / T + 1 + ((int64_t)p.sinks + T - 1) / T;
-  return seen < pool ? seen : pool;
+  return seen < all ? seen : all > 0 ? all : 1;
 }
 
 #ifdef __CUDACC__
@@ -289,8 +290,9 @@ __device__ __forceinline__ KvTile kv_find_tile(const KvAttendParams& p, int tile
   if (tok0 < 0 || tok0 + len > p.total_q) return w;       // rows beyond q are not touched
   const long long rows = len * p.group, row0 = (long long)j * tile_rows;
   if (row0 >= rows) return w;
-  // not beyond the pages that are listed, whatever the last page's offset says
-  const long long listed = ((long long)behind - first) * p.page_size;
+  // not beyond the pages that are listed, whatever kv_indptr and the last page's offset say
+  const long long pages = first < 0 ? 0 : (behind < p.num_indices ? behind : p.num_indices) - first;
+  const long long listed = pages * p.page_size;
   long long seq = listed - p.page_size + last;
   if (seq > listed) seq = listed;
   if (seq > kKvMostTokens) return w;                      // tokens are counted in 32 bits
@@ -332,7 +334,8 @@ __device__ __forceinline__ int kv_block_index(const KvBlocks& k, int i) {
 
 int launch_kv_attend_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st);
 int launch_kv_attend_tc(KvAttendParams& p, int64_t max_rows, void* workspace, size_t workspace_bytes, cudaStream_t st);
-int kv_attend_tc_workspace(KvAttendParams& p, int64_t max_rows, size_t* bytes);
-constexpr int64_t kKvRowsMost = 64;   // query rows per KV head up to which the mma.sync kernel runs
+// Estimates of the two kernels' times; bytes: workspace that the tcgen05 kernel can use.
+int kv_attend_rows_time(const KvAttendParams& p, int64_t max_rows, double* us);
+int kv_attend_tc_time(const KvAttendParams& p, int64_t max_rows, double* us, size_t* bytes);
 
 }  // namespace qr

@@ -218,10 +218,11 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
     batch = last_page_offset.shape[0]
     window, sink_tokens = min(int(window), 0x7fffffff) if window else 0, min(int(sink_tokens), 0x7fffffff)
     indptr = _check_i32(op, dev, "kv_indptr", kv_indptr, batch + 1)
+    indices, entries = _check_i32(op, dev, "kv_indices", kv_indices, 0), kv_indices.numel()      # none at all: not read
     # the shares of CTAs that meet in memory; decode-sized calls have none
     work = None
     if max_q_len * heads > 64 * kv_heads:
-        sizes = (pages, page_size, tokens, max_q_len, batch, heads, kv_heads, window, sink_tokens)
+        sizes = (entries, page_size, tokens, max_q_len, batch, heads, kv_heads, window, sink_tokens)
         if torch.cuda.current_device() == dev.index:
             nbytes = _lib_c.qr_kv_attend_workspace_bytes(*sizes)
         else:
@@ -230,7 +231,7 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
         if nbytes:
             work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(op, dev, _lib_c.qr_kv_attend_i4, o_p, ot, oh, q_p, qt, qh, kv_data.data_ptr(), kv_param.data_ptr(), pages,
-            indptr, _check_i32(op, dev, "kv_indices", kv_indices, 0) or indptr,            # no page at all: not read
+            indptr, indices or indptr, entries,
             _check_i32(op, dev, "last_page_offset", last_page_offset, batch), _check_i32(op, dev, "qo_indptr", qo_indptr, batch + 1),
             tokens, max_q_len, batch, layers, layer_idx, heads, kv_heads, page_size, 128, window, sink_tokens,
             1 if hadamard_q else 0, work.data_ptr() if work is not None else None, work.numel() if work is not None else 0)

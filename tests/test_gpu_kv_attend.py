@@ -14,6 +14,17 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
+@pytest.fixture(params=["mma.sync", "tcgen05"])
+def kernel(request):
+    """Both attention kernels serve every call; which one does is a matter of time."""
+    _lib.set_tuning("kv_attend", 1 if request.param == "mma.sync" else 2)
+    yield request.param
+    _lib.set_tuning("kv_attend", 0)
+
+
+both_kernels = pytest.mark.usefixtures("kernel")
+
+
 def _i32(v):
     return torch.tensor(v, dtype=torch.int32)
 
@@ -98,6 +109,7 @@ CASES = [
 ]
 
 
+@both_kernels
 @pytest.mark.parametrize("lens,new,heads,group,page,window,sinks,rotate", CASES)
 def test_chunk_attention_against_the_oracle(lens, new, heads, group, page, window, sinks, rotate):
     s = _setup(lens, new, heads, group, page, seed=sum(lens) + group)
@@ -106,6 +118,7 @@ def test_chunk_attention_against_the_oracle(lens, new, heads, group, page, windo
     _check(_attend(s, window, sinks, rotate), ref)             # without a bound on the chunk lengths
 
 
+@both_kernels
 @pytest.mark.parametrize("lens,heads,group,page,window,sinks,rotate", [
     ([1, 2, 31, 32, 33], 2, 4, 16, 0, 0, True), ([700, 1200, 64], 2, 8, 16, 0, 0, False), ([700, 1200, 64], 2, 1, 16, 500, 4, True),
     ([2000], 1, 16, 16, 0, 0, True), ([2000], 1, 24, 64, 1024, 4, True), ([40, 1], 1, 40, 5, 0, 0, False), ([900, 33], 3, 5, 16, 1, 0, False),
@@ -118,6 +131,7 @@ def test_single_tokens_with_window_and_shared_heads(lens, heads, group, page, wi
     _check(_attend(s, window, sinks, rotate, max_q=1), ref)
 
 
+@both_kernels
 def test_values_of_very_different_sizes_and_constant_rows():
     """Tokens whose rows are constant (the smallest scale the quantiser writes, a zero point a million times as large),
     tiny or large stand next to ordinary ones and get their weight and their value."""
@@ -136,6 +150,7 @@ def test_values_of_very_different_sizes_and_constant_rows():
     _check(_attend(s, max_q=20), ref)
 
 
+@both_kernels
 @pytest.mark.parametrize("new", [[3, 2], [150, 40]])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4)])
 def test_hidden_infinities_and_nan_do_not_reach_a_row(new, window, sinks):
@@ -161,6 +176,7 @@ def test_hidden_infinities_and_nan_do_not_reach_a_row(new, window, sinks):
         _check(got[keep], (clean[0][keep], clean[1][keep]))
 
 
+@both_kernels
 @pytest.mark.parametrize("new", [[2, 0, 3], [200, 0, 90]])
 def test_empty_sequences_and_rows_behind_the_last_one(new):
     """Sequences without new tokens, without cached tokens, rows of q beyond the last sequence, and a sequence with more
@@ -186,6 +202,7 @@ def test_empty_sequences_and_rows_behind_the_last_one(new):
     assert torch.isnan(got[1:]).all() and torch.isfinite(got[0]).all()
 
 
+@both_kernels
 @pytest.mark.parametrize("new", [[3], [140]])
 def test_strided_queries_and_outputs(new):
     """q as a column slice of a fused projection, o heads-first, both as [tokens, heads, 128] views; q itself as output."""
@@ -201,6 +218,7 @@ def test_strided_queries_and_outputs(new):
     _check(_attend(s, max_q=n, q=own, o=own), ref)
 
 
+@both_kernels
 def test_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes whose last pages are used."""
     free = torch.cuda.mem_get_info()[0]
@@ -225,6 +243,7 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(data[-1, 0, 1, :, 63].cpu(), qq[0]) and torch.equal(param[-1, 0, 0, :, 63].cpu(), torch.cat((sc, z), -1)[0])
 
 
+@both_kernels
 def test_another_stream_and_repeated_calls_give_the_same_bits():
     s = _setup([900, 300], [260, 4], 2, 4, 16, seed=31)
     first = _attend(s, max_q=260)

@@ -22,7 +22,7 @@ def _call(name, *args):
 
 
 def _attend(**kw):
-    a = dict(o=P, ots=1024, ohs=128, q=P, qts=1024, qhs=128, data=P, param=P, pages=10, indptr=P, indices=P, last=P, qo=P, total=8,
+    a = dict(o=P, ots=1024, ohs=128, q=P, qts=1024, qhs=128, data=P, param=P, pages=10, indptr=P, indices=P, entries=100, last=P, qo=P, total=8,
              most=8, batch=1, layers=1, layer=0, heads=8, kv_heads=8, page=16, dim=128, window=0, sinks=0, rotate=0, work=None, bytes=0,
              stream=None)
     assert not set(kw) - set(a)
@@ -31,7 +31,7 @@ def _attend(**kw):
 
 
 @pytest.mark.parametrize("kw,words", [
-    (dict(batch=-1), "negative"), (dict(total=-1), "negative"), (dict(most=-1), "negative"),
+    (dict(batch=-1), "negative"), (dict(total=-1), "negative"), (dict(most=-1), "negative"), (dict(entries=-1), "negative"),
     (dict(o=None), "null"), (dict(q=None), "null"), (dict(data=None), "null"), (dict(param=None), "null"), (dict(indptr=None), "null"),
     (dict(indices=None), "null"), (dict(last=None), "null"), (dict(dim=64), "head_dim"), (dict(layer=1), "layer"), (dict(layer=-1), "layer"),
     (dict(page=0), "page"), (dict(pages=0), "pages"), (dict(heads=12), "multiple"), (dict(kv_heads=0), "multiple"), (dict(heads=0), "multiple"),
