@@ -119,7 +119,9 @@ kv_attend_rows_kernel(const KvAttendParams p) {
   extern __shared__ __align__(128) unsigned char s_dyn[];
   unsigned char* ring = s_dyn;
   RwShared<NT>& sh = *reinterpret_cast<RwShared<NT>*>(s_dyn + RwConfig<NT>::kRing);
+  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  pdl_wait();
   const int unit = blockIdx.x / p.splits;
   uint32_t crank = 0;
   if (p.splits > 1) crank = kv_cluster_rank();
@@ -589,17 +591,19 @@ static int launch_rows(KvAttendParams& p, int64_t max_rows, cudaStream_t st) {
   if (const int rc = plan_rows<NT>(p, max_rows, &units, nullptr)) return rc;
   const int splits = p.splits;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = use_pdl(p.total_q);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(units * splits));
   cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
   QR_CUDA(cudaLaunchKernelEx(&cfg, kv_attend_rows_kernel<NT>, (const KvAttendParams)p));
   return QR_OK;
 }

@@ -12,8 +12,9 @@
 // memory) and then takes its share of the flat list of outputs; an entry finds its sequence by a binary search in
 // shared memory, 128 to 512 entries of kv_indices per search.  A new page is read from the free list by everyone, never from
 // the block table, whose new entries are written in the same launch: no CTA waits for another.
-// Measured: 16 requests 6.2 us, 2048 requests with 9 MB of table entries 12.6 us (3.4 us at the copy rate): latency of chained
-// reads and scans; a call from Python takes 18 us, a dozen torch operations for the same 600 us.
+// Measured: 16 requests 5.7 us, 2048 requests with 9 MB of table entries 11.9 us (3.4 us at the copy rate): latency of chained
+// reads and scans (programmatic dependent launch takes off 0.5 us); a call from Python takes 18 us, a dozen torch operations
+// for the same 600 us.
 #include "kv_common.cuh"
 
 namespace qr {
@@ -77,6 +78,7 @@ __device__ __forceinline__ int pt_find(const int* s, int n, int i) {
 template <int R>
 __global__ void __launch_bounds__(kPtThreads)
 kv_page_table_kernel(const PageTableParams p) {
+  pdl_launch_dependents();
   extern __shared__ int s_pt[];
   __shared__ long long s_warp[kPtThreads / 32];
   int* s_pages = s_pt;                          // [batch + 1] prefix sum of the pages
@@ -86,6 +88,7 @@ kv_page_table_kernel(const PageTableParams p) {
   const int tid = threadIdx.x;
   const int W = p.max_blocks;
   const bool take = p.block_table && p.num_free >= 0;
+  pdl_wait();
   long long base_rows = 0, base_need = 0, base_pages = 0, taken = 0, refused = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kPtThreads * kPtPer) {
     const int first = b0 + tid * kPtPer;
@@ -279,7 +282,6 @@ extern "C" int qr_kv_page_table(const int32_t* seq_lens, const int32_t* new_lens
   const int grid = (int)(want < num_sms() ? (want > 0 ? want : 1) : num_sms());
   auto kern = cap > 512ll * (kPtThreads / 32) * num_sms() ? kv_page_table_kernel<4> : kv_page_table_kernel<1>;
   if (smem > 48 * 1024) QR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<grid, kPtThreads, smem, (cudaStream_t)stream>>>(p);
-  QR_LAUNCH_CHECK("kv_page_table_kernel");
+  QR_CUDA(launch_kernel(kern, dim3(grid), dim3(kPtThreads), smem, (cudaStream_t)stream, g_tuning.pdl != 0, p));
   return QR_OK;
 }
