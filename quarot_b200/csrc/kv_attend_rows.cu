@@ -536,9 +536,13 @@ int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int6
   for (int s = 1; s <= 16 && s <= most; ++s) {
     const int fit = k.fit[s].load(std::memory_order_relaxed);
     if (fit < 1) continue;
-    // CTAs that the fullest SM works through, against those that it holds: an SM that is not full takes as long as a full one
+    // CTAs that the fullest SM works through, against those that it holds.  Of four, three take three quarters of the time
+    // (instructions); of two, one takes 0.6 of it (latency); an SM is not faster with fewer than it could hold in all.
     const int64_t load = (units * per_sm + fit - 1) / fit;
-    const double cost = (double)(load < per_sm ? per_sm : load) / per_sm * (1.0 / s + (s > 1 ? joined : alone));
+    // Clusters start as a whole: in several rounds of two CTAs per SM that costs some 15 % more.
+    double rounds = load <= per_sm ? 1.0 : (double)load / per_sm;
+    if (per_sm == 2 && load > 2) rounds = ((double)(load / 2) + 0.6 * (double)(load % 2)) * (s > 1 ? 1.15 : 1.0);
+    const double cost = rounds * (1.0 / s + (s > 1 ? joined : alone));
     if (s == 1 || cost < best * 0.98) { best = cost; *splits = s; }
   }
   if (cost_out) *cost_out = best;
@@ -562,12 +566,12 @@ static int plan_rows(KvAttendParams& p, int64_t max_rows, int64_t* units, double
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
-  // more; a list of pages much longer than what the sequences use must not lead to splits that only pay for such lengths
+  // more, two with sixteen rows; a list of pages much longer than what the sequences use must not lead to splits that only pay for such lengths
   const int64_t blocks = visible_blocks(p, max_rows, kRwTok, false), evenly = visible_blocks(p, max_rows, kRwTok, true);
   const double length = (double)(evenly < 256 ? evenly : 256) / kWarps;
   int resident = 0;
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
-                                    smem, *units, (blocks + kWarps - 1) / kWarps, 2.0 / length, 2.5 / length, &p.splits, &resident,
+                                    smem, *units, (blocks + kWarps - 1) / kWarps, 2.0 / length, (NT == 1 ? 2.5 : 4.0) / length, &p.splits, &resident,
                                     cost)) return rc;
   // more than one round: the longest sequences first (32 of ragged lengths: 87 us -> 75); a window makes them alike
   p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && *units * p.splits > resident;
@@ -579,7 +583,7 @@ int kv_attend_rows_time(const KvAttendParams& p, int64_t max_rows, double* us) {
   int64_t units = 0;
   double cost = 0.0;
   if (const int rc = plan_rows<2>(c, max_rows, &units, &cost)) return rc;
-  *us = 5.0 + cost * (double)visible_blocks(c, max_rows, kRwTok, true) * 0.425;      // 13.3 ns per token of a unit
+  *us = 1.0 + cost * (double)visible_blocks(c, max_rows, kRwTok, true) * 0.425;      // 13.3 ns per token of a unit
   return QR_OK;
 }
 
