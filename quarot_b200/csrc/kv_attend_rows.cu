@@ -566,13 +566,14 @@ static int plan_rows(KvAttendParams& p, int64_t max_rows, int64_t* units, double
   p.tiles_per_seq = uniform ? (int)per_seq : 0;
   p.max_tiles = (int)tiles;
   // start, query rows and the join of the warps take about as long as two blocks of a warp, a cluster's join half of one
-  // more, two with sixteen rows; a list of pages much longer than what the sequences use must not lead to splits that only pay for such lengths
+  // more, two with sixteen rows; a list of pages much longer than what the sequences use must not lead to splits that only
+  // pay for such lengths
   const int64_t blocks = visible_blocks(p, max_rows, kRwTok, false), evenly = visible_blocks(p, max_rows, kRwTok, true);
   const double length = (double)(evenly < 256 ? evenly : 256) / kWarps;
   int resident = 0;
   if (const int rc = kv_pick_splits(NT == 1 ? kKvKernelRows8 : kKvKernelRows16, (const void*)kv_attend_rows_kernel<NT>, 32 * kWarps,
-                                    smem, *units, (blocks + kWarps - 1) / kWarps, 2.0 / length, (NT == 1 ? 2.5 : 4.0) / length, &p.splits, &resident,
-                                    cost)) return rc;
+                                    smem, *units, (blocks + kWarps - 1) / kWarps, 2.0 / length, (NT == 1 ? 2.5 : 4.0) / length,
+                                    &p.splits, &resident, cost)) return rc;
   // more than one round: the longest sequences first (32 of ragged lengths: 87 us -> 75); a window makes them alike
   p.sorted = uniform && p.window <= 0 && p.batch > 1 && p.batch <= 64 && *units * p.splits > resident;
   return QR_OK;
@@ -638,8 +639,8 @@ static int kv_pick_kernel(const KvAttendParams& p, int64_t rows, bool* tc, size_
 extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_stride, const void* q, int64_t q_token_stride,
                                int64_t q_head_stride, const void* kv_data, const void* kv_param, int64_t num_pages,
                                const int32_t* kv_indptr, const int32_t* kv_indices, int64_t num_indices,
-                               const int32_t* last_page_offset, const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len, int batch, int num_layers, int layer,
-                               int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
+                               const int32_t* last_page_offset, const int32_t* qo_indptr, int64_t total_q, int64_t max_q_len,
+                               int batch, int num_layers, int layer, int num_q_heads, int num_kv_heads, int page_size, int head_dim, int window, int sink_tokens,
                                int hadamard_q, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace qr;
   if (batch < 0 || total_q < 0 || max_q_len < 0 || num_indices < 0) return fail(QR_EINVAL, "qr_kv_attend_i4: negative size");
@@ -658,7 +659,7 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
     return fail(QR_EINVAL, "qr_kv_attend_i4: without qo_indptr every sequence has one new token");
   if (max_q_len > total_q) return fail(QR_EINVAL, "qr_kv_attend_i4: max_q_len exceeds the number of new tokens");
   const int group = num_q_heads / num_kv_heads;
-  if (total_q * group > 0x3fffffffll || (int64_t)batch * max_q_len * group > 0xffffffffffll)
+  if (total_q > 0x3fffffffll / group || (int64_t)batch * max_q_len * group > 0xffffffffffll)
     return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many query rows");
   if (workspace && ((uintptr_t)workspace & 15)) return fail(QR_EALIGN, "qr_kv_attend_i4: workspace must be 16-byte aligned");
   if (((uintptr_t)q & 7) || ((uintptr_t)o & 7) || ((uintptr_t)kv_data & 15) || ((uintptr_t)kv_param & 3) || (q_token_stride & 3) ||
@@ -684,11 +685,12 @@ extern "C" int qr_kv_attend_i4(void* o, int64_t o_token_stride, int64_t o_head_s
 extern "C" size_t qr_kv_attend_workspace_bytes(int64_t num_indices, int page_size, int64_t total_q, int64_t max_q_len, int batch,
                                                int num_q_heads, int num_kv_heads, int window, int sink_tokens) {
   using namespace qr;
-  if (num_indices < 0 || page_size < 1 || total_q < 1 || max_q_len < 1 || batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads ||
+  if (num_indices < 0 || page_size < 1 || total_q < 1 || total_q > 0x3fffffffll || max_q_len < 1 || batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads ||
       num_q_heads % num_kv_heads || window < 0 || sink_tokens < 0 || max_q_len > total_q)
     return 0;
   KvAttendParams p = {};
-  p.num_indices = num_indices < 0x7fffffff ? num_indices : 0x7fffffff; p.page_size = page_size; p.total_q = total_q; p.batch = batch; p.kv_heads = num_kv_heads;
+  p.num_indices = num_indices < 0x7fffffff ? num_indices : 0x7fffffff;
+  p.page_size = page_size; p.total_q = total_q; p.batch = batch; p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads; p.window = window; p.sinks = window > 0 ? sink_tokens : 0;
   bool tc = false;
   size_t bytes = 0;

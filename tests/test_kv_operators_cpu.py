@@ -36,7 +36,7 @@ def _attend(**kw):
     (dict(indices=None), "null"), (dict(last=None), "null"), (dict(dim=64), "head_dim"), (dict(layer=1), "layer"), (dict(layer=-1), "layer"),
     (dict(page=0), "page"), (dict(pages=0), "pages"), (dict(heads=12), "multiple"), (dict(kv_heads=0), "multiple"), (dict(heads=0), "multiple"),
     (dict(pages=1 << 32), "2^32"), (dict(window=-1), "window"), (dict(sinks=-1), "sink"), (dict(qo=None), "one new token"),
-    (dict(qo=None, total=1, most=2), "one new token"), (dict(most=9), "max_q_len"), (dict(total=1 << 40, most=1), "rows"),
+    (dict(qo=None, total=1, most=2), "one new token"), (dict(most=9), "max_q_len"), (dict(total=1 << 40, most=1), "rows"), (dict(total=1 << 62, most=1), "rows"),
     (dict(o=P + 4), "aligned"), (dict(q=P + 2), "aligned"), (dict(data=P + 8), "aligned"), (dict(param=P + 2), "aligned"),
     (dict(qts=1022), "aligned"), (dict(ohs=130), "aligned"), (dict(work=P + 8, bytes=64), "aligned")])
 def test_attention_entry_refuses(kw, words):
