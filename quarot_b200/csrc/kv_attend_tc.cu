@@ -258,27 +258,30 @@ __device__ __forceinline__ void at_fetch(uint32_t (&s)[2][24], uint32_t t_s) {
   tmem_ld_16x256_x2(t_s + 32 + (16u << 16), s[1] + 16);
 }
 
-// The exponents of 48 columns, relative to M, in place of S; the lane's largest is returned.
-__device__ __forceinline__ float at_scores(uint32_t (&s)[2][24], const float* par, const AtRows& w) {
-  uint64_t off[4], qq[4];
-  float top0 = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    off[x] = f2_pack(-w.m[x], -w.m[x]);                   // +infinity before the row has seen a token: M has to be set
-    qq[x] = f2_pack(w.qs[x], w.qs[x]);
-  }
+// What the scores of 48 columns have besides S: u = log2 sigma - (z + 16 s) sum(q) - M, of the four rows of a lane.
+__device__ __forceinline__ void at_offsets(uint64_t (&u)[4][6], const float* par, const AtRows& w) {
 #pragma unroll
   for (int k = 0; k < 6; ++k) {
-    const float4 a = *reinterpret_cast<const float4*>(par + 4 * k * kAtPairFloats);
+    const float2 a = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 2);
     const float2 b = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats + 4);
-    const uint64_t ks = f2_pack(a.x, a.y), kz = f2_pack(a.z, a.w), lv = f2_pack(b.x, b.y);
+    const uint64_t kz = f2_pack(a.x, a.y), lv = f2_pack(b.x, b.y);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)                           // +infinity before the row has seen a token: M has to be set
+      u[x][k] = f2_add(f2_fma(kz, f2_pack(w.qs[x], w.qs[x]), lv), f2_pack(-w.m[x], -w.m[x]));
+  }
+}
+// The exponents of 48 columns, relative to M, in place of S; the lane's largest is returned.
+__device__ __forceinline__ float at_scores(uint32_t (&s)[2][24], const float* par, const uint64_t (&u)[4][6]) {
+  float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const float2 a = *reinterpret_cast<const float2*>(par + 4 * k * kAtPairFloats);
+    const uint64_t ks = f2_pack(a.x, a.y);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       uint32_t* r = s[x >> 1] + 4 * k + 2 * (x & 1);
-      uint64_t v = f2_fma(kz, qq[x], lv);
-      v = f2_fma(ks, f2_pack(__uint_as_float(r[0]), __uint_as_float(r[1])), v);
       float v0, v1;
-      f2_unpack(f2_add(v, off[x]), v0, v1);
+      f2_unpack(f2_fma(ks, f2_pack(__uint_as_float(r[0]), __uint_as_float(r[1])), u[x][k]), v0, v1);
       if (x & 1) top1 = max3(top1, v0, v1); else top0 = max3(top0, v0, v1);
       r[0] = __float_as_uint(v0);
       r[1] = __float_as_uint(v1);
@@ -550,9 +553,11 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
     for (int h = 0; ok && h < 2 * n; ++h) {
       const bool edge = t0 + kAtHalf - 1 > p_min || (p.window > 0 && t0 <= p_max - p.window && t0 + kAtHalf - 1 >= p.sinks);
       const uint32_t t_sb = t_s + (h & 1) * kAtHalf;
+      uint64_t u[4][6];
+      at_offsets(u, par, rw);                             // while S is on its way
       tmem_ld_done<24>(s[0]);
       tmem_ld_done<24>(s[1]);
-      float top = at_scores(s, par, rw);
+      float top = at_scores(s, par, u);
       if (__builtin_expect(edge, 0)) top = at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
       if (__builtin_expect(__any_sync(0xffffffffu, top > kAtTop), 0)) {
         // a weight would pass 2^15, or a row sees its first token: M moves, O follows by powers of two (or 0)
@@ -586,7 +591,8 @@ kv_attend_tc_kernel(const __grid_constant__ KvAttendParams p) {
           at_scale_o(t_o, f);
         }
         if (fresh) {
-          at_scores(s, par, rw);
+          at_offsets(u, par, rw);
+          at_scores(s, par, u);
           if (edge) at_mask(s, pos, t0 + 2 * c, p.window, p.sinks);
         } else {
 #pragma unroll
