@@ -34,10 +34,10 @@
 // Registers: 20 warps, five per scheduler, start with 96 each; the softmax warps go up to 160, the unpacking warps down to
 // 64 and the MMA warpgroup to 32 (per scheduler 2 x 160 + 2 x 64 + 32 = 5 x 96).  All waits are bounded (tc_ptx.cuh).
 //
-// Measured (2048 tokens x 64 heads over 10240 tokens, 8 KV heads): 845 us, 733 TFLOP/s.  A block of 96 tokens takes 4900
-// cycles: in each half the softmax of a warp takes 2300 -- 325 until S has arrived, 750 for scores, 760 for weights (exp2
-// alone would take 384 of a scheduler's special function unit per warp, and there are two), 450 waiting -- which is what
-// bounds it; the tensor cores are busy half of the time.  A CTA takes 15000 cycles before its first scores.
+// Measured (2048 tokens x 64 heads over 10240 tokens, 8 KV heads): 830 us, 746 TFLOP/s.  A block of 96 tokens takes 4800
+// cycles: in each half the softmax of a warp takes 2300 -- 325 until S has arrived, 750 for scores (a part of them now made
+// while S arrives), 760 for weights (exp2 alone would take 384 of a scheduler's special function unit per warp, and there
+// are two), 450 waiting -- which is what bounds it; the tensor cores are busy half of the time.  A CTA takes 15000 cycles before its first scores.
 #include "kv_common.cuh"
 #include "tc_ptx.cuh"
 
