@@ -181,6 +181,13 @@ def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None
             "slot_map": slots.view(torch.int64), "positions": positions, "seq_lens": after, "status": status}
 
 
+def _as_rows(x):
+    """x [tokens, heads, 128] as the slot append takes it: copied where the head dimension is not contiguous or the rows do
+    not begin on 8 bytes."""
+    ts, hs, ds = x.stride()
+    return x if ds == 1 and ts % 4 == 0 and hs % 4 == 0 and x.data_ptr() % 8 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
 def append_kv_slots_i4(kv_data, kv_param, slot_map, k, v, layer_idx, hadamard_k=True):
     """append_kv_i4 with the page slots from a slot map (build_page_table): slot_map int64 [tokens], k and v fp16 [tokens,
     heads, 128] (strided views are fine).  Tokens whose slot lies outside the pool, -1 among others, are left out; the other
@@ -385,7 +392,7 @@ class MultiLayerPagedKVCache4Bit:
         total = torch.full_like(new_lens, self.length) if attention_mask is None else attention_mask.sum(dim=-1, dtype=torch.int32)
         table = build_page_table(total - new_lens, new_lens, k.shape[0], self.page_size,
                                  max_blocks=self.pages.shape[0] // self.batch_size)
-        append_kv_slots_i4(self.pages, self.scales, table["slot_map"], k, v, layer_idx, hadamard_k=had)
+        append_kv_slots_i4(self.pages, self.scales, table["slot_map"], _as_rows(k), _as_rows(v), layer_idx, hadamard_k=had)
         if self._needs_init[layer_idx]:
             self._needs_init[layer_idx] = False
             return key_states, value_states
