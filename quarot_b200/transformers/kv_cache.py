@@ -300,15 +300,17 @@ class _AttentionStub(object):
     def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, chunk=None):
         batch_size, q_len, num_qo_heads, head_dim = q.shape
         table = {k: attention_kwargs[k] for k in _TABLE_KEYS}
-        if chunk is None:
-            assert q_len == 1
+        added, qo_indptr, shown = chunk or (1, None, None)
+        assert q_len == added
+        if q_len == 1:
             q = q.reshape(batch_size, num_qo_heads, head_dim).contiguous()
             attn_output = torch.empty_like(q)
             batch_decode_i4(attn_output, q, **table, layer_idx=layer_idx, hadamard_q=self.hadamard_dtype is not None,
                             window=self.window_size, sink_tokens=self.sink_tokens)
+            if shown is not None:               # a token that the mask hides gives zeros
+                attn_output.masked_fill_(~shown.view(batch_size, 1, 1), 0)
             return attn_output.unsqueeze(1)
-        added, qo_indptr, keep = chunk
-        assert q_len == added
+        keep = shown.flatten() if shown is not None else None
         rows = q.reshape(batch_size * q_len, num_qo_heads, head_dim)
         rows = (rows if keep is None else rows[keep]).contiguous()
         attn_output = torch.empty_like(rows)
@@ -365,7 +367,8 @@ class MultiLayerPagedKVCache4Bit:
         """First call per layer (the prompt): caches the keys / values and returns them unchanged, for the caller's own
         prefill attention.  Later calls: cache one token per sequence, or a chunk of them, and return a callable that maps
         the query [batch, tokens, heads, head_dim] to the attention output against the cache.  cache_kwargs may hold an
-        attention_mask [batch, cached + new tokens]; sequences may then differ in length by more than a page."""
+        attention_mask [batch, cached + new tokens]; sequences may then differ in length by more than a page, and a new
+        token that it hides is not cached and gives zeros."""
         b_sz, added_length, num_heads, head_dim = key_states.shape
         assert b_sz == self.batch_size
         attention_mask = (cache_kwargs or {}).get("attention_mask")
@@ -373,42 +376,51 @@ class MultiLayerPagedKVCache4Bit:
             new_length = self.length + added_length
             self._ensure_page_cnt_per_batch(self.page_cnt_from_length(new_length))
             self.length = new_length
-        specs = self.get_cache_specs_for_flash_infer(attention_mask)
         had = self.hadamard_dtype is not None
         k = key_states.reshape(b_sz * added_length, num_heads, head_dim)
         v = value_states.reshape(b_sz * added_length, num_heads, head_dim)
-        if not self._needs_init[layer_idx] and added_length == 1:
+        if attention_mask is None and not self._needs_init[layer_idx] and added_length == 1:
+            specs = self.get_cache_specs_for_flash_infer(None)
             append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
                          specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx, hadamard_k=had)
             return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
-        keep = new_lens = None
+        shown = None
         if attention_mask is not None:
-            new_mask = attention_mask[:, -added_length:].bool()
-            keep = new_mask.flatten()
-            new_lens = new_mask.sum(dim=-1, dtype=torch.int32)
-            k, v = k[keep], v[keep]
+            if 0 < self.length < attention_mask.shape[-1]:          # wider than the tokens so far: the last of these are the new ones
+                attention_mask = attention_mask[:, :self.length]
+            shown = attention_mask[:, -added_length:].bool()
+            new_lens = shown.sum(dim=-1, dtype=torch.int32)
         else:
             new_lens = torch.full((b_sz,), added_length, dtype=torch.int32, device=self.device)
-        total = torch.full_like(new_lens, self.length) if attention_mask is None else attention_mask.sum(dim=-1, dtype=torch.int32)
-        table = build_page_table(total - new_lens, new_lens, k.shape[0], self.page_size,
-                                 max_blocks=self.pages.shape[0] // self.batch_size)
-        append_kv_slots_i4(self.pages, self.scales, table["slot_map"], _as_rows(k), _as_rows(v), layer_idx, hadamard_k=had)
+        specs, table = self._page_table(attention_mask, new_lens, b_sz * added_length)
+        slots = table["slot_map"]
+        if shown is not None:
+            # the map holds the tokens that the mask shows one behind the other; the others are not cached
+            at = table["append_indptr"][:-1, None] + torch.cumsum(shown, 1, dtype=torch.int32) - 1
+            slots = slots[at.clamp(min=0)].masked_fill(~shown, -1).flatten()
+        append_kv_slots_i4(self.pages, self.scales, slots, _as_rows(k), _as_rows(v), layer_idx, hadamard_k=had)
         if self._needs_init[layer_idx]:
             self._needs_init[layer_idx] = False
             return key_states, value_states
         return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
-                                 chunk=(added_length, table["append_indptr"], keep))
+                                 chunk=(added_length, table["append_indptr"], shown))
 
-    def get_cache_specs_for_flash_infer(self, attention_mask):
-        """Page table of the cache as the kernels take it: sequence b owns pages b, b + batch, b + 2 batch, ..."""
+    def _page_table(self, attention_mask, new_lens=None, new_tokens=0):
+        """Page table of the cached tokens as the kernels take it (sequence b owns pages b, b + batch, b + 2 batch, ...) and,
+        on the GPU, all that build_page_table gives.  new_lens: how many of the tokens the step adds (None: none, they are
+        cached already), new_tokens: rows of the slot map."""
         if attention_mask is not None:
             seqlens = attention_mask.sum(dim=-1, dtype=torch.int32)
         else:
             seqlens = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self.device)
+        table = None
         if seqlens.is_cuda:
             most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
-            table = build_page_table(seqlens, torch.zeros_like(seqlens), 0, self.page_size,
-                                     max_blocks=max(self.page_cnt_from_length(most), 1))
+            if new_lens is None:
+                new_lens = torch.zeros_like(seqlens)
+            else:
+                seqlens = seqlens - new_lens
+            table = build_page_table(seqlens, new_lens, new_tokens, self.page_size, max_blocks=max(self.page_cnt_from_length(most), 1))
             indptr, indices, last = (table[k] for k in ("kv_indptr", "kv_indices", "last_page_offset"))
             if attention_mask is not None:
                 indices = indices[:int(indptr[-1])]
@@ -419,13 +431,18 @@ class MultiLayerPagedKVCache4Bit:
             indptr = torch.nn.functional.pad(torch.cumsum(page_cnt, 0), (1, 0)).to(torch.int32)
             indices = torch.cat([torch.arange(n, dtype=torch.int32) * self.batch_size + b for b, n in enumerate(page_cnt.tolist())])
             last = (seqlens - (page_cnt - 1).clamp(min=0) * self.page_size).to(torch.int32)
-        return {
+        specs = {
             "kv_data": self.pages,
             "kv_indptr": indptr,
             "kv_indices": indices,
             "last_page_offset": last,
             "kv_param": self.scales,
         }
+        return specs, table
+
+    def get_cache_specs_for_flash_infer(self, attention_mask):
+        """Page table of the cache as the kernels take it: sequence b owns pages b, b + batch, b + 2 batch, ..."""
+        return self._page_table(attention_mask)[0]
 
     def get_seq_length(self, layer_idx=0):
         return self.length

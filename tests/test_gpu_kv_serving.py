@@ -20,6 +20,58 @@ pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
+# ------------------------------------------------------------------ masks
+def _bytes(cache):
+    return cache.pages.cpu(), cache.scales.cpu().view(torch.int16)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("window,sinks,group", [(None, 0, 1), (None, 0, 2), (20, 2, 1), (20, 2, 4)])
+def test_a_single_token_that_the_mask_hides_is_not_cached(window, sinks, group, wide):
+    """Ragged sequences, an empty one among them; steps of one token that is padding for some of them.  What is cached of
+    those stays, their rows give zeros, the others get their token.  A mask may be wider than the tokens so far."""
+    B, H, P, L = 4, 2, 16, 2
+    cache = MultiLayerPagedKVCache4Bit(B, P, 64, DEV, L, H, 128, window_size=window, sink_tokens=sinks)
+    cache.pages.fill_(0xEE)
+    cache.scales.fill_(float("nan"))
+    g = torch.Generator().manual_seed(91)
+    mask = torch.zeros(B, 0, dtype=torch.int64)
+    count = [0] * B
+    for n, new in enumerate([[30, 16, 0, 5], [1, 0, 0, 1], [0, 0, 1, 1], [0, 0, 0, 0], [1, 1, 1, 1]]):
+        length = 33 if n == 0 else 1
+        column = torch.zeros(B, length, dtype=torch.int64)
+        for b, m in enumerate(new):
+            column[b, length - m:] = 1
+        mask = torch.cat((mask, column), 1)
+        given = torch.nn.functional.pad(mask, (0, 9)) if wide else mask
+        k, v = (torch.randn(B, length, H, 128, generator=g).half() for _ in range(2))
+        q = (torch.randn(B, length, H * group, 128, generator=g) * 1.5).half()
+        shown = [b for b in range(B) if new[b]]
+        for layer in range(L):
+            before = _bytes(cache)
+            r = cache.update((k + layer).half().to(DEV), v.to(DEV), layer, {"attention_mask": given.to(DEV)})
+            after = _bytes(cache)
+            ours = torch.zeros(before[0].shape[:5], dtype=torch.bool)
+            for b, m in enumerate(new):
+                for t in range(count[b], count[b] + m):
+                    ours[t // P * B + b, layer, :, :, t % P] = True
+            assert torch.equal(before[0][~ours], after[0][~ours]) and torch.equal(before[1][~ours], after[1][~ours])
+            assert bool((after[1][ours][:, 0] != before[1][ours][:, 0]).all())
+            if n == 0:
+                continue
+            got = r(q.to(DEV)).view(B, H * group, 128).cpu()
+            total = [c + m for c, m in zip(count, new)]
+            assert all(bool((got[b] == 0).all()) for b in range(B) if not new[b])
+            if not shown:
+                continue
+            pages = [-(-t // P) for t in total]
+            ref = O.paged_attention(O.kv_hadamard_fp16(q.view(B, H * group, 128)[shown]), cache.pages.cpu(), cache.scales.cpu(), layer,
+                                    torch.tensor([0] + pages).cumsum(0), torch.tensor([j * B + b for b in range(B) for j in range(pages[b])]),
+                                    [t - max(p - 1, 0) * P for t, p in zip(total, pages)], torch.tensor([0] + new).cumsum(0), window or 0, sinks)
+            _check(got[shown], ref)
+        count = [c + m for c, m in zip(count, new)]
+
+
 def test_a_prompt_in_any_strides_is_cached():
     """Keys and values whose head dimension is not contiguous are copied, as a single token's are."""
     T, H, P = 21, 2, 16
