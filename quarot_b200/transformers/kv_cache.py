@@ -278,7 +278,8 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
     dev = kv_data.device
     with torch.cuda.device(dev):
         _lib.check(_lib_c.qr_kv_decode_i4(
-            o.data_ptr(), q.data_ptr(), kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
+            o.data_ptr(), q.data_ptr(), kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(),
+            kv_indices.data_ptr() or kv_indptr.data_ptr(),         # no page at all: not read
             last_page_offset.data_ptr(), batch, kv_data.shape[1], int(layer_idx), heads, kv_data.shape[4], head_dim,
             1 if hadamard_q else 0, _stream(dev)), "batch_decode_i4")
 

@@ -72,6 +72,28 @@ def test_a_single_token_that_the_mask_hides_is_not_cached(window, sinks, group, 
         count = [c + m for c, m in zip(count, new)]
 
 
+@pytest.mark.parametrize("window", [None, 8])
+def test_masks_that_hide_everything(window):
+    """No sequence has a page: single tokens and chunks give zeros and cache nothing; the next token is the first."""
+    B, H, P = 2, 2, 16
+    cache = MultiLayerPagedKVCache4Bit(B, P, 64, DEV, 1, H, 128, hadamard_dtype=None, window_size=window)
+    cache.pages.fill_(0xEE)
+    g = torch.Generator().manual_seed(101)
+    mask = torch.zeros(B, 0, dtype=torch.int64, device=DEV)
+    for length in (5, 1, 3):
+        mask = torch.cat((mask, mask.new_zeros(B, length)), 1)
+        k = torch.randn(B, length, H, 128, generator=g).half().to(DEV)
+        r = cache.update(k, k, 0, {"attention_mask": mask})
+        assert length == 5 or bool((r(k) == 0).all())
+    assert bool((cache.pages == 0xEE).all())
+    mask = torch.cat((mask, mask.new_ones(B, 1)), 1)
+    k = torch.randn(B, 1, H, 128, generator=g).half().to(DEV)
+    got = cache.update(k, k, 0, {"attention_mask": mask})(k)
+    codes, scale, zero = O.kv_asym_quant_pack(k.cpu().view(B, H, 128))
+    value = torch.stack((codes & 15, codes >> 4), -1).view(B, H, 128) * scale.float() - zero.float()
+    assert float((got.cpu().view(B, H, 128).float() - value).abs().max()) <= 2.0 ** -11 * float(value.abs().max()) * 1.01
+
+
 def test_a_prompt_in_any_strides_is_cached():
     """Keys and values whose head dimension is not contiguous are copied, as a single token's are."""
     T, H, P = 21, 2, 16
