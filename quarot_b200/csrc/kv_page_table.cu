@@ -281,7 +281,10 @@ extern "C" int qr_kv_page_table(const int32_t* seq_lens, const int32_t* new_lens
   const int64_t want = (cap + 4 * kPtThreads - 1) / (4 * kPtThreads) + (new_tokens + kPtThreads - 1) / kPtThreads;
   const int grid = (int)(want < num_sms() ? (want > 0 ? want : 1) : num_sms());
   auto kern = cap > 512ll * (kPtThreads / 32) * num_sms() ? kv_page_table_kernel<4> : kv_page_table_kernel<1>;
-  if (smem > 48 * 1024) QR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // More than 48 KB, the kernel's own shared memory counted, has to be asked for.  Always the most that a call can need: the
+  // limit belongs to the kernel, and another thread's smaller batch must not lower it between this line and the launch.
+  constexpr int kMost = (4 * kPtMaxBatch + 2) * (int)sizeof(int);
+  if (smem > 40 * 1024) QR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
   QR_CUDA(launch_kernel(kern, dim3(grid), dim3(kPtThreads), smem, (cudaStream_t)stream, g_tuning.pdl != 0, p));
   return QR_OK;
 }

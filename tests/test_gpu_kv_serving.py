@@ -108,3 +108,43 @@ def test_a_prompt_in_any_strides_is_cached():
         r = cache.update(kk[:, :3], vv[:, :3], 0, {})
         pools.append((cache.pages, cache.scales, r(kk[:, :3])))
     assert all(torch.equal(a, b) for a, b in zip(*pools)) and bool((pools[0][1] != 0).any())
+
+
+# ------------------------------------------------------------------ page tables
+_FRESH = """
+import torch
+from quarot_b200.transformers import kv_cache as KV
+for width in (3, 400):
+    for batch in (3060, 3063, 3064, 3067, 3071, 3075, 4000):
+        lens = torch.randint(0, width * 16 - 1, (batch,), generator=torch.Generator().manual_seed(batch)).int()
+        t = KV.build_page_table(lens.cuda(), None, batch, 16, max_blocks=width)
+        want = torch.cat((torch.zeros(1, dtype=torch.int64), ((lens.long() + 16) // 16).cumsum(0)))
+        assert torch.equal(t["kv_indptr"].cpu().long(), want), batch
+        assert torch.equal(t["positions"].cpu(), lens) and t["status"].tolist() == [0, 0]
+print("fine")
+"""
+
+
+def test_page_tables_around_48_kb_of_shared_memory_in_a_fresh_process():
+    """No larger batch has come before: every launch asks for what it needs itself."""
+    r = subprocess.run([sys.executable, "-c", _FRESH], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr[-2000:]
+
+
+def test_page_tables_of_different_sizes_from_two_threads():
+    errors = []
+
+    def work(batch):
+        try:
+            lens = torch.full((batch,), 20, dtype=torch.int32, device=DEV)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    t = KV.build_page_table(lens, None, batch, 16, max_blocks=2)
+                assert t["kv_indptr"][-1].item() == 2 * batch and t["slot_map"][-1].item() == (2 * batch - 1) * 16 + 4
+        except Exception as e:  # noqa: BLE001 - reported below, from the main thread
+            errors.append((batch, str(e)))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(n,)) for n in (8192, 3100, 6000)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
