@@ -415,19 +415,22 @@ class MultiLayerPagedKVCache4Bit:
         else:
             seqlens = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self.device)
         table = None
+        most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
+        # a mask may claim more tokens than the pool holds; what is listed lies in the pool
+        blocks = max(min(self.page_cnt_from_length(most), self.pages.shape[0] // self.batch_size), 1)
         if seqlens.is_cuda:
-            most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
             if new_lens is None:
                 new_lens = torch.zeros_like(seqlens)
             else:
                 seqlens = seqlens - new_lens
-            table = build_page_table(seqlens, new_lens, new_tokens, self.page_size, max_blocks=max(self.page_cnt_from_length(most), 1))
+            table = build_page_table(seqlens, new_lens, new_tokens, self.page_size, max_blocks=blocks)
             indptr, indices, last = (table[k] for k in ("kv_indptr", "kv_indices", "last_page_offset"))
             if attention_mask is not None:
                 indices = indices[:int(indptr[-1])]
             elif self.length == 0:
                 indices = indices[:0]
         else:
+            seqlens = seqlens.clamp(max=blocks * self.page_size)
             page_cnt = self.page_cnt_from_length(seqlens)
             indptr = torch.nn.functional.pad(torch.cumsum(page_cnt, 0), (1, 0)).to(torch.int32)
             indices = torch.cat([torch.arange(n, dtype=torch.int32) * self.batch_size + b for b, n in enumerate(page_cnt.tolist())])

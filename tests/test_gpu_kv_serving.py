@@ -110,6 +110,14 @@ def test_a_prompt_in_any_strides_is_cached():
     assert all(torch.equal(a, b) for a, b in zip(*pools)) and bool((pools[0][1] != 0).any())
 
 
+def test_the_page_table_of_the_cache_stays_in_the_pool():
+    cache = MultiLayerPagedKVCache4Bit(2, 16, 32, DEV, 1, 1, 128)
+    cache.length = 30
+    got = cache.get_cache_specs_for_flash_infer(torch.ones(2, 90, dtype=torch.int64, device=DEV))
+    assert got["kv_indices"].tolist() == [0, 2, 1, 3] and got["kv_indptr"].tolist() == [0, 2, 4]
+    assert got["last_page_offset"].tolist() == [16, 16]
+
+
 # ------------------------------------------------------------------ page tables
 _FRESH = """
 import torch
