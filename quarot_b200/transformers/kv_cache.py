@@ -284,6 +284,28 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             1 if hadamard_q else 0, _stream(dev)), "batch_decode_i4")
 
 
+_TABLE_MOST = 8192                              # sequences that build_page_table takes
+
+
+def _fixed_page_table(seq_lens, new_lens, new_tokens, page_size, max_blocks):
+    """What the cache needs of build_page_table without a block_table, in torch operations: on the CPU, and for more
+    sequences than the kernel takes.  seq_lens: lengths WITH the new tokens."""
+    batch, dev = seq_lens.shape[0], seq_lens.device
+    rows = lambda n: torch.nn.functional.pad(torch.cumsum(n, 0, dtype=torch.int32), (1, 0))  # noqa: E731
+    held = seq_lens.clamp(min=0, max=max_blocks * page_size)
+    page_cnt = (held + page_size - 1) // page_size
+    indptr, append = rows(page_cnt), rows(new_lens)
+    total = int(indptr[-1])
+    b = torch.repeat_interleave(torch.arange(batch, device=dev), page_cnt.long(), output_size=total)
+    indices = ((torch.arange(total, device=dev) - indptr[b]) * batch + b).to(torch.int32)
+    i = torch.arange(new_tokens, device=dev, dtype=torch.int32)
+    b = torch.searchsorted(append[1:], i, right=True).clamp(max=batch - 1)
+    pos = (seq_lens - new_lens)[b].long() + i - append[b]
+    slots = ((pos // page_size) * batch + b) * page_size + pos % page_size
+    return {"kv_indptr": indptr, "kv_indices": indices, "last_page_offset": (held - (page_cnt - 1).clamp(min=0) * page_size).to(torch.int32),
+            "append_indptr": append, "slot_map": torch.where((i < append[-1]) & (seq_lens[b] <= max_blocks * page_size), slots, -1)}
+
+
 _TABLE_KEYS = ("kv_data", "kv_indptr", "kv_indices", "last_page_offset", "kv_param")
 
 
@@ -407,34 +429,27 @@ class MultiLayerPagedKVCache4Bit:
                                  chunk=(added_length, table["append_indptr"], shown))
 
     def _page_table(self, attention_mask, new_lens=None, new_tokens=0):
-        """Page table of the cached tokens as the kernels take it (sequence b owns pages b, b + batch, b + 2 batch, ...) and,
-        on the GPU, all that build_page_table gives.  new_lens: how many of the tokens the step adds (None: none, they are
-        cached already), new_tokens: rows of the slot map."""
+        """Page table of the cached tokens as the kernels take it (sequence b owns pages b, b + batch, b + 2 batch, ...), and
+        with it where a step's tokens go, as build_page_table gives it.  new_lens: how many of the tokens the step adds (None:
+        none, they are cached already), new_tokens: rows of the slot map."""
         if attention_mask is not None:
             seqlens = attention_mask.sum(dim=-1, dtype=torch.int32)
         else:
             seqlens = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self.device)
-        table = None
         most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
         # a mask may claim more tokens than the pool holds; what is listed lies in the pool
         blocks = max(min(self.page_cnt_from_length(most), self.pages.shape[0] // self.batch_size), 1)
-        if seqlens.is_cuda:
-            if new_lens is None:
-                new_lens = torch.zeros_like(seqlens)
-            else:
-                seqlens = seqlens - new_lens
-            table = build_page_table(seqlens, new_lens, new_tokens, self.page_size, max_blocks=blocks)
-            indptr, indices, last = (table[k] for k in ("kv_indptr", "kv_indices", "last_page_offset"))
-            if attention_mask is not None:
-                indices = indices[:int(indptr[-1])]
-            elif self.length == 0:
-                indices = indices[:0]
+        if new_lens is None:
+            new_lens = torch.zeros_like(seqlens)
+        if seqlens.is_cuda and self.batch_size <= _TABLE_MOST:
+            table = build_page_table(seqlens - new_lens if new_tokens else seqlens, new_lens, new_tokens, self.page_size, max_blocks=blocks)
         else:
-            seqlens = seqlens.clamp(max=blocks * self.page_size)
-            page_cnt = self.page_cnt_from_length(seqlens)
-            indptr = torch.nn.functional.pad(torch.cumsum(page_cnt, 0), (1, 0)).to(torch.int32)
-            indices = torch.cat([torch.arange(n, dtype=torch.int32) * self.batch_size + b for b, n in enumerate(page_cnt.tolist())])
-            last = (seqlens - (page_cnt - 1).clamp(min=0) * self.page_size).to(torch.int32)
+            table = _fixed_page_table(seqlens, new_lens, new_tokens, self.page_size, blocks)
+        indptr, indices, last = (table[k] for k in ("kv_indptr", "kv_indices", "last_page_offset"))
+        if attention_mask is not None:
+            indices = indices[:int(indptr[-1])]
+        elif self.length == 0:
+            indices = indices[:0]
         specs = {
             "kv_data": self.pages,
             "kv_indptr": indptr,

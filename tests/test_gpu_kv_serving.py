@@ -118,6 +118,40 @@ def test_the_page_table_of_the_cache_stays_in_the_pool():
     assert got["last_page_offset"].tolist() == [16, 16]
 
 
+def test_a_cache_of_more_sequences_than_the_page_table_kernel_takes():
+    """Prompt, single tokens with and without a mask, and a chunk for 9000 sequences."""
+    B, H, P = 9000, 1, 8
+    g = torch.Generator().manual_seed(93)
+    mask = torch.ones(B, 6, dtype=torch.int64)
+    mask[::3, :4] = 0
+    for masked in (False, True):
+        cache = MultiLayerPagedKVCache4Bit(B, P, 16, DEV, 1, H, 128, hadamard_dtype=None)
+        seen = mask if masked else torch.ones_like(mask)
+        keys = []
+        for n, length in enumerate((6, 1, 4)):
+            k = torch.randn(B, length, H, 128, generator=g).half()
+            if n:
+                seen = torch.cat((seen, torch.ones(B, length, dtype=torch.int64)), 1)
+            keys.append(k)
+            r = cache.update(k.to(DEV), k.to(DEV), 0, {"attention_mask": seen.to(DEV)} if masked else {})
+            if n == 0:
+                continue
+            got = r(k.to(DEV)).cpu()
+            every = torch.cat(keys, 1)
+            pick = [0, 1, 2, 3, 8191, 8192, 8193, B - 2, B - 1]
+            for b in pick:
+                mine = every[b][seen[b].bool()]
+                m = mine.shape[0]
+                pages, par = torch.zeros(2, 1, 2, H, P, 64, dtype=torch.uint8), torch.zeros(2, 1, 2, H, P, 2).half()
+                qq, s, z = O.kv_asym_quant_pack(mine)
+                for t in range(m):
+                    pages[t // P, 0, :, 0, t % P] = qq[t, 0]
+                    par[t // P, 0, :, 0, t % P] = torch.cat((s, z), -1)[t, 0]
+                used = -(-m // P)
+                ref = O.paged_attention(k[b], pages, par, 0, [0, used], torch.arange(used), [m - (used - 1) * P], [0, length])
+                _check(got[b], ref)
+
+
 # ------------------------------------------------------------------ page tables
 _FRESH = """
 import torch
