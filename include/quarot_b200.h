@@ -289,7 +289,8 @@ int qr_kv_decode_i4(void* o, const void* q, const void* kv_data, const void* kv_
  *   slot_map, positions [new_tokens]  page * page_size + slot and position in its sequence of every new token
  *   seq_lens_out [batch], status [2] = (free pages taken, sequences refused)
  * A sequence whose row of the block table, the free list or the new_tokens rows cannot hold its new tokens is refused: it
- * keeps its old length, takes no page, and its tokens get slot and position -1.  Sequences are served in order; once the
+ * keeps its old length, takes no page, and its tokens get slot and position -1.  So is one whose old length exceeds its row,
+ * also without new tokens: seq_lens_out repeats that length, the table lists the row's pages, all full.  Sequences are served in order; once the
  * free list has run out every later sequence that needs a page is refused.  new_tokens may exceed the sum of new_lens
  * (a padded batch): the rows behind get -1.  Negative lengths count as 0.  Outputs must not overlap inputs.
  * batch <= 8192 and batch * max_blocks < 2^31 (QR_EUNSUPPORTED otherwise). */

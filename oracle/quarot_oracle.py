@@ -278,9 +278,10 @@ def kv_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, f
     wanted = taken = refused = 0
     for b in range(batch):
         old, new = min(max(seq_lens[b], 0), width * page_size), max(new_lens[b], 0)
+        over = seq_lens[b] > width * page_size                 # longer than its row: refused, all of the row listed
         row = out["append_indptr"][-1]
         out["append_indptr"].append(row + new)
-        ok = new == 0 or (pages(old + new) <= width and row + new <= new_tokens)
+        ok = not over and (new == 0 or (pages(old + new) <= width and row + new <= new_tokens))
         if ok and block_table is not None and free_pages is not None:
             need = pages(old + new) - pages(old)
             first = wanted
@@ -295,7 +296,7 @@ def kv_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None, f
         mine = [block_table[b][j] if block_table is not None else j * batch + b for j in range(pages(after))]
         out["kv_indices"] += mine
         out["kv_indptr"].append(len(out["kv_indices"]))
-        out["seq_lens"].append(after)
+        out["seq_lens"].append(seq_lens[b] if over else after)
         out["last_page_offset"].append(after - max(len(mine) - 1, 0) * page_size)
         for i in range(new if ok else 0):
             pos = old + i

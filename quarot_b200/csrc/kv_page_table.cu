@@ -5,7 +5,7 @@
 // of need.  Everything the cache kernels read follows from three prefix sums over the batch: indptr (of the pages), the
 // rows of the new tokens (of new) and N.  A sequence that does not fit -- its row of the block table, the free list or
 // the slot map ends before it -- keeps its old length and its new tokens get slot -1, so that no consumer writes
-// anywhere for them.  Since N only grows, the sequences that the free list serves are a prefix of those that need pages.
+// anywhere for them; one that is longer than its row already does not fit either, and the row's pages are listed for it.  Since N only grows, the sequences that the free list serves are a prefix of those that need pages.
 //
 // The call writes a few megabytes at most, so it is one launch without a second pass: every CTA makes the three prefix
 // sums of the whole batch itself (512 threads x 4 sequences per round, the sums of up to 8192 sequences in shared
@@ -93,14 +93,16 @@ kv_page_table_kernel(const PageTableParams p) {
   for (int b0 = 0; b0 < p.batch; b0 += kPtThreads * kPtPer) {
     const int first = b0 + tid * kPtPer;
     int old[kPtPer], add[kPtPer], held[kPtPer], need[kPtPer];
-    bool fits[kPtPer];
+    bool fits[kPtPer], over[kPtPer];
     long long sum = 0, total;
 #pragma unroll
     for (int k = 0; k < kPtPer; ++k) {
       const int b = first + k;
       const long long cap = (long long)W * p.page_size;
       const int most = cap < 0x7fffffffll ? (int)cap : 0x7fffffff;
-      old[k] = b < p.batch ? min(max(p.seq_lens[b], 0), most) : 0;
+      const int len = b < p.batch ? max(p.seq_lens[b], 0) : 0;
+      over[k] = len > most;                     // longer than its row: refused, and the row's pages are listed
+      old[k] = min(len, most);
       add[k] = b < p.batch ? (p.new_lens ? max(p.new_lens[b], 0) : 1) : 0;
       sum += add[k];
     }
@@ -116,7 +118,7 @@ kv_page_table_kernel(const PageTableParams p) {
       const int b = first + k;
       if (b < p.batch) s_rows[b] = (int)min(rows, 0x7fffffffll);
       rows += add[k];
-      fits[k] = add[k] == 0 || (after < 0x7fffffffll && want <= W && rows <= p.new_tokens);
+      fits[k] = !over[k] && (add[k] == 0 || (after < 0x7fffffffll && want <= W && rows <= p.new_tokens));
       need[k] = fits[k] && take ? want - held[k] : 0;
       // where the pages are there already the sequence just has more of them
       if (fits[k] && !take) held[k] = want;
@@ -151,7 +153,7 @@ kv_page_table_kernel(const PageTableParams p) {
         mine_refused += fits[k] ? 0 : 1;
         if (blockIdx.x == 0) {
           const int after = fits[k] ? old[k] + add[k] : old[k];
-          p.seq_lens_out[b] = after;
+          p.seq_lens_out[b] = over[k] ? p.seq_lens[b] : after;
           p.last_page_offset[b] = after - (n > 1 ? (n - 1) * p.page_size : 0);
         }
       }

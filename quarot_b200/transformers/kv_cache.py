@@ -137,7 +137,8 @@ def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None
     [batch] -- the sequences WITH the new tokens -- append_indptr [batch + 1], slot_map int64 [new_tokens], positions
     int32 [new_tokens], seq_lens [batch] after the step, status int32 [2] = (free pages taken, sequences refused).  A
     sequence that does not fit (free list, block table or slot map too short) is refused: it keeps its length and its
-    tokens get slot and position -1, which append_kv_slots_i4 skips.
+    tokens get slot and position -1, which append_kv_slots_i4 skips.  So is one that is longer than its row of the block
+    table already, new tokens or not; the row's pages are listed for it.
     """
     op = "build_page_table"
     if seq_lens.dim() != 1 or not seq_lens.is_cuda:

@@ -190,3 +190,17 @@ def test_page_tables_of_different_sizes_from_two_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not errors
+
+
+@pytest.mark.parametrize("form", ["free list", "pages there", "fixed"])
+def test_sequences_longer_than_their_row_are_refused_as_they_are(form):
+    """Their length is reported as it was, with and without new tokens; the pages listed are those of the row."""
+    table, free, width = [[1, 2], [3, 4], [5, 6], [7, -1]], [8, 9], None
+    if form == "pages there":
+        free = None
+    elif form == "fixed":
+        table, free, width = None, None, 2
+    got = _run_table([100, 33, 32, 5], [0, 2, 0, 4], 6, 16, table, free, width)
+    assert got["seq_lens"].tolist() == [100, 33, 32, 9] and got["status"].tolist() == [0, 2]
+    assert got["kv_indptr"].tolist() == [0, 2, 4, 6, 7] and got["last_page_offset"].tolist() == [16, 16, 16, 9]
+    assert got["slot_map"].tolist()[:2] == [-1, -1] and got["positions"].tolist() == [-1, -1, 5, 6, 7, 8]
