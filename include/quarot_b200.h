@@ -285,7 +285,9 @@ int qr_kv_decode_i4(void* o, const void* q, const void* kv_data, const void* kv_
  * Writes
  *   kv_indptr [batch + 1], kv_indices [batch * max_blocks] (entries behind the last page: -1), last_page_offset [batch]:
  *                      the sequences WITH the new tokens, as the other calls take them
- *   append_indptr [batch + 1]  prefix sum of new_lens (also the qo_indptr of qr_kv_attend_i4)
+ *   append_indptr [batch + 1]  prefix sum of new_lens, refused sequences included: the rows of k, v and q (the qo_indptr of
+ *                      qr_kv_attend_i4, which takes the rows of a refused sequence for the last of its old tokens: they are
+ *                      those with position -1, and of no use)
  *   slot_map, positions [new_tokens]  page * page_size + slot and position in its sequence of every new token
  *   seq_lens_out [batch], status [2] = (free pages taken, sequences refused)
  * A sequence whose row of the block table, the free list or the new_tokens rows cannot hold its new tokens is refused: it

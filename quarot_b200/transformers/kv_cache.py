@@ -137,7 +137,8 @@ def build_page_table(seq_lens, new_lens, new_tokens, page_size, block_table=None
     [batch] -- the sequences WITH the new tokens -- append_indptr [batch + 1], slot_map int64 [new_tokens], positions
     int32 [new_tokens], seq_lens [batch] after the step, status int32 [2] = (free pages taken, sequences refused).  A
     sequence that does not fit (free list, block table or slot map too short) is refused: it keeps its length and its
-    tokens get slot and position -1, which append_kv_slots_i4 skips.  So is one that is longer than its row of the block
+    tokens get slot and position -1, which append_kv_slots_i4 skips; append_indptr, which lays out the rows of k, v and q,
+    counts them all the same, and the attention is told by `positions` which of its rows they are.  So is one that is longer than its row of the block
     table already, new tokens or not; the row's pages are listed for it.
     """
     op = "build_page_table"
@@ -245,15 +246,29 @@ def _attend_i4(op, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
             1 if hadamard_q else 0, work.data_ptr() if work is not None else None, work.numel() if work is not None else 0)
 
 
+def _check_positions(op, q, positions):
+    if positions is not None and (positions.dtype is not torch.int32 or positions.device != q.device or positions.shape != q.shape[:1]):
+        raise RuntimeError("%s: positions must be int32 on %s with one entry per token" % (op, q.device))
+
+
+def _clear_refused(o, positions):
+    """The rows of tokens that have no place in the cache, by the page table's positions."""
+    if positions is not None:
+        o.masked_fill_((positions < 0).view(-1, 1, 1), 0)
+
+
 def chunk_attention_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr, layer_idx, max_q_len=None,
-                       hadamard_q=False, window=None, sink_tokens=0):
+                       hadamard_q=False, window=None, sink_tokens=0, positions=None):
     """Causal attention of several new tokens per sequence over the packed pages, which already hold them.
 
     q, o fp16 [tokens, heads, 128] (strided views are fine), the new tokens of sequence b in rows qo_indptr[b] ..
     qo_indptr[b + 1]; they are the last of its cached tokens.  heads may be a multiple of the cache's heads: query head h
     reads KV head h // (heads // kv_heads).  window: a token sees itself and the window - 1 tokens before it, and the first
     sink_tokens tokens.  max_q_len: an upper bound of the new tokens of any sequence (default: all of q; a close bound
-    makes a better grid).  Rows that see nothing give zeros; rows of o that belong to no sequence stay as they are."""
+    makes a better grid).  Rows that see nothing give zeros; rows of o that belong to no sequence stay as they are.
+    positions int32 [tokens], as build_page_table gives them: rows with -1, those of refused sequences and of padding behind
+    the last one, give zeros.  Without it the new tokens of a refused sequence are taken for the last of its old ones."""
+    _check_positions("chunk_attention_i4", q, positions)
     max_q_len = q.shape[0] if max_q_len is None else int(max_q_len)
     if qo_indptr is None:
         raise RuntimeError("chunk_attention_i4: qo_indptr is needed")
@@ -261,19 +276,23 @@ def chunk_attention_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page
         raise RuntimeError("chunk_attention_i4: max_q_len must be positive")
     _attend_i4("chunk_attention_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, qo_indptr,
                min(max_q_len, q.shape[0]), layer_idx, hadamard_q, window, sink_tokens)
+    _clear_refused(o, positions)
 
 
 def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, hadamard_q=False, window=None,
-                    sink_tokens=0):
+                    sink_tokens=0, positions=None):
     """o[b, h] = softmax(q[b, h] K^T / sqrt(d)) V over the packed pages, one new token per sequence
     (quarot/transformers/kv_cache.py:64-72); with hadamard_q the query is Hadamard-transformed first.  With a window only
-    the last `window` tokens and the first sink_tokens are seen; the query may have a multiple of the cache's heads."""
+    the last `window` tokens and the first sink_tokens are seen; the query may have a multiple of the cache's heads.
+    positions as in chunk_attention_i4."""
     shape = q.shape
+    _check_positions("batch_decode_i4", q, positions)
     if window is not None or len(shape) == 3 and shape[1] != kv_data.shape[3]:
         if shape[0] != last_page_offset.shape[0]:
             raise RuntimeError("batch_decode_i4: %d queries for %d sequences" % (shape[0], last_page_offset.shape[0]))
-        return _attend_i4("batch_decode_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, None, 1, layer_idx,
-                          hadamard_q, window, sink_tokens)
+        _attend_i4("batch_decode_i4", o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, None, 1, layer_idx,
+                   hadamard_q, window, sink_tokens)
+        return _clear_refused(o, positions)
     batch, heads, head_dim = shape
     assert o.shape == shape and q.dtype == o.dtype == torch.float16 and q.is_contiguous() and o.is_contiguous()
     dev = kv_data.device
@@ -283,6 +302,7 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             kv_indices.data_ptr() or kv_indptr.data_ptr(),         # no page at all: not read
             last_page_offset.data_ptr(), batch, kv_data.shape[1], int(layer_idx), heads, kv_data.shape[4], head_dim,
             1 if hadamard_q else 0, _stream(dev)), "batch_decode_i4")
+    _clear_refused(o, positions)
 
 
 _TABLE_MOST = 8192                              # sequences that build_page_table takes

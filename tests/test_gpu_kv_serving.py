@@ -204,3 +204,55 @@ def test_sequences_longer_than_their_row_are_refused_as_they_are(form):
     assert got["seq_lens"].tolist() == [100, 33, 32, 9] and got["status"].tolist() == [0, 2]
     assert got["kv_indptr"].tolist() == [0, 2, 4, 6, 7] and got["last_page_offset"].tolist() == [16, 16, 16, 9]
     assert got["slot_map"].tolist()[:2] == [-1, -1] and got["positions"].tolist() == [-1, -1, 5, 6, 7, 8]
+
+
+@both_kernels
+@pytest.mark.parametrize("new", [[2, 3, 1], [70, 90, 80]])
+def test_rows_of_a_refused_sequence(new):
+    """The free list ends at the second sequence.  Its tokens are not cached; its rows, which stand among the others in q,
+    give zeros where the positions are passed on, and the other sequences do not notice."""
+    page, H, G, W = 16, 2, 2, 12
+    lens = [30, 31, 4]
+    g = torch.Generator().manual_seed(94)
+    need = [-(-(n + m) // page) - -(-n // page) for n, m in zip(lens, new)]
+    bt = torch.zeros(3, W, dtype=torch.int32, device=DEV)
+    free = torch.randperm(40, generator=g).to(torch.int32).to(DEV)
+    data = torch.zeros((40, 1, 2, H, page, 64), dtype=torch.uint8, device=DEV)
+    param = torch.full((40, 1, 2, H, page, 2), float("nan"), dtype=torch.float16, device=DEV)
+    first = KV.build_page_table(torch.zeros(3, dtype=torch.int32, device=DEV), _i32(lens).to(DEV), sum(lens), page, bt, free)
+    k = torch.randn(sum(lens), H, 128, generator=g).half().to(DEV)
+    KV.append_kv_slots_i4(data, param, first["slot_map"], k, -k, 0)
+    used = sum(-(-n // page) for n in lens)
+    left = free[used:used + need[0] + need[1] - 1].clone()
+    t = KV.build_page_table(first["seq_lens"], _i32(new).to(DEV), sum(new), page, bt, left)
+    # the third needs no page if it stays in its last one, and none is left for it otherwise
+    fits = [True, False, need[2] == 0]
+    assert t["status"].tolist()[1] == fits.count(False)
+    assert t["seq_lens"].tolist() == [n + m * f for n, m, f in zip(lens, new, fits)]
+    k = torch.randn(sum(new), H, 128, generator=g).half().to(DEV)
+    q = torch.randn(sum(new), H * G, 128, generator=g).half()
+    KV.append_kv_slots_i4(data, param, t["slot_map"], k, k, 0)
+    o = torch.full(q.shape, float("nan"), dtype=torch.float16, device=DEV)
+    KV.chunk_attention_i4(o, q.to(DEV), data, param, t["kv_indptr"], t["kv_indices"], t["last_page_offset"], t["append_indptr"], 0,
+                          max_q_len=max(new), positions=t["positions"])
+    ref = O.paged_attention(q, data.cpu(), param.cpu(), 0, t["kv_indptr"].cpu(), t["kv_indices"].cpu(), t["last_page_offset"].cpu(),
+                            t["append_indptr"].cpu())
+    shown = torch.repeat_interleave(torch.tensor(fits), torch.tensor(new))
+    _check(o.cpu()[shown], (ref[0][shown], ref[1][shown]))
+    assert bool((o.cpu()[~shown] == 0).all())
+    assert (t["positions"].cpu() < 0).tolist() == (~shown).tolist()
+
+
+@pytest.mark.parametrize("window,group", [(None, 1), (None, 2), (20, 1)])
+def test_single_tokens_of_a_refused_sequence(window, group):
+    s = _setup([40, 17, 33], [1, 1, 1], 2, group, 16, seed=95)
+    positions = _i32([39, -1, 32]).to(DEV)
+    o = torch.full(s["q"].shape, float("nan"), dtype=torch.float16, device=DEV)
+    args = (s["pages"].to(DEV), s["params"].to(DEV), s["indptr"].to(DEV), s["indices"].to(DEV), s["last"].to(DEV), s["layer"])
+    KV.batch_decode_i4(o, s["q"].to(DEV), *args, window=window, positions=positions)
+    ref = _oracle(s, window or 0)
+    _check(o.cpu()[[0, 2]], (ref[0][[0, 2]], ref[1][[0, 2]]))
+    assert bool((o[1] == 0).all())
+    for bad in (positions[:2], positions.long(), positions.cpu()):
+        with pytest.raises(RuntimeError):
+            KV.batch_decode_i4(o, s["q"].to(DEV), *args, window=window, positions=bad)
