@@ -559,7 +559,8 @@ static int plan_rows(KvAttendParams& p, int64_t max_rows, int64_t* units, double
   // tiles: at most one ragged tile per sequence beyond the full ones; a grid of equal shares per sequence needs no search
   const int64_t per_seq = (max_rows + R - 1) / R;
   const int64_t bound = p.total_q * p.group / R + p.batch;
-  const bool uniform = !p.qo_indptr || p.batch * per_seq <= 2 * bound;
+  // by the sizes alone, which the workspace query has too; without qo_indptr (one token each) it always holds
+  const bool uniform = p.batch * per_seq <= 2 * bound;
   const int64_t tiles = uniform ? p.batch * per_seq : bound;
   *units = tiles * p.kv_heads;
   if (*units > 0x7fffffff / 16) return fail(QR_EUNSUPPORTED, "qr_kv_attend_i4: too many tiles");

@@ -256,3 +256,24 @@ def test_single_tokens_of_a_refused_sequence(window, group):
     for bad in (positions[:2], positions.long(), positions.cpu()):
         with pytest.raises(RuntimeError):
             KV.batch_decode_i4(o, s["q"].to(DEV), *args, window=window, positions=bad)
+
+
+# ------------------------------------------------------------------ workspace
+@pytest.mark.parametrize("lens,new,heads,group", [
+    ([300] * 64, [1] * 63 + [200], 1, 4), ([600] + [40] * 63, [512] + [1] * 63, 1, 4), ([900] * 20, [300] + [2] * 19, 2, 4),
+    ([1000] * 16, [100] + [1] * 15, 2, 8), ([512] + [300] * 63, [512] + [1] * 63, 2, 8), ([300] * 150, [100] + [1] * 149, 8, 1),
+    ([2000, 30], [90, 1], 1, 1), ([4000], [128], 2, 2), ([200] * 100, [100] + [1] * 99, 2, 8)])
+def test_the_workspace_that_is_asked_for_is_the_one_that_is_used(lens, new, heads, group):
+    """The query and the call make the same plan: bytes are written exactly where some were asked for, and not with one byte
+    less."""
+    s = _setup(lens, new, heads, group, 16, seed=96)
+    need = _need(s, max(new))
+    work = torch.empty(max(need, 1 << 25), dtype=torch.uint8, device=DEV)
+    o = torch.empty_like(s["q"], device=DEV)
+    for size, used in ((need, need > 0), (work.numel(), need > 0), (need - 1, False)):
+        if size < 0:
+            continue
+        work.fill_(0xA5)
+        assert _raw(s, o, max(new), work[:size]) == 0
+        assert bool((work[:max(size, 1)] != 0xA5).any()) == used
+        assert bool((work[need:] == 0xA5).all())
