@@ -277,3 +277,38 @@ def test_the_workspace_that_is_asked_for_is_the_one_that_is_used(lens, new, head
         assert _raw(s, o, max(new), work[:size]) == 0
         assert bool((work[:max(size, 1)] != 0xA5).any()) == used
         assert bool((work[need:] == 0xA5).all())
+
+
+def test_the_tcgen05_kernel_uses_the_workspace_that_it_asks_for(request):
+    _lib.set_tuning("kv_attend", 2)
+    request.addfinalizer(lambda: _lib.set_tuning("kv_attend", 0))
+    s = _setup([3000, 100], [40, 70], 1, 4, 16, seed=97)
+    need = _need(s, 70)
+    assert need > 0
+    o = torch.empty_like(s["q"], device=DEV)
+    for size in (need, need - 1):
+        work = torch.full((need,), 0xA5, dtype=torch.uint8, device=DEV)
+        assert _raw(s, o, 70, work[:size]) == 0
+        assert bool((work != 0xA5).any()) == (size == need)
+
+
+# ------------------------------------------------------------------ long contexts
+@both_kernels
+@pytest.mark.parametrize("lens,new,group,window,sinks", [([70001], [3], 2, 0, 0), ([40000, 66000], [2, 1], 3, 0, 0), ([70001], [9], 1, 65000, 5)])
+def test_contexts_of_many_thousand_tokens(lens, new, group, window, sinks):
+    s = _setup(lens, new, 1, group, 64, seed=98)
+    _check(_attend(s, window, sinks, max_q=max(new)), _oracle(s, window, sinks))
+
+
+@both_kernels
+def test_a_first_token_that_dominates_a_long_context():
+    """Its key is the query's direction: all other tokens share what the softmax leaves them."""
+    s = _setup([20000], [2], 1, 2, 16, seed=99)
+    q = torch.randn(1, 1, 128, generator=torch.Generator().manual_seed(100)).half()
+    s["q"] = (q * torch.tensor([1.0, 0.75, 0.5, 0.25]).view(2, 2, 1)).half()
+    codes, scale, zero = O.kv_asym_quant_pack(q)
+    first = int(s["indices"][0])
+    s["pages"][first, 1, 0, :, 0] = codes[0]
+    s["params"][first, 1, 0, :, 0] = torch.cat((scale, zero), -1)[0]
+    for window, sinks in ((0, 0), (5000, 4)):
+        _check(_attend(s, window, sinks, max_q=2), _oracle(s, window, sinks))
