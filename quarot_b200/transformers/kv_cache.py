@@ -66,8 +66,9 @@ def append_kv_i4(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, k, 
     dev = kv_data.device
     with torch.cuda.device(dev):
         _lib.check(_lib_c.qr_kv_append_i4(
-            kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_offset.data_ptr(),
-            k.data_ptr(), v.data_ptr(), seqlen_indptr.data_ptr() if seqlen_indptr is not None else None,
+            kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(),
+            kv_indices.data_ptr() or kv_indptr.data_ptr(),         # no page at all: not read
+            last_page_offset.data_ptr(), k.data_ptr(), v.data_ptr(), seqlen_indptr.data_ptr() if seqlen_indptr is not None else None,
             tokens, last_page_offset.shape[0], kv_data.shape[1], int(layer_idx), heads, kv_data.shape[4], head_dim,
             1 if hadamard_k else 0, _stream(dev)), "append_kv_i4")
 
@@ -344,17 +345,15 @@ class _AttentionStub(object):
     def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, chunk=None):
         batch_size, q_len, num_qo_heads, head_dim = q.shape
         table = {k: attention_kwargs[k] for k in _TABLE_KEYS}
-        added, qo_indptr, shown = chunk or (1, None, None)
-        assert q_len == added
-        if q_len == 1:
+        if chunk is None:
+            assert q_len == 1
             q = q.reshape(batch_size, num_qo_heads, head_dim).contiguous()
             attn_output = torch.empty_like(q)
             batch_decode_i4(attn_output, q, **table, layer_idx=layer_idx, hadamard_q=self.hadamard_dtype is not None,
                             window=self.window_size, sink_tokens=self.sink_tokens)
-            if shown is not None:               # a token that the mask hides gives zeros
-                attn_output.masked_fill_(~shown.view(batch_size, 1, 1), 0)
             return attn_output.unsqueeze(1)
-        keep = shown.flatten() if shown is not None else None
+        added, qo_indptr, keep = chunk
+        assert q_len == added
         rows = q.reshape(batch_size * q_len, num_qo_heads, head_dim)
         rows = (rows if keep is None else rows[keep]).contiguous()
         attn_output = torch.empty_like(rows)
@@ -423,16 +422,18 @@ class MultiLayerPagedKVCache4Bit:
         had = self.hadamard_dtype is not None
         k = key_states.reshape(b_sz * added_length, num_heads, head_dim)
         v = value_states.reshape(b_sz * added_length, num_heads, head_dim)
-        if attention_mask is None and not self._needs_init[layer_idx] and added_length == 1:
-            specs = self.get_cache_specs_for_flash_infer(None)
-            append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
-                         specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx, hadamard_k=had)
-            return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
         shown = None
         if attention_mask is not None:
             if 0 < self.length < attention_mask.shape[-1]:          # wider than the tokens so far: the last of these are the new ones
                 attention_mask = attention_mask[:, :self.length]
-            shown = attention_mask[:, -added_length:].bool()
+            shown = attention_mask[:, -added_length:]
+        if not self._needs_init[layer_idx] and added_length == 1:
+            # a sequence whose token the mask hides is empty in the table of this step: nothing is written, and its row is zero
+            specs = self._page_table(attention_mask, only=shown)[0]
+            append_kv_i4(specs["kv_data"], specs["kv_param"], specs["kv_indptr"], specs["kv_indices"],
+                         specs["last_page_offset"], k.contiguous(), v.contiguous(), layer_idx, hadamard_k=had)
+            return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
+        if shown is not None:
             new_lens = shown.sum(dim=-1, dtype=torch.int32)
         else:
             new_lens = torch.full((b_sz,), added_length, dtype=torch.int32, device=self.device)
@@ -441,7 +442,8 @@ class MultiLayerPagedKVCache4Bit:
         if shown is not None:
             # the map holds the tokens that the mask shows one behind the other; the others are not cached
             at = table["append_indptr"][:-1, None] + torch.cumsum(shown, 1, dtype=torch.int32) - 1
-            slots = slots[at.clamp(min=0)].masked_fill(~shown, -1).flatten()
+            shown = shown.bool().flatten()
+            slots = slots.index_select(0, at.clamp(min=0).flatten()).masked_fill(~shown, -1)
         append_kv_slots_i4(self.pages, self.scales, slots, _as_rows(k), _as_rows(v), layer_idx, hadamard_k=had)
         if self._needs_init[layer_idx]:
             self._needs_init[layer_idx] = False
@@ -449,14 +451,16 @@ class MultiLayerPagedKVCache4Bit:
         return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
                                  chunk=(added_length, table["append_indptr"], shown))
 
-    def _page_table(self, attention_mask, new_lens=None, new_tokens=0):
+    def _page_table(self, attention_mask, new_lens=None, new_tokens=0, only=None):
         """Page table of the cached tokens as the kernels take it (sequence b owns pages b, b + batch, b + 2 batch, ...), and
         with it where a step's tokens go, as build_page_table gives it.  new_lens: how many of the tokens the step adds (None:
-        none, they are cached already), new_tokens: rows of the slot map."""
+        none, they are cached already), new_tokens: rows of the slot map.  only [batch, 1]: sequences with a 0 are left empty."""
         if attention_mask is not None:
             seqlens = attention_mask.sum(dim=-1, dtype=torch.int32)
         else:
             seqlens = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self.device)
+        if only is not None:
+            seqlens.masked_fill_(only[:, 0] == 0, 0)
         most = self.length if attention_mask is None else max(self.length, attention_mask.shape[-1])
         # a mask may claim more tokens than the pool holds; what is listed lies in the pool
         blocks = max(min(self.page_cnt_from_length(most), self.pages.shape[0] // self.batch_size), 1)
