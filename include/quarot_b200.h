@@ -256,7 +256,8 @@ int qr_linear_i4_f16_static(const uint8_t* A, const void* sA, const uint8_t* B, 
  * scale), 0, 15), every step rounded to fp16 as the torch reference does) -> pack -> write into the page slots, for k
  * and v [tokens, heads, head_dim] fp16.  The page table must already describe the sequences WITH the new tokens;
  * append_indptr [batch + 1] gives the new tokens per sequence (a prompt), NULL means one token per sequence
- * (tokens == batch).  One kernel for matmul_had_cuda + asym_quantize_and_pack_i4 (quarot/transformers/kv_cache.py:10-35)
+ * (tokens == batch).  New tokens that the sequence, as the table has it, is too short for are left out (all of them where it
+ * has no page).  One kernel for matmul_had_cuda + asym_quantize_and_pack_i4 (quarot/transformers/kv_cache.py:10-35)
  * + init_kv_i4 / append_kv_i4 (quarot/kernels/bindings.cpp:140-260, flashinfer/page.cuh:120,167). */
 int qr_kv_append_i4(void* kv_data, void* kv_param, const int32_t* kv_indptr, const int32_t* kv_indices,
                     const int32_t* last_page_offset, const void* k, const void* v, const int32_t* append_indptr,

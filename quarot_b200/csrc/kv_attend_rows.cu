@@ -14,7 +14,8 @@
 //   l = sum w / s'_t  (the softmax denominator),   y = sum w (z'_t / s'_t - 7.5),   o = (sum w~ c' - 7.5 sum w~ - y) / l,
 // so that a cut of weight t moves the result by its difference from v_t - o only (a row that looks at one token has
 // nothing of it) and their common part not at all.  l and y are fp32 sums of w; w~ (the B operand) differs from w below
-// 2^-14 of the largest, by at most 2^-25, and meets the centred codes c' - 7.5 with it (sum w~: one more MMA row of ones).
+// 2^-14 of the largest, by at most 2^-25, and meets the centred codes c' - 7.5 with it (sum w~: one more MMA row of ones):
+// next to a token with the weight 1, one below 2^-25 has its share of the softmax and its centre, but not its codes.
 //
 // Mapping.  A warp takes blocks of 32 tokens.  Scores: S^T = K Q^T with mma.m16n8k16, 16 tokens as M, 8 rows as N; lane
 // (g, c) = (lane / 4, lane % 4) reads 16 bytes of each of its token rows (32 codes), and since the order of the 128
@@ -540,6 +541,8 @@ int kv_pick_splits(int which, const void* kernel, int threads, size_t smem, int6
     // (instructions); of two, one takes 0.6 of it (latency); an SM is not faster with fewer than it could hold in all.
     const int64_t load = (units * per_sm + fit - 1) / fit;
     // Clusters start as a whole: in several rounds of two CTAs per SM that costs some 15 % more.
+    // With these two against neither, units x tokens, us: 192 x 1000 31 -> 20, 512 x 4000 132 -> 108; where several rounds of
+    // long units run the rule is not borne out: 192 x 16000 170 -> 187, 320 x 16000 270 -> 309.
     double rounds = load <= per_sm ? 1.0 : (double)load / per_sm;
     if (per_sm == 2 && load > 2) rounds = ((double)(load / 2) + 0.6 * (double)(load % 2)) * (s > 1 ? 1.15 : 1.0);
     const double cost = rounds * (1.0 / s + (s > 1 ? joined : alone));

@@ -17,7 +17,9 @@
 // M does not follow the maximum: it is set 1 below the first one and moves, in whole steps, only where a weight would pass
 // 2^15 (all rows of the warp that have grown by 2 move then; what is summed up in tensor memory is multiplied through, by
 // powers of two, which round nothing).  So weights are made in one pass, without looking for a maximum first, and the
-// normal fp16 range reaches down to 2^-14 of the first largest or further.
+// normal fp16 range reaches down to 2^-14 of the first largest or further.  The fp16 range ends below: a weight under 2^-25
+// of the reference's unit is 0 in all sums, so that next to one token that dominates by as much, n such tokens lose up to
+// n 2^-25 of the softmax (2^-9 for 65536 of them).
 //
 // S is made and used in halves of 48 tokens with a buffer each, the weights lie over the half of S they came from: while
 // the softmax is on one half, the tensor cores make the products of the other and then its next scores.

@@ -10,7 +10,7 @@ int4 quantisation, packing and the write into the page slot, for prompt and sing
 Beyond upstream: `build_page_table` (page table and slot map from request lengths, on the GPU), `append_kv_slots_i4` (the
 append that takes that slot map), `chunk_attention_i4` (causal attention of several new tokens per sequence, ragged, with
 grouped query heads), and a sliding window with sink tokens for chunks and single tokens.  The cache class uses them for
-chunks after the prompt, for sequences of different page counts and with `window_size` / `sink_tokens`.
+prompts and chunks, for sequences of different page counts and with `window_size` / `sink_tokens`.
 
 Not built: `disable_quant=True` (the fp16 variant of the cache) raises NotImplementedError.
 """
@@ -285,7 +285,8 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
     """o[b, h] = softmax(q[b, h] K^T / sqrt(d)) V over the packed pages, one new token per sequence
     (quarot/transformers/kv_cache.py:64-72); with hadamard_q the query is Hadamard-transformed first.  With a window only
     the last `window` tokens and the first sink_tokens are seen; the query may have a multiple of the cache's heads.
-    positions as in chunk_attention_i4."""
+    positions as in chunk_attention_i4.  With a window or shared heads the softmax weights have 11 bits, as chunks have them,
+    without these they are fp32."""
     shape = q.shape
     _check_positions("batch_decode_i4", q, positions)
     if window is not None or len(shape) == 3 and shape[1] != kv_data.shape[3]:
